@@ -444,6 +444,135 @@ J1_API j1_status j1_op_attention_noalloc(const void* qkv, int64_t t, int32_t hid
                                          const uint32_t* seq_lens, size_t nseq, int32_t window, void* ctx,
                                          void* stream, int sync);
 
+/* ---- the feed-forward block for training and serving (no reference counterpart)
+ * Row-major matrices of 16-bit elements on device memory, one token per row; `ld*` are row
+ * strides in elements (>= the row's width, any alignment of a whole element; rows that start
+ * on 16-byte boundaries take the faster path). Any M >= 0, N >= 1, K >= 1. Weights are used as
+ * a checkpoint stores them, [N, K]. Products accumulate in FP32, every epilogue works on the
+ * unrounded FP32 values, each result is rounded once. Biases and their gradients are FP32.
+ *
+ * All pointers of a call must be memory of the calling thread's current device, and `stream`
+ * a stream of it (NULL: its default stream); other pointers give J1_ERR_INVALID_ARG. Results
+ * must not overlap each other or any input, except that j1_op_linear's out may be its residual
+ * (same pointer and row stride). Elements between a row's width and its stride are neither
+ * read nor written. With sync = 0 the calls only enqueue work and may be captured into a CUDA
+ * graph; the first call of each kind on a device loads its kernels and should come before any
+ * capture. Nothing is allocated. Device-side timeouts of sync = 0 calls are reported by the
+ * next of these calls made with sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Equal
+ * inputs give equal bits: no result depends on the order in which blocks finish. */
+typedef enum j1_dtype { J1_DTYPE_BF16 = 0, J1_DTYPE_FP16 = 1 } j1_dtype;
+typedef enum j1_act {
+  J1_ACT_NONE = 0,
+  J1_ACT_RELU = 1,
+  J1_ACT_GELU = 2,      /* p Phi(p) (erf) */
+  J1_ACT_GELU_TANH = 3, /* 0.5 p (1 + tanh(sqrt(2/pi) (p + 0.044715 p^3))) */
+  J1_ACT_SILU = 4       /* p / (1 + exp(-p)) */
+} j1_act;
+
+/* p = x w^T + bias; out = act(p) + residual; pre (optional) = p, rounded, for the backward. */
+typedef struct j1_linear_args {
+  int32_t dtype;         /* j1_dtype of x, w, residual, out, pre */
+  int32_t act;           /* j1_act */
+  int32_t M, N, K;
+  const void* x;         /* [M, K] */
+  int64_t ldx;
+  const void* w;         /* [N, K] */
+  int64_t ldw;
+  const float* bias;     /* [N] or NULL */
+  const void* residual;  /* [M, N] or NULL */
+  int64_t ldr;
+  void* out;             /* [M, N] */
+  int64_t ldo;
+  void* pre;             /* [M, N] or NULL */
+  int64_t ldp;
+} j1_linear_args;
+J1_API j1_status j1_op_linear(const j1_linear_args* args, void* stream, int sync);
+
+/* Gradients of j1_op_linear: dp = dout * act'(pre); dx = dp w; dw = dp^T x; dbias = sum of dp
+ * over rows. dx, dw and dbias are written, not added to; each may be NULL (not wanted), not
+ * all three. x is read for dw only, w for dx only, pre unless act is J1_ACT_NONE (where dp =
+ * dout); what is not read may be NULL. dp is rounded to the dtype before the two products,
+ * dbias sums the unrounded values. The residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
+ * workspace: at least j1_op_linear_backward_workspace bytes, 256-byte aligned; its contents
+ * need not survive between calls, and calls that may overlap on the GPU need one each. */
+typedef struct j1_linear_grad_args {
+  int32_t dtype, act;
+  int32_t M, N, K;
+  const void* dout;  /* [M, N] */
+  int64_t lddo;
+  const void* x;     /* [M, K] */
+  int64_t ldx;
+  const void* w;     /* [N, K] */
+  int64_t ldw;
+  const void* pre;   /* [M, N], as j1_op_linear stored it */
+  int64_t ldp;
+  void* dx;          /* [M, K] */
+  int64_t lddx;
+  void* dw;          /* [N, K] */
+  int64_t lddw;
+  float* dbias;      /* [N] */
+  void* workspace;
+  size_t workspace_bytes;
+} j1_linear_grad_args;
+J1_API j1_status j1_op_linear_backward(const j1_linear_grad_args* args, void* stream, int sync);
+/* Host only. Enough for every dtype, act, set of gradients and row stride of these sizes. */
+J1_API j1_status j1_op_linear_backward_workspace(int32_t M, int32_t N, int32_t K, size_t* bytes);
+
+/* a = x wa^T + ba; g = x wg^T + bg; out = act(a) * g. A checkpoint's Wi [2N, K] is wa = its first N
+ * rows (the activated half) and wg = the others, in place. pre_a, pre_g (both or neither) = a and
+ * g, rounded, for the backward. */
+typedef struct j1_gated_args {
+  int32_t dtype, act;
+  int32_t M, N, K;
+  const void* x;   /* [M, K] */
+  int64_t ldx;
+  const void* wa;  /* [N, K] */
+  int64_t ldwa;
+  const void* wg;  /* [N, K] */
+  int64_t ldwg;
+  const float* ba; /* [N] or NULL */
+  const float* bg; /* [N] or NULL */
+  void* out;       /* [M, N] */
+  int64_t ldo;
+  void* pre_a;     /* [M, N] or NULL */
+  int64_t ldpa;
+  void* pre_g;     /* [M, N] or NULL */
+  int64_t ldpg;
+} j1_gated_args;
+J1_API j1_status j1_op_gated(const j1_gated_args* args, void* stream, int sync);
+
+/* Gradients of j1_op_gated: da = dout * pre_g * act'(pre_a); dg = dout * act(pre_a);
+ * dx = da wa + dg wg; dwa = da^T x; dwg = dg^T x; dba, dbg = sums over rows. Rules as for
+ * j1_op_linear_backward; pre_a and pre_g are always read; dwa and dwg go together. */
+typedef struct j1_gated_grad_args {
+  int32_t dtype, act;
+  int32_t M, N, K;
+  const void* dout;  /* [M, N] */
+  int64_t lddo;
+  const void* x;     /* [M, K] */
+  int64_t ldx;
+  const void* wa;    /* [N, K] */
+  int64_t ldwa;
+  const void* wg;    /* [N, K] */
+  int64_t ldwg;
+  const void* pre_a; /* [M, N] */
+  int64_t ldpa;
+  const void* pre_g; /* [M, N] */
+  int64_t ldpg;
+  void* dx;          /* [M, K] */
+  int64_t lddx;
+  void* dwa;         /* [N, K] */
+  int64_t lddwa;
+  void* dwg;         /* [N, K] */
+  int64_t lddwg;
+  float* dba;        /* [N] */
+  float* dbg;        /* [N] */
+  void* workspace;
+  size_t workspace_bytes;
+} j1_gated_grad_args;
+J1_API j1_status j1_op_gated_backward(const j1_gated_grad_args* args, void* stream, int sync);
+J1_API j1_status j1_op_gated_backward_workspace(int32_t M, int32_t N, int32_t K, size_t* bytes);
+
 /* Host helper: dst rows of a [2*inter, K] Wi laid out for J1_EPI_GEGLU (FP32 -> BF16 on device). */
 J1_API j1_status j1_op_geglu_interleave(const float* src_dev, void* dst_dev, int32_t inter, int32_t k, void* stream);
 

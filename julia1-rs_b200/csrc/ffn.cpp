@@ -1,0 +1,417 @@
+// j1_op_linear, j1_op_gated and their backward passes: argument checks, workspace layout and
+// the launches. Everything here runs on the host; no call allocates device memory.
+#include <climits>
+#include <cstdint>
+#include <mutex>
+#include <string>
+
+#include "ffn.h"
+#include "model.h"
+
+using namespace j1rt;
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+constexpr int kMaxDim = 1 << 30;
+
+// The operators' error word (0: no timed-out wait), one per device: a file-scope array, so that
+// no call allocates (a call may be captured, or a pool may own all of the device's memory).
+struct FfnDevice {
+  std::once_flag once;
+  cudaError_t rc = cudaSuccess;
+  int* err = nullptr;
+  int num_sms = 0;
+};
+FfnDevice g_dev[kMaxDevices];
+
+j1_status device_state(FfnDevice** out, int* ordinal) {
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_error(e, "cudaGetDevice");
+  if (dev < 0 || dev >= kMaxDevices) return set_error(J1_ERR_UNSUPPORTED, "device ordinal above 63");
+  FfnDevice& s = g_dev[dev];
+  std::call_once(s.once, [&s, dev] {
+    s.rc = ffn_error_word(&s.err);
+    if (s.rc == cudaSuccess) s.rc = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
+  });
+  if (s.rc != cudaSuccess) return cuda_error(s.rc, "error word");
+  *out = &s;
+  *ordinal = dev;
+  return J1_OK;
+}
+
+// One matrix (or vector) argument of a call.
+struct Arg {
+  const char* name;
+  const void* p;
+  int64_t rows, cols, ld;
+  int elem;  // bytes
+  bool write;
+  uint64_t lo() const { return reinterpret_cast<uintptr_t>(p); }
+  uint64_t hi() const {
+    return rows && cols ? lo() + (static_cast<uint64_t>(rows - 1) * ld + cols) * elem : lo();
+  }
+};
+
+j1_status bad(const std::string& msg) { return set_error(J1_ERR_INVALID_ARG, msg); }
+
+// Whether two arguments share memory. Matrices of one row stride whose columns are apart (two
+// halves of the rows of one buffer) do not, although their address ranges interleave.
+bool overlap(const Arg& a, const Arg& b) {
+  if (a.lo() >= b.hi() || b.lo() >= a.hi()) return false;
+  if (a.ld != b.ld || a.elem != b.elem || a.rows < 2 || b.rows < 2) return true;
+  const uint64_t row = static_cast<uint64_t>(a.ld) * a.elem;
+  const uint64_t d = a.lo() <= b.lo() ? (b.lo() - a.lo()) % row : (row - (a.lo() - b.lo()) % row) % row;
+  return d < static_cast<uint64_t>(a.cols) * a.elem || d + static_cast<uint64_t>(b.cols) * b.elem > row;
+}
+
+// Host checks of a call's sizes and matrices: strides, alignment, overlaps. `same`: index of an
+// input that the output `same_out` may coincide with.
+j1_status check_args(int dtype, int act, int M, int N, int K, const Arg* a, int n, int same = -1, int same_out = -1) {
+  if (dtype != J1_DTYPE_BF16 && dtype != J1_DTYPE_FP16) return bad("unknown dtype");
+  if (act < J1_ACT_NONE || act > J1_ACT_SILU) return bad("unknown activation");
+  if (M < 0 || N <= 0 || K <= 0) return bad("M must be >= 0, N and K positive");
+  if (M > kMaxDim || N > kMaxDim || K > kMaxDim) return set_error(J1_ERR_UNSUPPORTED, "sizes above 2^30");
+  for (int i = 0; i < n; ++i) {
+    if (!a[i].p) continue;
+    if (a[i].ld < a[i].cols) return bad(std::string(a[i].name) + ": row stride below the row's width");
+    if (a[i].ld > (int64_t(1) << 38)) return set_error(J1_ERR_UNSUPPORTED, std::string(a[i].name) + ": row stride above 2^38");
+    if (a[i].lo() % a[i].elem) return bad(std::string(a[i].name) + ": not aligned to its element type");
+  }
+  for (int i = 0; i < n; ++i) {
+    if (!a[i].p || !a[i].write) continue;
+    for (int j = 0; j < n; ++j) {
+      if (j == i || !a[j].p || (a[j].write && j < i)) continue;
+      if (i == same_out && j == same && a[i].p == a[j].p && a[i].ld == a[j].ld) continue;
+      if (overlap(a[i], a[j]))
+        return bad(std::string(a[i].name) + " overlaps " + a[j].name);
+    }
+  }
+  return J1_OK;
+}
+
+// Every pointer must be device memory of the current device.
+j1_status check_device(const Arg* a, int n, int device) {
+  for (int i = 0; i < n; ++i) {
+    if (!a[i].p || !a[i].rows) continue;
+    cudaPointerAttributes at;
+    const cudaError_t e = cudaPointerGetAttributes(&at, a[i].p);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_error(e, a[i].name);
+    }
+    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+      return bad(std::string(a[i].name) + " is not device memory");
+    if (at.type == cudaMemoryTypeDevice && at.device != device)
+      return bad(std::string(a[i].name) + " is on device " + std::to_string(at.device) + ", the current device is " +
+                 std::to_string(device));
+  }
+  return J1_OK;
+}
+
+j1_status finish(FfnDevice* d, cudaStream_t st, int sync) {
+  if (!sync) return J1_OK;
+  cudaError_t e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return cuda_error(e, "op");
+  int w = 0;
+  e = cudaMemcpyAsync(&w, d->err, 4, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e != cudaSuccess) return cuda_error(e, "op error word");
+  if (w) {
+    e = cudaMemsetAsync(d->err, 0, 4, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    return set_error(J1_ERR_DEVICE_TIMEOUT, "device-side wait timed out (site " + std::to_string(w >> 16) + ")");
+  }
+  return J1_OK;
+}
+
+FfnGemm gemm_for(int dtype, int layout, int M, int N, int K, const FfnDevice* d) {
+  FfnGemm g = {};
+  g.fp16 = dtype == J1_DTYPE_FP16;
+  g.layout = layout;
+  g.act = J1_ACT_NONE;
+  g.M = M, g.N = N, g.K = K;
+  g.segs = 1;
+  g.row1 = g.rows0 = INT_MAX;
+  g.err = d->err;
+  g.num_sms = d->num_sms;
+  return g;
+}
+
+// ---- backward workspace: gradients at the pre-activations (rows padded to 32 elements; the
+// gated pair side by side), slab sums of the bias gradients, partial products of dw.
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+int pad32(int n) { return (n + 31) / 32 * 32; }
+struct Workspace {
+  size_t grads, sums, partials, bytes;  // offsets of the three parts, total
+  size_t partial_bytes;
+  long long ld;  // of the gradients
+};
+Workspace workspace_for(int M, int N, int K, int projections) {
+  Workspace w;
+  w.ld = static_cast<long long>(projections) * pad32(N);
+  w.grads = 0;
+  w.sums = up256(static_cast<size_t>(M) * w.ld * 2);
+  w.partials = w.sums + up256(static_cast<size_t>(ffn_grad_slabs(M, N)) * projections * N * 4);
+  w.partial_bytes = ffn_partial_bytes(projections * pad32(N), K, M);
+  w.bytes = w.partials + up256(w.partial_bytes);
+  return w;
+}
+
+j1_status workspace_query(int M, int N, int K, int projections, size_t* bytes) {
+  if (!bytes) return bad("NULL argument");
+  if (M < 0 || N <= 0 || K <= 0) return bad("M must be >= 0, N and K positive");
+  if (M > kMaxDim || N > kMaxDim || K > kMaxDim) return set_error(J1_ERR_UNSUPPORTED, "sizes above 2^30");
+  *bytes = workspace_for(M, N, K, projections).bytes;
+  return J1_OK;
+}
+
+j1_status check_workspace(const void* p, size_t bytes, size_t need) {
+  if (bytes < need || (need && !p))
+    return bad("workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " needed");
+  if (reinterpret_cast<uintptr_t>(p) % 256) return bad("workspace must be 256-byte aligned");
+  return J1_OK;
+}
+
+#define FFN_LAUNCH(expr, what)                                             \
+  do {                                                                     \
+    if (take_fault(J1_FAULT_LAUNCH)) return cuda_error(cudaErrorLaunchFailure, what " (injected)"); \
+    const int rc_ = (expr);                                                \
+    if (rc_) return cuda_error(static_cast<cudaError_t>(rc_), what);       \
+  } while (0)
+
+#define FFN_TRY(expr)          \
+  do {                         \
+    const j1_status s_ = (expr); \
+    if (s_) return s_;         \
+  } while (0)
+
+j1_status zero_rows(void* p, int64_t ld, int rows, int cols, size_t elem, cudaStream_t st) {
+  if (!p) return J1_OK;
+  const cudaError_t e = cudaMemset2DAsync(p, ld * elem, 0, static_cast<size_t>(cols) * elem, rows, st);
+  return e == cudaSuccess ? J1_OK : cuda_error(e, "memset");
+}
+
+}  // namespace
+
+extern "C" {
+
+j1_status j1_op_linear(const j1_linear_args* a, void* stream, int sync) {
+  return guard("j1_op_linear", [&]() -> j1_status {
+    if (!a || !a->w || (a->M > 0 && (!a->x || !a->out))) return bad("NULL argument");
+    const Arg args[] = {{"x", a->x, a->M, a->K, a->ldx, 2, false},
+                        {"w", a->w, a->N, a->K, a->ldw, 2, false},
+                        {"bias", a->bias, 1, a->N, a->N, 4, false},
+                        {"residual", a->residual, a->M, a->N, a->ldr, 2, false},
+                        {"out", a->out, a->M, a->N, a->ldo, 2, true},
+                        {"pre", a->pre, a->M, a->N, a->ldp, 2, true}};
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 6, 3, 4));
+    FfnDevice* d;
+    int dev;
+    FFN_TRY(device_state(&d, &dev));
+    FFN_TRY(check_device(args, 6, dev));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->M) {
+      FfnGemm g = gemm_for(a->dtype, FFN_NT, a->M, a->N, a->K, d);
+      g.act = a->act;
+      g.a[0] = {a->x, a->ldx};
+      g.b[0] = {a->w, a->ldw};
+      g.bias[0] = a->bias;
+      g.residual = {a->residual, a->ldr};
+      g.out[0] = {a->out, a->ldo};
+      g.pre[0] = {a->pre, a->ldp};
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "linear launch");
+    }
+    return finish(d, st, sync);
+  });
+}
+
+j1_status j1_op_gated(const j1_gated_args* a, void* stream, int sync) {
+  return guard("j1_op_gated", [&]() -> j1_status {
+    if (!a || !a->wa || !a->wg || (a->M > 0 && (!a->x || !a->out))) return bad("NULL argument");
+    if (!a->pre_a != !a->pre_g) return bad("pre_a and pre_g go together");
+    const Arg args[] = {{"x", a->x, a->M, a->K, a->ldx, 2, false},
+                        {"wa", a->wa, a->N, a->K, a->ldwa, 2, false},
+                        {"wg", a->wg, a->N, a->K, a->ldwg, 2, false},
+                        {"ba", a->ba, 1, a->N, a->N, 4, false},
+                        {"bg", a->bg, 1, a->N, a->N, 4, false},
+                        {"out", a->out, a->M, a->N, a->ldo, 2, true},
+                        {"pre_a", a->pre_a, a->M, a->N, a->ldpa, 2, true},
+                        {"pre_g", a->pre_g, a->M, a->N, a->ldpg, 2, true}};
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 8));
+    FfnDevice* d;
+    int dev;
+    FFN_TRY(device_state(&d, &dev));
+    FFN_TRY(check_device(args, 8, dev));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->M) {
+      FfnGemm g = gemm_for(a->dtype, FFN_NT, a->M, a->N, a->K, d);
+      g.gated = 1;
+      g.act = a->act;
+      g.a[0] = {a->x, a->ldx};
+      g.b[0] = {a->wa, a->ldwa};
+      g.b[1] = {a->wg, a->ldwg};
+      g.bias[0] = a->ba;
+      g.bias[1] = a->bg;
+      g.out[0] = {a->out, a->ldo};
+      g.pre[0] = {a->pre_a, a->ldpa};
+      g.pre[1] = {a->pre_g, a->ldpg};
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "gated launch");
+    }
+    return finish(d, st, sync);
+  });
+}
+
+j1_status j1_op_linear_backward_workspace(int32_t M, int32_t N, int32_t K, size_t* bytes) {
+  return guard("j1_op_linear_backward_workspace", [&]() -> j1_status { return workspace_query(M, N, K, 1, bytes); });
+}
+j1_status j1_op_gated_backward_workspace(int32_t M, int32_t N, int32_t K, size_t* bytes) {
+  return guard("j1_op_gated_backward_workspace", [&]() -> j1_status { return workspace_query(M, N, K, 2, bytes); });
+}
+
+j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int sync) {
+  return guard("j1_op_linear_backward", [&]() -> j1_status {
+    if (!a || (a->M > 0 && !a->dout)) return bad("NULL argument");
+    if (!a->dx && !a->dw && !a->dbias && a->M > 0) return bad("no gradient wanted");
+    if (a->dw && !a->x && a->M > 0) return bad("dw needs x");
+    if (a->dx && !a->w) return bad("dx needs w");
+    if (a->act != J1_ACT_NONE && !a->pre && a->M > 0) return bad("pre is NULL");
+    const bool slope = a->act != J1_ACT_NONE;
+    const Arg args[] = {{"dout", a->dout, a->M, a->N, a->lddo, 2, false},
+                        {"x", a->dw ? a->x : nullptr, a->M, a->K, a->ldx, 2, false},
+                        {"w", a->dx ? a->w : nullptr, a->N, a->K, a->ldw, 2, false},
+                        {"pre", slope ? a->pre : nullptr, a->M, a->N, a->ldp, 2, false},
+                        {"dx", a->dx, a->M, a->K, a->lddx, 2, true},
+                        {"dw", a->dw, a->N, a->K, a->lddw, 2, true},
+                        {"dbias", a->dbias, 1, a->N, a->N, 4, true},
+                        {"workspace", a->workspace, 1, static_cast<int64_t>(a->workspace_bytes),
+                         static_cast<int64_t>(a->workspace_bytes), 1, true}};
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 8));
+    const Workspace ws = workspace_for(a->M, a->N, a->K, 1);
+    FFN_TRY(check_workspace(a->workspace, a->workspace_bytes, ws.bytes));
+    FfnDevice* d;
+    int dev;
+    FFN_TRY(device_state(&d, &dev));
+    FFN_TRY(check_device(args, 8, dev));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->M == 0) {
+      FFN_TRY(zero_rows(a->dw, a->lddw, a->N, a->K, 2, st));
+      FFN_TRY(zero_rows(a->dbias, a->N, 1, a->N, 4, st));
+      return finish(d, st, sync);
+    }
+    uint8_t* base = static_cast<uint8_t*>(a->workspace);
+    FfnMat dp = {a->dout, a->lddo};
+    const bool products = a->dx || a->dw;
+    if ((slope && products) || a->dbias) {
+      FfnGrad k = {};
+      k.fp16 = a->dtype == J1_DTYPE_FP16;
+      k.act = a->act;
+      k.M = a->M, k.N = a->N;
+      k.dout = {a->dout, a->lddo};
+      k.p0 = {slope ? a->pre : nullptr, a->ldp};
+      if (slope && products) k.d0 = dp = {base + ws.grads, ws.ld};
+      k.sum0 = a->dbias;
+      k.partials = reinterpret_cast<float*>(base + ws.sums);
+      FFN_LAUNCH(launch_ffn_grad(k, st), "linear gradient launch");
+    }
+    if (a->dx) {
+      FfnGemm g = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d);
+      g.a[0] = dp;
+      g.b[0] = {a->w, a->ldw};
+      g.out[0] = {a->dx, a->lddx};
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "dx launch");
+    }
+    if (a->dw) {
+      FfnGemm g = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
+      g.a[0] = dp;
+      g.b[0] = {a->x, a->ldx};
+      g.out[0] = {a->dw, a->lddw};
+      g.partials = reinterpret_cast<float*>(base + ws.partials);
+      g.partial_bytes = ws.partial_bytes;
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "dw launch");
+    }
+    return finish(d, st, sync);
+  });
+}
+
+j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sync) {
+  return guard("j1_op_gated_backward", [&]() -> j1_status {
+    if (!a || (a->M > 0 && (!a->dout || !a->pre_a || !a->pre_g))) return bad("NULL argument");
+    if (!a->dwa != !a->dwg) return bad("dwa and dwg go together");
+    if (!a->dx && !a->dwa && !a->dba && !a->dbg && a->M > 0) return bad("no gradient wanted");
+    if (a->dwa && !a->x && a->M > 0) return bad("dwa and dwg need x");
+    if (a->dx && (!a->wa || !a->wg)) return bad("dx needs wa and wg");
+    const Arg args[] = {{"dout", a->dout, a->M, a->N, a->lddo, 2, false},
+                        {"x", a->dwa ? a->x : nullptr, a->M, a->K, a->ldx, 2, false},
+                        {"wa", a->dx ? a->wa : nullptr, a->N, a->K, a->ldwa, 2, false},
+                        {"wg", a->dx ? a->wg : nullptr, a->N, a->K, a->ldwg, 2, false},
+                        {"pre_a", a->pre_a, a->M, a->N, a->ldpa, 2, false},
+                        {"pre_g", a->pre_g, a->M, a->N, a->ldpg, 2, false},
+                        {"dx", a->dx, a->M, a->K, a->lddx, 2, true},
+                        {"dwa", a->dwa, a->N, a->K, a->lddwa, 2, true},
+                        {"dwg", a->dwg, a->N, a->K, a->lddwg, 2, true},
+                        {"dba", a->dba, 1, a->N, a->N, 4, true},
+                        {"dbg", a->dbg, 1, a->N, a->N, 4, true},
+                        {"workspace", a->workspace, 1, static_cast<int64_t>(a->workspace_bytes),
+                         static_cast<int64_t>(a->workspace_bytes), 1, true}};
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 12));
+    const Workspace ws = workspace_for(a->M, a->N, a->K, 2);
+    FFN_TRY(check_workspace(a->workspace, a->workspace_bytes, ws.bytes));
+    FfnDevice* d;
+    int dev;
+    FFN_TRY(device_state(&d, &dev));
+    FFN_TRY(check_device(args, 12, dev));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->M == 0) {
+      FFN_TRY(zero_rows(a->dwa, a->lddwa, a->N, a->K, 2, st));
+      FFN_TRY(zero_rows(a->dwg, a->lddwg, a->N, a->K, 2, st));
+      FFN_TRY(zero_rows(a->dba, a->N, 1, a->N, 4, st));
+      FFN_TRY(zero_rows(a->dbg, a->N, 1, a->N, 4, st));
+      return finish(d, st, sync);
+    }
+    uint8_t* base = static_cast<uint8_t*>(a->workspace);
+    const int np = pad32(a->N);
+    FfnGrad k = {};
+    k.fp16 = a->dtype == J1_DTYPE_FP16;
+    k.gated = 1;
+    k.act = a->act;
+    k.M = a->M, k.N = a->N;
+    k.dout = {a->dout, a->lddo};
+    k.p0 = {a->pre_a, a->ldpa};
+    k.p1 = {a->pre_g, a->ldpg};
+    if (a->dx || a->dwa) {
+      k.d0 = {base + ws.grads, ws.ld};
+      k.d1 = {base + ws.grads + static_cast<size_t>(np) * 2, ws.ld};
+    }
+    k.sum0 = a->dba;
+    k.sum1 = a->dbg;
+    k.partials = reinterpret_cast<float*>(base + ws.sums);
+    FFN_LAUNCH(launch_ffn_grad(k, st), "gated gradient launch");
+    if (a->dx) {
+      FfnGemm g = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d);
+      g.segs = 2;
+      g.a[0] = k.d0;
+      g.a[1] = k.d1;
+      g.b[0] = {a->wa, a->ldwa};
+      g.b[1] = {a->wg, a->ldwg};
+      g.out[0] = {a->dx, a->lddx};
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "dx launch");
+    }
+    if (a->dwa) {  // both weights' gradients as one product: rows [0, np) of da | dg are dwa's
+      FfnGemm g = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
+      g.rows0 = a->N;
+      g.row1 = np;
+      g.a[0] = k.d0;
+      g.b[0] = {a->x, a->ldx};
+      g.out[0] = {a->dwa, a->lddwa};
+      g.out[1] = {a->dwg, a->lddwg};
+      g.partials = reinterpret_cast<float*>(base + ws.partials);
+      g.partial_bytes = ws.partial_bytes;
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "dw launch");
+    }
+    return finish(d, st, sync);
+  });
+}
+
+}  // extern "C"

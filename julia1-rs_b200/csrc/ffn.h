@@ -1,0 +1,66 @@
+// Internal launch interface of the feed-forward operators (j1_op_linear, j1_op_gated and their
+// backward passes): ffn.cpp checks arguments and plans, the .cu files launch.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace j1rt {
+
+// A row-major matrix of 16-bit elements: row r starts at p + r * ld elements.
+struct FfnMat {
+  const void* p;
+  long long ld;
+};
+
+// How the operands of out[M, N] = A . B lie in memory (K: the contraction).
+enum FfnLayout : int {
+  FFN_NT = 0,  // A [M, K], B [N, K]: forward
+  FFN_NN = 1,  // A [M, K], B [K, N]: dx = dp . w
+  FFN_TN = 2,  // A [K, M], B [K, N]: dw = dp^T . x
+};
+
+struct FfnGemm {
+  int fp16;    // element type: 0 BF16, 1 FP16
+  int layout;  // FfnLayout
+  int gated;   // two B operands, out = act(A B0^T + bias0) * (A B1^T + bias1) (NT)
+  int act;     // j1_act
+  int M, N, K;
+  int segs;    // out = sum over s < segs of A[s] . B[s] (NN: the two halves of a gated dx)
+  int row1;    // TN: output rows >= row1 (a multiple of 32) go to out[1] from its row 0, rows in
+               // [rows0, row1) nowhere; INT_MAX: all to out[0]
+  int rows0;
+  FfnMat a[2], b[2];
+  const float* bias[2];
+  FfnMat residual;  // p NULL: none
+  FfnMat out[2];    // written
+  FfnMat pre[2];    // written; p NULL: not wanted
+  float* partials;  // workspace of split contractions, NULL: never split
+  size_t partial_bytes;
+  int* err;         // device error word
+  int num_sms;
+};
+
+int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream);
+// Workspace that a split contraction of these sizes may take (host arithmetic only).
+size_t ffn_partial_bytes(int M, int N, int K);
+// Device address of the operators' error word on the current device.
+cudaError_t ffn_error_word(int** p);
+
+// dp = dout * act'(pre) (linear), or da = dout * g * act'(a), dg = dout * act(a) (gated): the
+// gradients at the pre-activations, rounded to the element type, with the column sums of the
+// unrounded values. d0 (and d1) may be NULL (sums only); sums may be NULL.
+struct FfnGrad {
+  int fp16, gated, act;
+  int M, N;
+  FfnMat dout, p0, p1;  // p0: pre / pre_a (NULL p: act NONE), p1: pre_g
+  FfnMat d0, d1;        // written: dp / da, dg
+  float* sum0;          // [N] or NULL
+  float* sum1;
+  float* partials;      // ffn_grad_slabs(M, N) * 2 * N floats when a sum is wanted
+};
+int ffn_grad_slabs(int M, int N);
+int launch_ffn_grad(const FfnGrad& g, cudaStream_t stream);
+
+}  // namespace j1rt

@@ -39,11 +39,15 @@ EXPORTS = [
     "j1_text_encoder_clear_cache", "j1_text_encoder_options", "j1_text_encoder_tokenize", "j1_text_encoder_encode",
     "j1_text_encoder_request_tokens", "j1_text_encoder_encode_batch", "j1_engine_logits_text", "j1_json_dumps",
     "j1_inject_fault", "j1_selftest_device_timeout",
+    "j1_op_linear", "j1_op_linear_backward", "j1_op_linear_backward_workspace",
+    "j1_op_gated", "j1_op_gated_backward", "j1_op_gated_backward_workspace",
 ]
 FAULT_ALLOC, FAULT_LAUNCH, FAULT_NAN, FAULT_HOST, FAULT_WORKER, FAULT_THREAD, FAULT_DEVICE_WAIT = 1, 2, 3, 4, 5, 6, 7
 PROF_FAMILIES = 12
 
 EPI_BF16, EPI_QKV_ROPE, EPI_GEGLU, EPI_RESID_LN, EPI_RESID, EPI_SCORER = range(6)
+DTYPE_BF16, DTYPE_FP16 = range(2)
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)
 
 
 class J1Error(RuntimeError):
@@ -77,6 +81,36 @@ class J1GemmArgs(C.Structure):
                 ("ldxn", C.c_int32), ("pos", C.c_void_p), ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p),
                 ("rope_cols", C.c_int32), ("w2", C.c_void_p), ("b2", C.c_float), ("scores", C.c_void_p),
                 ("grid_limit", C.c_int32)]
+
+
+def _ffn_fields(*mats, tail=()):
+    """dtype, act, M, N, K, then pointer + row stride pairs; a name with "*" has no stride."""
+    f = [(n, C.c_int32) for n in ("dtype", "act", "M", "N", "K")]
+    short = {"residual": "r", "out": "o", "dout": "do", "pre": "p", "pre_a": "pa", "pre_g": "pg"}
+    for m in mats:
+        f.append((m.strip("*"), C.c_void_p))
+        if not m.endswith("*"):
+            f.append(("ld" + short.get(m, m), C.c_int64))
+    return f + list(tail)
+
+
+_WORKSPACE = (("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t))
+
+
+class J1LinearArgs(C.Structure):
+    _fields_ = _ffn_fields("x", "w", "bias*", "residual", "out", "pre")
+
+
+class J1LinearGradArgs(C.Structure):
+    _fields_ = _ffn_fields("dout", "x", "w", "pre", "dx", "dw", "dbias*", tail=_WORKSPACE)
+
+
+class J1GatedArgs(C.Structure):
+    _fields_ = _ffn_fields("x", "wa", "wg", "ba*", "bg*", "out", "pre_a", "pre_g")
+
+
+class J1GatedGradArgs(C.Structure):
+    _fields_ = _ffn_fields("dout", "x", "wa", "wg", "pre_a", "pre_g", "dx", "dwa", "dwg", "dba*", "dbg*", tail=_WORKSPACE)
 
 
 class J1EncoderOptions(C.Structure):
@@ -239,6 +273,13 @@ def lib():
     L.j1_inject_fault.restype = None
     L.j1_selftest_device_timeout.argtypes = [C.c_int, C.c_int64]
     L.j1_selftest_device_timeout.restype = C.c_int
+    for name, args in (("linear", J1LinearArgs), ("linear_backward", J1LinearGradArgs), ("gated", J1GatedArgs),
+                       ("gated_backward", J1GatedGradArgs)):
+        f = getattr(L, "j1_op_" + name)
+        f.argtypes, f.restype = [C.POINTER(args), C.c_void_p, C.c_int], C.c_int
+    for name in ("linear", "gated"):
+        f = getattr(L, "j1_op_%s_backward_workspace" % name)
+        f.argtypes, f.restype = [C.c_int32] * 3 + [C.POINTER(C.c_size_t)], C.c_int
     L.j1_op_gemm.argtypes = [C.POINTER(J1GemmArgs), C.c_void_p, C.c_int]
     L.j1_op_attention.argtypes = [C.c_void_p, C.c_int64, C.c_int32, u32p, u32p, C.c_size_t, C.c_int32, C.c_void_p,
                                   C.c_void_p, C.c_int]
@@ -1100,3 +1141,118 @@ def op_attention_noalloc(qkv, hidden, seq_starts, seq_lens, window, ctx, stream=
 def op_geglu_interleave(src_f32, dst_bf16, inter, k, stream=None):
     check(lib().j1_op_geglu_interleave(C.c_void_p(src_f32.data_ptr()), C.c_void_p(dst_bf16.data_ptr()), inter, k,
                                        C.c_void_p(stream) if stream else None))
+
+
+# ---- the feed-forward block (include/j1.h, "the feed-forward block for training and serving"):
+# 2-D bf16 or fp16 tensors whose rows are contiguous (any row stride), float32 biases.
+_ffn_dtypes = {}  # torch dtype -> j1_dtype
+
+
+def _ffn_dtype(t):
+    d = _ffn_dtypes.get(t.dtype)
+    if d is None:
+        d = {"torch.bfloat16": DTYPE_BF16, "torch.float16": DTYPE_FP16}.get(str(t.dtype))
+        if d is None:
+            raise J1Error(UNSUPPORTED, "matrices must be bfloat16 or float16, not %s" % t.dtype)
+        _ffn_dtypes[t.dtype] = d
+    return d
+
+
+def _ffn_mat(name, t, rows, cols, dtype):
+    """(pointer, row stride) of a [rows, cols] matrix of `dtype`; None: (None, 0)."""
+    if t is None:
+        return None, 0
+    if t.shape != (rows, cols) or t.dtype != dtype:
+        raise J1Error(INVALID_ARG, "%s: expected %s of shape (%d, %d), got %s of %s" % (
+            name, dtype, rows, cols, t.dtype, tuple(t.shape)))
+    s = t.stride()
+    if s[1] != 1 and cols > 1:
+        raise J1Error(INVALID_ARG, "%s: the elements of a row must be contiguous (strides %s)" % (name, s))
+    return t.data_ptr(), s[0] if rows > 1 else max(s[0], cols)
+
+
+def _ffn_vec(name, t, n):
+    if t is None:
+        return None
+    if t.shape != (n,) or str(t.dtype) != "torch.float32" or (n > 1 and t.stride(0) != 1):
+        raise J1Error(INVALID_ARG, "%s: expected contiguous float32 of shape (%d,), got %s of %s" % (
+            name, n, t.dtype, tuple(t.shape)))
+    return t.data_ptr()
+
+
+def _ffn_sizes(x, w):
+    if x.dim() != 2 or w.dim() != 2:
+        raise J1Error(INVALID_ARG, "matrices must have two dimensions")
+    if max(x.shape[0], w.shape[0], w.shape[1]) > 1 << 30:
+        raise J1Error(UNSUPPORTED, "sizes above 2^30")
+    return x.shape[0], w.shape[0], w.shape[1]
+
+
+def _ffn_workspace(t):
+    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+
+
+def op_linear(x, w, out, bias=None, act=ACT_NONE, residual=None, pre=None, stream=None, sync=True):
+    """out = act(x w^T + bias) + residual; pre (optional) receives x w^T + bias for op_linear_backward.
+    x [M, K], w [N, K], out / residual / pre [M, N] (out may be residual), bias float32 [N]."""
+    M, N, K = _ffn_sizes(x, w)
+    d = x.dtype
+    a = J1LinearArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("x", x, M, K, d), *_ffn_mat("w", w, N, K, d),
+                     _ffn_vec("bias", bias, N), *_ffn_mat("residual", residual, M, N, d),
+                     *_ffn_mat("out", out, M, N, d), *_ffn_mat("pre", pre, M, N, d))
+    check(lib().j1_op_linear(a, stream, 1 if sync else 0))
+
+
+def op_linear_backward_workspace(M, N, K):
+    """Bytes of workspace op_linear_backward needs (any dtype, activation and set of gradients)."""
+    n = C.c_size_t()
+    check(lib().j1_op_linear_backward_workspace(M, N, K, C.byref(n)))
+    return n.value
+
+
+def op_linear_backward(dout, x, w, pre=None, act=ACT_NONE, dx=None, dw=None, dbias=None, workspace=None, stream=None,
+                       sync=True):
+    """Gradients of op_linear, written into those of dx [M, K], dw [N, K], dbias (float32 [N]) that are given.
+    pre: as op_linear stored it (not needed for ACT_NONE). workspace: a CUDA tensor of at least
+    op_linear_backward_workspace(M, N, K) bytes."""
+    M, N, K = _ffn_sizes(x, w)
+    d = x.dtype
+    a = J1LinearGradArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("dout", dout, M, N, d), *_ffn_mat("x", x, M, K, d),
+                         *_ffn_mat("w", w, N, K, d), *_ffn_mat("pre", pre, M, N, d), *_ffn_mat("dx", dx, M, K, d),
+                         *_ffn_mat("dw", dw, N, K, d), _ffn_vec("dbias", dbias, N), *_ffn_workspace(workspace))
+    check(lib().j1_op_linear_backward(a, stream, 1 if sync else 0))
+
+
+def op_gated(x, wa, wg, out, ba=None, bg=None, act=ACT_GELU, pre_a=None, pre_g=None, stream=None, sync=True):
+    """out = act(x wa^T + ba) * (x wg^T + bg); pre_a and pre_g (optional, together) receive the two factors'
+    pre-activations for op_gated_backward. x [M, K], wa / wg [N, K] (e.g. the two halves of a Wi [2N, K]),
+    out / pre_a / pre_g [M, N], ba / bg float32 [N]."""
+    M, N, K = _ffn_sizes(x, wa)
+    d = x.dtype
+    a = J1GatedArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("x", x, M, K, d), *_ffn_mat("wa", wa, N, K, d),
+                    *_ffn_mat("wg", wg, N, K, d), _ffn_vec("ba", ba, N), _ffn_vec("bg", bg, N),
+                    *_ffn_mat("out", out, M, N, d), *_ffn_mat("pre_a", pre_a, M, N, d),
+                    *_ffn_mat("pre_g", pre_g, M, N, d))
+    check(lib().j1_op_gated(a, stream, 1 if sync else 0))
+
+
+def op_gated_backward_workspace(M, N, K):
+    """Bytes of workspace op_gated_backward needs (any dtype, activation and set of gradients)."""
+    n = C.c_size_t()
+    check(lib().j1_op_gated_backward_workspace(M, N, K, C.byref(n)))
+    return n.value
+
+
+def op_gated_backward(dout, x, wa, wg, pre_a, pre_g, act=ACT_GELU, dx=None, dwa=None, dwg=None, dba=None, dbg=None,
+                      workspace=None, stream=None, sync=True):
+    """Gradients of op_gated, written into those of dx [M, K], dwa and dwg [N, K] (together), dba and dbg
+    (float32 [N]) that are given. pre_a, pre_g: as op_gated stored them. workspace: a CUDA tensor of at least
+    op_gated_backward_workspace(M, N, K) bytes."""
+    M, N, K = _ffn_sizes(x, wa)
+    d = x.dtype
+    a = J1GatedGradArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("dout", dout, M, N, d), *_ffn_mat("x", x, M, K, d),
+                        *_ffn_mat("wa", wa, N, K, d), *_ffn_mat("wg", wg, N, K, d),
+                        *_ffn_mat("pre_a", pre_a, M, N, d), *_ffn_mat("pre_g", pre_g, M, N, d),
+                        *_ffn_mat("dx", dx, M, K, d), *_ffn_mat("dwa", dwa, N, K, d), *_ffn_mat("dwg", dwg, N, K, d),
+                        _ffn_vec("dba", dba, N), _ffn_vec("dbg", dbg, N), *_ffn_workspace(workspace))
+    check(lib().j1_op_gated_backward(a, stream, 1 if sync else 0))

@@ -1,0 +1,490 @@
+"""The feed-forward operators against their definitions in float64.
+
+Tolerances are derived, per element, from what the kernels round:
+* a result of type T is rounded once: eps(T) / 2 of its value (and half of fp16's smallest
+  step, 2^-25, where a value is subnormal);
+* a contraction in FP32 of n terms is off by at most (n + 2) 2^-23 of the sum of the terms'
+  magnitudes (2^-23, not 2^-24: tensor cores may cut instead of rounding);
+* an activation is off by at most ACT_ERR |p| and has slope at most 1.13, so it passes 1.13 of
+  its argument's error on; a slope is off by at most SLOPE_ERR (both follow from the errors of
+  one exponential, one reciprocal and, for the erf form, 1.5e-7 of its approximation);
+* backward, the gradients at the pre-activations are rounded to T before the two products.
+"""
+import math
+
+import pytest
+import torch
+
+import julia1 as j1
+
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+ACTS = {"none": j1.ACT_NONE, "relu": j1.ACT_RELU, "gelu": j1.ACT_GELU, "gelu_tanh": j1.ACT_GELU_TANH, "silu": j1.ACT_SILU}
+ACT_ERR, SLOPE_ERR, LIP = 2e-6, 5e-6, 1.13
+
+
+def act64(p, act):
+    f = torch.nn.functional
+    return {"none": lambda v: v, "relu": torch.relu, "gelu": f.gelu, "gelu_tanh": lambda v: f.gelu(v, approximate="tanh"),
+            "silu": f.silu}[act](p)
+
+
+def slope64(p, act):
+    q = p.detach().clone().requires_grad_()
+    return torch.autograd.grad(act64(q, act).sum(), q)[0] if act != "none" else torch.ones_like(p)
+
+
+def unit(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return 2.0 ** -25 if t == HF else 0.0
+
+
+def acc_err(n):
+    return (n + 2) * 2.0 ** -23
+
+
+def mat(rows, cols, dtype, gen=None, std=1.0, pad=0, fill=float("nan")):
+    """A [rows, cols] view of rows that are `pad` longer; what is behind a row holds `fill`."""
+    t = torch.full((rows, cols + pad), fill, device="cuda", dtype=dtype)
+    v = t[:, :cols]
+    if gen is not None:
+        v.copy_(torch.randn((rows, cols), generator=gen, device="cuda") * std)
+    return v
+
+
+def pad_untouched(v, fill=float("nan")):
+    """Nothing was written behind the rows of v (a view of mat())."""
+    base = v._base
+    if base is None or base.shape[1] == v.shape[1]:
+        return True
+    rest = base[:, v.shape[1]:].float()
+    return bool((rest.isnan() if math.isnan(fill) else rest == fill).all())
+
+
+def close(name, got, ref, tol):
+    assert got.shape == ref.shape
+    off = (got.double() - ref).abs()
+    ok = off <= tol
+    assert bool(ok.all()), "%s: %d of %d outside, worst %.3g of its tolerance, |off| %.3g" % (
+        name, int((~ok).sum()), ok.numel(), float((off / tol.clamp_min(1e-300)).max()), float(off.max()))
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def affine64(x, w, b):
+    x, w = x.double(), w.double()
+    p, mag = x @ w.t(), x.abs() @ w.abs().t()
+    if b is not None:
+        p, mag = p + b.double(), mag + b.double().abs()
+    return p, acc_err(x.shape[1]) * mag
+
+
+def check_linear(M, N, K, dtype, act, bias, residual, save, pad=0, seed=0, inplace=False):
+    g = gen(seed)
+    x, w = mat(M, K, dtype, g, 1.0, pad), mat(N, K, dtype, g, K ** -0.5, pad)
+    b = torch.randn(N, generator=g, device="cuda") * 0.5 if bias else None
+    r = mat(M, N, dtype, g, 1.0, pad) if residual else None
+    r64 = r.double() if residual else 0.0
+    out = r if inplace else mat(M, N, dtype, pad=pad)
+    pre = mat(M, N, dtype, pad=pad) if save else None
+    j1.op_linear(x, w, out, bias=b, act=ACTS[act], residual=r, pre=pre)
+    p, ep = affine64(x, w, b)
+    ref = act64(p, act) + r64
+    e = LIP * ep + (ACT_ERR * p.abs() if act not in ("none", "relu") else 0.0)
+    close("out", out, ref, unit(dtype) * (ref.abs() + e) + e + 2.0 ** -23 * ref.abs() + tiny(dtype) + 1e-30)
+    if save:
+        close("pre", pre, p, unit(dtype) * (p.abs() + ep) + ep + tiny(dtype) + 1e-30)
+    assert pad_untouched(out) and (pre is None or pad_untouched(pre))
+
+
+def check_gated(M, N, K, dtype, act, bias, save, pad=0, seed=0):
+    g = gen(seed)
+    x = mat(M, K, dtype, g, 1.0, pad)
+    wa, wg = mat(N, K, dtype, g, K ** -0.5, pad), mat(N, K, dtype, g, K ** -0.5, pad)
+    ba, bg = (torch.randn(N, generator=g, device="cuda") * 0.5 for _ in range(2)) if bias else (None, None)
+    out = mat(M, N, dtype, pad=pad)
+    pa, pg = (mat(M, N, dtype, pad=pad) for _ in range(2)) if save else (None, None)
+    j1.op_gated(x, wa, wg, out, ba=ba, bg=bg, act=ACTS[act], pre_a=pa, pre_g=pg)
+    a, ea = affine64(x, wa, ba)
+    q, eq = affine64(x, wg, bg)
+    f = act64(a, act)
+    ref = f * q
+    e = q.abs() * (LIP * ea + ACT_ERR * a.abs()) + f.abs() * eq + 2.0 ** -23 * ref.abs() + eq * LIP * ea
+    close("out", out, ref, unit(dtype) * (ref.abs() + e) + e + tiny(dtype) + 1e-30)
+    if save:
+        close("pre_a", pa, a, unit(dtype) * (a.abs() + ea) + ea + tiny(dtype) + 1e-30)
+        close("pre_g", pg, q, unit(dtype) * (q.abs() + eq) + eq + tiny(dtype) + 1e-30)
+    assert pad_untouched(out)
+    assert not save or (pad_untouched(pa) and pad_untouched(pg))
+
+
+def scratch(n):
+    return torch.full((max(n, 1),), 255, device="cuda", dtype=torch.uint8)  # NaN in every type
+
+
+def check_grads(dtype, x, ds, es, ws, dx, dws, dbs):
+    """dx = sum ds ws, dws = ds^T x, dbs = sum of rows of ds, where the computed ds (before their
+    rounding to dtype) are off by at most es."""
+    u, t = unit(dtype), tiny(dtype)
+    x = x.double()
+    rounded = [u * (d.abs() + e) + e + t for d, e in zip(ds, es)]
+    if dx is not None:
+        ref = sum(d @ w.double() for d, w in zip(ds, ws))
+        mag = sum((d.abs() + r) @ w.double().abs() for d, r, w in zip(ds, rounded, ws))
+        e = sum(r @ w.double().abs() for r, w in zip(rounded, ws)) + acc_err(len(ds) * ds[0].shape[1]) * mag
+        close("dx", dx, ref, u * (ref.abs() + e) + e + t + 1e-30)
+        assert pad_untouched(dx)
+    for i, dw in enumerate(dws):
+        if dw is None:
+            continue
+        ref = ds[i].t() @ x
+        e = rounded[i].t() @ x.abs() + acc_err(x.shape[0]) * ((ds[i].abs() + rounded[i]).t() @ x.abs())
+        close("dw%d" % i, dw, ref, u * (ref.abs() + e) + e + t + 1e-30)
+        assert pad_untouched(dw)
+    for i, db in enumerate(dbs):
+        if db is None:
+            continue
+        e = es[i].sum(0) + acc_err(x.shape[0]) * (ds[i].abs() + es[i]).sum(0)
+        close("db%d" % i, db, ds[i].sum(0), e + 1e-30)
+
+
+def check_linear_backward(M, N, K, dtype, act, pad=0, seed=0, want="dx dw db"):
+    g = gen(seed)
+    x, w, dout = mat(M, K, dtype, g, 1.0, pad), mat(N, K, dtype, g, K ** -0.5, pad), mat(M, N, dtype, g, 0.5, pad)
+    pre = mat(M, N, dtype, g, 1.5, pad) if act != "none" else None
+    dx = mat(M, K, dtype, pad=pad) if "dx" in want else None
+    dw = mat(N, K, dtype, pad=pad) if "dw" in want else None
+    db = torch.full((N,), float("nan"), device="cuda") if "db" in want else None
+    j1.op_linear_backward(dout, x, w, pre=pre, act=ACTS[act], dx=dx, dw=dw, dbias=db,
+                          workspace=scratch(j1.op_linear_backward_workspace(M, N, K)))
+    d = dout.double()
+    if act == "none":
+        dp, e = d, torch.zeros_like(d)
+    else:
+        dp = d * slope64(pre.double(), act)
+        e = d.abs() * SLOPE_ERR + 2.0 ** -23 * dp.abs()
+    check_grads(dtype, x, [dp], [e], [w], dx, [dw], [db])
+
+
+def check_gated_backward(M, N, K, dtype, act, pad=0, seed=0, want="dx dw db"):
+    g = gen(seed)
+    x, dout = mat(M, K, dtype, g, 1.0, pad), mat(M, N, dtype, g, 0.5, pad)
+    wa, wg = mat(N, K, dtype, g, K ** -0.5, pad), mat(N, K, dtype, g, K ** -0.5, pad)
+    pa, pg = mat(M, N, dtype, g, 1.5, pad), mat(M, N, dtype, g, 1.0, pad)
+    dx = mat(M, K, dtype, pad=pad) if "dx" in want else None
+    dwa, dwg = (mat(N, K, dtype, pad=pad) for _ in range(2)) if "dw" in want else (None, None)
+    dba, dbg = (torch.full((N,), float("nan"), device="cuda") for _ in range(2)) if "db" in want else (None, None)
+    j1.op_gated_backward(dout, x, wa, wg, pa, pg, act=ACTS[act], dx=dx, dwa=dwa, dwg=dwg, dba=dba, dbg=dbg,
+                         workspace=scratch(j1.op_gated_backward_workspace(M, N, K)))
+    d, a, q = dout.double(), pa.double(), pg.double()
+    da, dg = d * q * slope64(a, act), d * act64(a, act)
+    ea = (d * q).abs() * SLOPE_ERR + 2.0 ** -22 * da.abs()
+    eg = d.abs() * ACT_ERR * a.abs() + 2.0 ** -22 * dg.abs()
+    check_grads(dtype, x, [da, dg], [ea, eg], [wa, wg], dx, [dwa, dwg], [dba, dbg])
+
+
+# one row to several tiles; widths around the tile sizes (64, 128, 256) and 16-byte rows; odd widths
+SIZES = [(1, 1, 1), (1, 8, 16), (2, 3, 5), (5, 64, 64), (16, 1152, 768), (17, 200, 136), (33, 65, 96), (64, 127, 72),
+         (100, 129, 257), (128, 128, 128), (129, 256, 64), (200, 264, 328), (255, 768, 768), (256, 31, 33),
+         (300, 1155, 771), (513, 130, 1000), (1000, 1152, 768), (2048, 96, 40)]
+TYPES = [(BF, "gelu"), (HF, "silu"), (BF, "none"), (HF, "gelu_tanh"), (BF, "relu")]
+
+
+def _id(v):
+    return str(v).replace("torch.", "")
+
+
+@pytest.mark.parametrize("i,size", list(enumerate(SIZES)), ids=[_id(s) for s in SIZES])
+def test_linear(torch_cuda, i, size):
+    for j, (dtype, act) in enumerate(TYPES):
+        check_linear(*size, dtype, act, bias=(i + j) % 3 > 0, residual=(i + j) % 2 > 0, save=j % 2 == 0, seed=i)
+
+
+@pytest.mark.parametrize("i,size", list(enumerate(SIZES)), ids=[_id(s) for s in SIZES])
+def test_gated(torch_cuda, i, size):
+    for j, (dtype, act) in enumerate(TYPES):
+        check_gated(*size, dtype, act, bias=(i + j) % 3 > 0, save=j % 2 == 0, seed=i)
+
+
+@pytest.mark.parametrize("i,size", list(enumerate(SIZES)), ids=[_id(s) for s in SIZES])
+def test_linear_backward(torch_cuda, i, size):
+    for j, (dtype, act) in enumerate(TYPES):
+        check_linear_backward(*size, dtype, act, seed=i)
+
+
+@pytest.mark.parametrize("i,size", list(enumerate(SIZES)), ids=[_id(s) for s in SIZES])
+def test_gated_backward(torch_cuda, i, size):
+    for j, (dtype, act) in enumerate(TYPES):
+        check_gated_backward(*size, dtype, act, seed=i)
+
+
+@pytest.mark.parametrize("pad", [1, 2, 4, 8, 56])
+def test_padded_rows(torch_cuda, pad):
+    """Rows longer than the matrix, with NaN behind them: not read, not written."""
+    for size in ((40, 72, 136), (300, 100, 70), (3, 264, 200)):
+        check_linear(*size, BF, "gelu", True, True, True, pad=pad)
+        check_gated(*size, HF, "silu", True, True, pad=pad)
+        check_linear_backward(*size, BF, "gelu", pad=pad)
+        check_gated_backward(*size, BF, "silu", pad=pad)
+
+
+def test_residual_in_place(torch_cuda):
+    for size in ((1, 768, 64), (300, 771, 64), (1000, 768, 128)):
+        check_linear(*size, BF, "gelu", True, True, False, inplace=True)
+        check_linear(*size, HF, "none", False, True, True, pad=8, inplace=True)
+
+
+@pytest.mark.parametrize("want", ["dx", "dw", "db", "dx dw", "dw db"])
+def test_some_gradients_only(torch_cuda, want):
+    for act in ("none", "silu"):
+        check_linear_backward(150, 136, 72, BF, act, want=want)
+        check_gated_backward(150, 136, 72, BF, act, want=want)
+
+
+def test_long_contractions(torch_cuda):
+    """Few results over many terms: a long K forward, many rows in the weight gradients."""
+    check_linear(8, 40, 20000, BF, "none", True, False, False)
+    check_linear(130, 70, 9999, HF, "gelu", True, False, False)
+    check_linear_backward(40000, 64, 48, BF, "gelu")
+    check_gated_backward(30011, 72, 56, BF, "gelu")
+    check_gated_backward(9000, 33, 45, HF, "silu")
+
+
+def test_halves_of_one_buffer(torch_cuda):
+    """Weights as the two halves of one Wi, the stored pre-activations side by side in one buffer."""
+    M, N, K = 200, 96, 64
+    g = gen(3)
+    x, wi = mat(M, K, BF, g), mat(2 * N, K, BF, g, K ** -0.5)
+    pre, out = torch.empty((M, 2 * N), device="cuda", dtype=BF), torch.empty((M, N), device="cuda", dtype=BF)
+    j1.op_gated(x, wi[:N], wi[N:], out, act=j1.ACT_GELU, pre_a=pre[:, :N], pre_g=pre[:, N:])
+    ref, e = affine64(x, wi, None)
+    close("pre", pre, ref, unit(BF) * (ref.abs() + e) + e)
+    dwi, dx = torch.empty_like(wi), torch.empty_like(x)
+    j1.op_gated_backward(out, x, wi[:N], wi[N:], pre[:, :N], pre[:, N:], act=j1.ACT_GELU, dx=dx, dwa=dwi[:N],
+                         dwg=dwi[N:], workspace=scratch(j1.op_gated_backward_workspace(M, N, K)))
+    two = [torch.empty((N, K), device="cuda", dtype=BF) for _ in range(2)]
+    j1.op_gated_backward(out, x, wi[:N].clone(), wi[N:].clone(), pre[:, :N].clone(), pre[:, N:].clone(),
+                         act=j1.ACT_GELU, dwa=two[0], dwg=two[1],
+                         workspace=scratch(j1.op_gated_backward_workspace(M, N, K)))
+    assert torch.equal(dwi, torch.cat(two))
+
+
+def test_no_rows(torch_cuda):
+    x, w = torch.empty((0, 24), device="cuda", dtype=BF), torch.ones((40, 24), device="cuda", dtype=BF)
+    out = torch.empty((0, 40), device="cuda", dtype=BF)
+    j1.op_linear(x, w, out)
+    j1.op_gated(x, w, w, out)
+    dw = [mat(40, 24, BF, pad=3) for _ in range(2)]
+    db = [torch.full((40,), float("nan"), device="cuda") for _ in range(2)]
+    j1.op_linear_backward(out, x, w, act=j1.ACT_NONE, dw=dw[0], dbias=db[0], workspace=scratch(
+        j1.op_linear_backward_workspace(0, 40, 24)))
+    assert bool((dw[0] == 0).all()) and bool((db[0] == 0).all()) and pad_untouched(dw[0])
+    dw[0].fill_(1.0)
+    j1.op_gated_backward(out, x, w, w, out, out, dwa=dw[0], dwg=dw[1], dba=db[0], dbg=db[1], workspace=scratch(
+        j1.op_gated_backward_workspace(0, 40, 24)))
+    assert all(bool((t == 0).all()) for t in dw + db)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_extreme_values(torch_cuda, act):
+    """Large finite pre-activations give finite results and gradients (0 or the value itself on the
+    far sides), a NaN stays in its own row forward, an infinity keeps its sign."""
+    K, N = 16, 24
+    vals = torch.tensor([-3e38, -1e30, -1e4, -60.0, -40.0, -6.0, 0.0, 6.0, 40.0, 60.0, 1e4, 1e30, 3e38, -0.0, 1e-30, -1e-30],
+                        device="cuda")
+    M = vals.numel()
+    x, w = torch.zeros((M, K), device="cuda", dtype=BF), torch.zeros((N, K), device="cuda", dtype=BF)
+    x[:, 0], w[:, 0] = vals, 1.0
+    p = x[:, :1].double().expand(M, N)
+    out, pre = torch.empty((M, N), device="cuda", dtype=BF), torch.empty((M, N), device="cuda", dtype=BF)
+    j1.op_linear(x, w, out, act=ACTS[act], pre=pre)
+    ref = act64(p, act)
+    assert torch.equal(pre, x[:, :1].expand(M, N))
+    # far negative values: within 2e-6 * 40 of 0, see ACT_ERR
+    close("out", out, ref, unit(BF) * ref.abs() * 1.01 + ACT_ERR * p.abs().clamp_max(40.0))
+    dout = torch.ones((M, N), device="cuda", dtype=BF)
+    db = torch.empty(N, device="cuda")
+    dx = torch.empty_like(x)
+    j1.op_linear_backward(dout, x, w, pre=pre, act=ACTS[act], dx=dx, dbias=db,
+                          workspace=scratch(j1.op_linear_backward_workspace(M, N, K)))
+    s = slope64(p.clamp(-100, 100), act)
+    close("dx", dx[:, :1], N * s[:, :1], N * (SLOPE_ERR + 2 * unit(BF) * s[:, :1].abs()))
+    close("db", db, s.sum(0), torch.full_like(db, M * 2 * SLOPE_ERR).double())
+    x[3, 0] = float("nan")
+    x[5, 0] = float("inf")
+    j1.op_linear(x, w, out, act=ACTS[act])
+    assert bool(out[3].isnan().all()) and bool((out[5] == float("inf")).all())
+    assert not bool(out[torch.arange(M, device="cuda") != 3].isnan().any())
+
+
+def test_offsets_past_32_bits(torch_cuda):
+    """Rows far apart: element offsets above 2^32 in every matrix of M rows."""
+    M, N, K, far = 70000, 24, 40, 65536  # 70000 x 65536 = 4.6e9 elements, 9.2 GB
+    g = gen(5)
+    big = torch.zeros((M, far), device="cuda", dtype=BF)
+    x, out, r, pre = big[:, 0:K], big[:, 64:64 + N], big[:, 128:128 + N], big[:, 256:256 + N]
+    x.copy_(torch.randn((M, K), generator=g, device="cuda"))
+    r.copy_(torch.randn((M, N), generator=g, device="cuda"))
+    w = mat(N, K, BF, g, K ** -0.5)
+    j1.op_linear(x, w, out, act=j1.ACT_GELU, residual=r, pre=pre)
+    small = [torch.empty((M, N), device="cuda", dtype=BF) for _ in range(2)]
+    j1.op_linear(x.contiguous(), w, small[0], act=j1.ACT_GELU, residual=r.contiguous(), pre=small[1])
+    assert torch.equal(out, small[0]) and torch.equal(pre, small[1])
+    p, e = affine64(x[-1000:], w, None)
+    close("pre", pre[-1000:], p, unit(BF) * (p.abs() + e) + e)
+    dx = big[:, 512:512 + K]
+    dw = [torch.empty_like(w) for _ in range(2)]
+    ws = scratch(j1.op_linear_backward_workspace(M, N, K))
+    j1.op_linear_backward(out, x, w, pre=pre, act=j1.ACT_GELU, dx=dx, dw=dw[0], workspace=ws)
+    dxs = torch.empty((M, K), device="cuda", dtype=BF)
+    j1.op_linear_backward(small[0], x.contiguous(), w, pre=small[1], act=j1.ACT_GELU, dx=dxs, dw=dw[1], workspace=ws)
+    assert torch.equal(dx, dxs) and torch.equal(dw[0], dw[1])
+
+
+def _block(M, N, K, dtype, seed):
+    """Buffers of a feed-forward block: y = x + (gelu(x wa^T) (x wg^T)) wo^T + bo."""
+    g = gen(seed)
+    e = lambda *s: torch.empty(s, device="cuda", dtype=dtype)  # noqa: E731
+    return dict(M=M, N=N, K=K, x=mat(M, K, dtype, g), wa=mat(N, K, dtype, g, K ** -0.5), wg=mat(N, K, dtype, g, K ** -0.5),
+                wo=mat(K, N, dtype, g, N ** -0.5), bo=torch.randn(K, generator=g, device="cuda") * 0.3,
+                h=e(M, N), pa=e(M, N), pg=e(M, N), y=e(M, K), dy=mat(M, K, dtype, g), dh=e(M, N), dx=e(M, K),
+                dwa=e(N, K), dwg=e(N, K), dwo=e(K, N), dbo=torch.empty(K, device="cuda"),
+                ws=scratch(max(j1.op_gated_backward_workspace(M, N, K), j1.op_linear_backward_workspace(M, K, N))))
+
+
+def _step(b, stream=None, sync=False):
+    o = dict(stream=stream, sync=sync)
+    j1.op_gated(b["x"], b["wa"], b["wg"], b["h"], act=j1.ACT_GELU, pre_a=b["pa"], pre_g=b["pg"], **o)
+    j1.op_linear(b["h"], b["wo"], b["y"], bias=b["bo"], residual=b["x"], **o)
+    j1.op_linear_backward(b["dy"], b["h"], b["wo"], dx=b["dh"], dw=b["dwo"], dbias=b["dbo"], workspace=b["ws"], **o)
+    j1.op_gated_backward(b["dh"], b["x"], b["wa"], b["wg"], b["pa"], b["pg"], act=j1.ACT_GELU, dx=b["dx"], dwa=b["dwa"],
+                         dwg=b["dwg"], workspace=b["ws"], **o)
+
+
+RESULTS = ("h", "pa", "pg", "y", "dh", "dx", "dwa", "dwg", "dwo", "dbo")
+
+
+@pytest.mark.parametrize("M,N,K,dtype", [(1, 1152, 768, BF), (513, 1152, 768, BF), (300, 200, 136, HF), (77, 65, 51, BF)])
+def test_feed_forward_block(torch_cuda, M, N, K, dtype):
+    """The operators in a row against float64 autograd of the whole block. Each step's inputs are
+    rounded to the type: a handful of roundings of eps / 2 stack up, relative to the result's norm."""
+    b = _block(M, N, K, dtype, 7)
+    _step(b, sync=True)
+    d = {k: b[k].double().requires_grad_() for k in ("x", "wa", "wg", "wo", "bo")}
+    h = act64(d["x"] @ d["wa"].t(), "gelu") * (d["x"] @ d["wg"].t())
+    y = d["x"] + h @ d["wo"].t() + d["bo"]
+    grads = dict(zip(d, torch.autograd.grad(y, list(d.values()), b["dy"].double())))
+    refs = {"h": h, "y": y, "dx": grads["x"] - b["dy"].double(), "dwa": grads["wa"], "dwg": grads["wg"],
+            "dwo": grads["wo"], "dbo": grads["bo"]}
+    for k, ref in refs.items():
+        # at most six roundings precede any result (pre, h or dh, da / dg, the result, and FP32 sums)
+        off = (b[k].double() - ref).norm() / ref.norm()
+        assert off <= 6 * unit(dtype), (k, float(off))
+
+
+def test_gradients_against_differences(torch_cuda):
+    """The gradients against central differences of the float64 definition along random directions:
+    independent of any formula for the slopes."""
+    M, N, K = 9, 12, 10
+    for act in ("gelu", "gelu_tanh", "silu"):
+        b = _block(M, N, K, HF, 11)
+        j1.op_gated(b["x"], b["wa"], b["wg"], b["h"], act=ACTS[act], pre_a=b["pa"], pre_g=b["pg"])
+        b["dh"].copy_(torch.randn((M, N), generator=gen(1), device="cuda"))
+        j1.op_gated_backward(b["dh"], b["x"], b["wa"], b["wg"], b["pa"], b["pg"], act=ACTS[act], dx=b["dx"], dwa=b["dwa"],
+                             dwg=b["dwg"], workspace=b["ws"])
+
+        def value(x, wa, wg):
+            return float((act64(x @ wa.t(), act) * (x @ wg.t()) * b["dh"].double()).sum())
+
+        at = [b[k].double() for k in ("x", "wa", "wg")]
+        for i, k in enumerate(("dx", "dwa", "dwg")):
+            v = torch.randn(at[i].shape, generator=gen(20 + i), device="cuda", dtype=torch.float64)
+            step = 1e-5
+            up, dn = list(at), list(at)
+            up[i], dn[i] = at[i] + step * v, at[i] - step * v
+            num = (value(*up) - value(*dn)) / (2 * step)
+            got = float((b[k].double() * v).sum())
+            # the roundings of pre, da / dg and the result, each eps / 2 of terms that sum up in magnitude
+            scale = float((b[k].double().abs() * v.abs()).sum())
+            assert abs(got - num) <= 8 * unit(HF) * scale + 1e-6, (act, k, got, num)
+
+
+def test_same_bits_again(torch_cuda):
+    for size in ((1, 768, 768), (2048, 1152, 768), (777, 333, 129)):
+        b = _block(*size, BF, 13)
+        _step(b, sync=True)
+        first = {k: b[k].clone() for k in RESULTS}
+        for _ in range(3):
+            b["ws"].random_(0, 255)
+            for k in RESULTS:
+                b[k].fill_(float("nan"))
+            _step(b, sync=True)
+            for k in RESULTS:
+                assert torch.equal(b[k], first[k]), k
+
+
+def test_two_streams_at_once(torch_cuda):
+    """Blocks with a workspace each on two streams, interleaved, give what they give alone."""
+    blocks = [_block(1500, 768, 384, BF, 17), _block(700, 520, 264, HF, 19)]
+    refs = []
+    for b in blocks:
+        _step(b, sync=True)
+        refs.append({k: b[k].clone() for k in RESULTS})
+        for k in RESULTS:
+            b[k].fill_(float("nan"))
+    streams = [torch.cuda.Stream() for _ in blocks]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for b, s in zip(blocks, streams):
+            _step(b, stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    for b, ref in zip(blocks, refs):
+        for k in RESULTS:
+            assert torch.equal(b[k], ref[k]), k
+
+
+def test_captured_and_replayed(torch_cuda):
+    """A whole step in a CUDA graph, replayed on new inputs in the same buffers."""
+    b = _block(600, 384, 256, BF, 23)
+    _step(b, sync=True)
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        _step(b, stream=torch.cuda.current_stream().cuda_stream)
+    for seed in (1, 2):
+        g = gen(seed)
+        for k in ("x", "dy"):
+            b[k].copy_(torch.randn(b[k].shape, generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = {k: b[k].clone() for k in RESULTS}
+        _step(b, sync=True)
+        for k in RESULTS:
+            assert torch.equal(b[k], got[k]), k
+
+
+def test_refused_pointers(torch_cuda):
+    x = torch.zeros((4, 16), dtype=BF)
+    w, out = torch.zeros((8, 16), device="cuda", dtype=BF), torch.zeros((4, 8), device="cuda", dtype=BF)
+    with pytest.raises(j1.J1Error) as e:
+        j1.op_linear(x, w, out)
+    assert e.value.status == j1.INVALID_ARG and "x is not device memory" in str(e.value)
+    with pytest.raises(j1.J1Error) as e:
+        j1.op_linear(x.pin_memory(), w, out)
+    assert e.value.status == j1.INVALID_ARG and "x is not device memory" in str(e.value)
+    j1.inject_fault(j1.FAULT_LAUNCH, 1)
+    try:
+        with pytest.raises(j1.J1Error) as e:
+            j1.op_linear(x.cuda(), w, out)
+    finally:
+        j1.inject_fault(j1.FAULT_LAUNCH, 0)
+    assert e.value.status == j1.CUDA
+    j1.op_linear(x.cuda(), w, out)
+    assert bool((out == 0).all())
