@@ -1,94 +1,68 @@
-// Matrix products of the feed-forward operators with their epilogues.
-//
-// out[M, N] = act(A . B + bias) (+ residual), or act(A B0^T + bias0) * (A B1^T + bias1), any
-// operand order and stride. This is the plain form: 64 x 64 tiles, 16 deep, FP32 arithmetic on
-// the CUDA cores, 4 x 4 results per thread.
+// Plans the products of the feed-forward operators: tile shape, split and tensor maps of a call.
 #include <cuda_runtime.h>
 
-#include "ffn.h"
-#include "ffn_math.cuh"
+#include <algorithm>
+#include <climits>
+
+#include "ffn_tc.h"
 #include "kernels.h"
-#include "ptx.cuh"
 
 namespace j1rt {
 
 namespace {
 
-constexpr int TM = 64, TN = 64, TK = 16;
-
-__device__ __forceinline__ float act_any(int act, float p) {
-  switch (act) {
-    case J1_ACT_RELU: return act_value<J1_ACT_RELU>(p);
-    case J1_ACT_GELU: return act_value<J1_ACT_GELU>(p);
-    case J1_ACT_GELU_TANH: return act_value<J1_ACT_GELU_TANH>(p);
-    case J1_ACT_SILU: return act_value<J1_ACT_SILU>(p);
-  }
-  return p;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) simple_kernel(const FfnGemm g) {
-  __shared__ float sa[TK][TM + 1], sb[2][TK][TN + 1];
-  const long long m0 = static_cast<long long>(blockIdx.y) * TM;
-  const int n0 = blockIdx.x * TN;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int nb = g.gated ? 2 : 1;
-  float acc[2][4][4] = {};
-  grid_dep_launch();
-  grid_dep_wait();
-  for (int s = 0; s < g.segs; ++s)
-    for (int k0 = 0; k0 < g.K; k0 += TK) {
-      for (int i = threadIdx.x; i < TM * TK; i += 256) {
-        // neighbouring threads along the contiguous dimension
-        const int m = g.layout == FFN_TN ? i % TM : i / TK, k = g.layout == FFN_TN ? i / TM : i % TK;
-        const long long r = m0 + m;
-        const long long kk = k0 + k;
-        sa[k][m] = r < g.M && kk < g.K
-                       ? Elem<T>::load(g.a[s].p, g.layout == FFN_TN ? kk * g.a[s].ld + r : r * g.a[s].ld + kk)
-                       : 0.f;
-        const int n = g.layout == FFN_NT ? i / TK : i % TN, kb = g.layout == FFN_NT ? i % TK : i / TN;
-        const long long c = n0 + n, kkb = k0 + kb;
-        for (int h = 0; h < nb; ++h) {
-          const FfnMat& b = g.b[g.gated ? h : s];
-          sb[h][kb][n] = c < g.N && kkb < g.K ? Elem<T>::load(b.p, g.layout == FFN_NT ? c * b.ld + kkb : kkb * b.ld + c)
-                                              : 0.f;
-        }
-      }
-      __syncthreads();
-      for (int k = 0; k < TK; ++k)
-        for (int h = 0; h < nb; ++h)
-          for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) acc[h][i][j] = fmaf(sa[k][ty * 4 + i], sb[h][k][tx + 16 * j], acc[h][i][j]);
-      __syncthreads();
-    }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      long long r = m0 + ty * 4 + i;
-      const int c = n0 + tx + 16 * j;
-      if (r >= g.M || c >= g.N) continue;
-      float p = acc[0][i][j];
-      if (g.bias[0]) p += g.bias[0][c];
-      if (g.pre[0].p) Elem<T>::store(const_cast<void*>(g.pre[0].p), r * g.pre[0].ld + c, p);
-      float v = act_any(g.act, p);
-      if (g.gated) {
-        float q = acc[1][i][j];
-        if (g.bias[1]) q += g.bias[1][c];
-        if (g.pre[1].p) Elem<T>::store(const_cast<void*>(g.pre[1].p), r * g.pre[1].ld + c, q);
-        v *= q;
-      }
-      if (g.residual.p) v += Elem<T>::load(g.residual.p, r * g.residual.ld + c);
-      int o = 0;
-      if (r >= g.row1) {
-        o = 1;
-        r -= g.row1;
-      } else if (r >= g.rows0) {
-        continue;
-      }
-      Elem<T>::store(const_cast<void*>(g.out[o].p), r * g.out[o].ld + c, v);
-    }
-}
-
 __device__ int g_ffn_error;
+
+constexpr int kPairs = 74;                        // most CTA pairs a stream-K product uses
+constexpr size_t kPieceBytes = 256 * 256 * 4;     // FP32 accumulators of a pair
+
+// Rows on 16-byte boundaries: what TMA and 16-byte accesses need.
+bool rows16(const FfnMat& m) { return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0; }
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+struct Plan {
+  int cfg, cg, bn, split;
+  bool stream_k;
+  double us;
+};
+
+// Microseconds per 64-block of a tile and CTA (or pair) and the fixed part of a tile that
+// nothing hides (first loads, last epilogue).
+Plan choose(const FfnGemm& g, bool aligned, int kb) {
+  const int sms = g.num_sms;
+  const auto single = [&](int cfg, int bn, double step) {
+    const long long tiles = ceil_div(g.M, 128) * ceil_div(g.N, g.gated ? bn / 2 : bn);
+    Plan best = {cfg, 1, bn, 1, false, 0.0};
+    best.us = static_cast<double>(ceil_div(tiles, sms)) * kb * step + 1.5;
+    for (int s = 2; s <= 8 && s <= kb; s *= 2) {
+      const double us = static_cast<double>(ceil_div(tiles * s, sms)) * (static_cast<double>(ceil_div(kb, s)) * step + 1.5) + 1.0;
+      if (us < best.us) best.split = s, best.us = us;
+    }
+    return best;
+  };
+  if (!aligned) return single(FFN_CG1_128_GEN, 128, 0.5);
+  Plan best = single(FFN_CG1_128, 128, 0.22);
+  const auto take = [&](const Plan& p) {
+    if (p.us < best.us) best = p;
+  };
+  if (!g.gated) take(single(FFN_CG1_64, 64, 0.13));
+  const auto pair = [&](int cfg, int bn, double step) {
+    const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
+    const int pairs = std::max(1, std::min(kPairs, sms / 2));
+    Plan p = {cfg, 2, bn, 1, false, 0.0};
+    p.us = static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 2.5;
+    if (g.layout == FFN_TN && bn == 256 && g.partials &&
+        (tiles + pairs) * kPieceBytes <= g.partial_bytes) {  // equal shares, then a pass over the pieces
+      const double us = static_cast<double>(tiles) * kb * step / pairs + 6.0 + 0.1 * static_cast<double>(tiles + pairs) / 4;
+      if (us < p.us) p.stream_k = true, p.us = us;
+    }
+    return p;
+  };
+  take(pair(FFN_CG2_256, 256, 0.40));
+  if (g.layout == FFN_NT && !g.gated) take(pair(FFN_CG2_192, 192, 0.31));
+  return best;
+}
 
 }  // namespace
 
@@ -99,12 +73,74 @@ cudaError_t ffn_error_word(int** p) {
   return e;
 }
 
-size_t ffn_partial_bytes(int, int, int) { return 0; }
+// Pieces of a stream-K product: one per worker and tile boundary. With more tiles than four per
+// pair whole tiles balance well enough, and nothing is set aside.
+size_t ffn_partial_bytes(int M, int N, int K) {
+  const long long tiles = ceil_div(M, 256) * ceil_div(N, 256);
+  if (tiles > 4 * kPairs || K <= 64) return 0;
+  return static_cast<size_t>(tiles + kPairs) * kPieceBytes;
+}
 
-int launch_ffn_gemm(const FfnGemm& g, cudaStream_t st) {
-  const dim3 grid((g.N + TN - 1) / TN, (g.M + TM - 1) / TM);
-  return static_cast<int>(g.fp16 ? launch_kernel(simple_kernel<__half>, grid, dim3(256), 0, st, g)
-                                 : launch_kernel(simple_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, g));
+int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
+  FfnTc p = {};
+  bool aligned = true;
+  const int nb = g.gated ? 2 : g.segs;
+  for (int i = 0; i < 2; ++i) {
+    p.a[i] = g.a[i], p.b[i] = g.b[i], p.out[i] = g.out[i], p.pre[i] = g.pre[i], p.bias[i] = g.bias[i];
+    if (i < g.segs) aligned = aligned && rows16(g.a[i]);
+    if (i < nb) aligned = aligned && rows16(g.b[i]);
+  }
+  p.M = g.M, p.N = g.N, p.K = g.K;
+  p.segs = g.segs;
+  p.kb_seg = static_cast<int>(ceil_div(g.K, 64));
+  if (static_cast<long long>(p.kb_seg) * g.segs > INT_MAX) return static_cast<int>(cudaErrorInvalidValue);
+  p.kb = p.kb_seg * g.segs;
+  const Plan plan = choose(g, aligned, p.kb);
+  p.act = g.act;
+  p.row1 = g.row1, p.rows0 = g.rows0;
+  const long long m_tiles = ceil_div(g.M, 128 * plan.cg);
+  const long long n_tiles = ceil_div(g.N, g.gated ? plan.bn / 2 : plan.bn);
+  if (m_tiles * n_tiles * plan.split > INT_MAX / 64) return static_cast<int>(cudaErrorInvalidValue);
+  p.m_tiles = static_cast<int>(m_tiles), p.n_tiles = static_cast<int>(n_tiles);
+  p.tiles = p.m_tiles * p.n_tiles;
+  p.group = 8;
+  p.split = plan.split;
+  p.stream_k = plan.stream_k;
+  p.partials = g.partials;
+  const int slots = plan.cg == 2 ? std::max(1, std::min(kPairs, g.num_sms / 2)) : g.num_sms;
+  p.workers = plan.split > 1 ? p.tiles : plan.stream_k ? slots : std::min(p.tiles, slots);
+  p.a_rows = plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
+  p.err = g.err;
+  p.residual = g.residual;
+  p.vec_res = g.residual.p && rows16(g.residual) && g.N % 8 == 0;
+  const int outs = g.row1 == INT_MAX ? 1 : 2;
+  // a TMA store clips at whole 16-byte units: with a ragged width it would write behind the rows
+  p.tma_out = p.tma_pre = g.N % 8 == 0;
+  for (int i = 0; i < 2; ++i) {
+    if (i < outs) p.tma_out = p.tma_out && rows16(g.out[i]);
+    if (g.pre[i].p) p.tma_pre = p.tma_pre && rows16(g.pre[i]);
+  }
+  const char* why = nullptr;
+  bool ok = true;
+  if (aligned) {
+    for (int i = 0; i < g.segs; ++i)
+      ok = ok && (g.layout == FFN_TN ? make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.K, g.M, g.a[i].ld, 64, 64, &why)
+                                     : make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.M, g.K, g.a[i].ld, 64, p.a_rows, &why));
+    const uint32_t b_rows = g.layout != FFN_NT ? 64 : g.gated ? plan.bn / 2 : plan.bn / plan.cg;
+    for (int i = 0; i < nb; ++i)
+      ok = ok && (g.layout == FFN_NT ? make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.N, g.K, g.b[i].ld, 64, b_rows, &why)
+                                     : make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.K, g.N, g.b[i].ld, 64, b_rows, &why));
+  }
+  if (p.tma_out)
+    for (int i = 0; i < outs; ++i)
+      ok = ok && make_tmap_16bit(&p.mout[i], g.fp16, g.out[i].p, i ? g.M - g.row1 : std::min(g.M, g.rows0), g.N, g.out[i].ld,
+                                 32, 32, &why);
+  if (p.tma_pre)
+    for (int i = 0; i < 2; ++i)
+      if (g.pre[i].p) ok = ok && make_tmap_16bit(&p.mpre[i], g.fp16, g.pre[i].p, g.M, g.N, g.pre[i].ld, 32, 32, &why);
+  if (!ok) return static_cast<int>(cudaErrorInvalidValue);
+  return g.fp16 ? launch_ffn_tc_fp16(plan.cfg, g.layout, g.gated, p, stream)
+                : launch_ffn_tc_bf16(plan.cfg, g.layout, g.gated, p, stream);
 }
 
 }  // namespace j1rt

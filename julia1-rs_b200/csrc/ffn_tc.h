@@ -1,0 +1,32 @@
+// Parameters of the tensor-core product kernel (ffn_tc.cuh) and its launchers, one translation
+// unit per element type.
+#pragma once
+#include "ffn.h"
+
+namespace j1rt {
+
+struct FfnTc {
+  CUtensorMap ma[2], mb[2], mout[2], mpre[2];
+  FfnMat a[2], b[2], out[2], pre[2], residual;
+  const float* bias[2];
+  int M, N, K;              // output rows, columns, contraction per segment
+  int segs, kb_seg, kb;     // segments, 64-blocks per segment, 64-blocks in all
+  int act;
+  int row1, rows0;          // see FfnGemm
+  int m_tiles, n_tiles, tiles, group;
+  int workers;              // CTAs (CG 1) or CTA pairs (CG 2) that walk the tiles; cluster splits: tiles
+  int split;                // CTAs of a cluster that share a tile's contraction (CG 1), else 1
+  int stream_k;             // each worker takes an equal share of all tiles' blocks; FP32 pieces to partials
+  float* partials;
+  int stages;
+  int tma_out, tma_pre, vec_res;  // 16-byte rows: outputs / stored pre-activations by TMA, residual by 16-byte loads
+  int a_rows;               // rows of one A box (K-major A): fewer than 128 when M is smaller
+  int* err;
+};
+
+// Configurations: CG (CTAs per tile pair) x BN (accumulator columns of a tile).
+enum FfnCfg : int { FFN_CG2_256 = 0, FFN_CG2_192, FFN_CG1_128, FFN_CG1_64, FFN_CG1_128_GEN };
+int launch_ffn_tc_bf16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream);
+int launch_ffn_tc_fp16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream);
+
+}  // namespace j1rt

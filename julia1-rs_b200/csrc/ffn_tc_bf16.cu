@@ -1,0 +1,8 @@
+// The feed-forward products (ffn_tc.cuh) on BF16.
+#include "ffn_tc.cuh"
+
+namespace j1rt {
+int launch_ffn_tc_bf16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream) {
+  return ffn::launch_tc<__nv_bfloat16>(cfg, layout, gated, p, stream);
+}
+}  // namespace j1rt

@@ -538,7 +538,8 @@ EncodeTiledFn encode_fn() {
 }
 
 bool make_tmap(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, const void* base, uint64_t rows,
-               uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows, const char** why) {
+               uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows, const char** why,
+               CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) {
     if (why) *why = "cuTensorMapEncodeTiled unavailable";
@@ -550,7 +551,7 @@ bool make_tmap(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, const v
   const cuuint32_t box[2] = {box_cols, box_rows};
   const cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     if (why) *why = "cuTensorMapEncodeTiled failed (alignment or shape)";
     return false;
@@ -562,6 +563,12 @@ bool make_tmap(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, const v
 bool make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                     uint32_t box_rows, const char** why) {
   return make_tmap(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, rows, cols, ld, 64, box_rows, why);
+}
+
+bool make_tmap_16bit(CUtensorMap* map, bool fp16, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                     uint32_t box_cols, uint32_t box_rows, const char** why) {
+  return make_tmap(map, fp16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, rows, cols, ld,
+                   box_cols, box_rows, why, box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 bool make_tmap_f32_resid(CUtensorMap* map, const float* base, uint64_t rows, uint64_t cols, uint64_t ld,

@@ -158,6 +158,9 @@ int launch_wait_timeout_selftest(int* err, long long limit, cudaStream_t stream)
 // 2D bf16 row-major [rows, cols] with row stride `ld` elements; 128B swizzle box (64 x box_rows).
 bool make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
                     uint32_t box_rows, const char** why);
+// 2D row-major 16-bit [rows, cols] of either type: boxes of 64 columns (128B swizzle) or 32 columns (64B swizzle).
+bool make_tmap_16bit(CUtensorMap* map, bool fp16, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                     uint32_t box_cols, uint32_t box_rows, const char** why);
 // 2D fp32 row-major residual [rows, cols] (row stride `ld` elements); 128B-swizzled 32 x 128 box.
 bool make_tmap_f32_resid(CUtensorMap* map, const float* base, uint64_t rows, uint64_t cols, uint64_t ld,
                          const char** why, uint32_t box_rows = 128);
