@@ -41,12 +41,11 @@ Plan choose(const FfnGemm& g, bool aligned, int kb) {
     }
     return best;
   };
-  if (!aligned) return single(FFN_CG1_128_GEN, 128, 0.5);
-  Plan best = single(FFN_CG1_128, 128, 0.22);
+  Plan best = aligned ? single(FFN_CG1_128, 128, 0.22) : single(FFN_CG1_128_GEN, 128, 0.6);
   const auto take = [&](const Plan& p) {
     if (p.us < best.us) best = p;
   };
-  if (!g.gated) take(single(FFN_CG1_64, 64, 0.13));
+  if (aligned && !g.gated) take(single(FFN_CG1_64, 64, 0.13));
   const auto pair = [&](int cfg, int bn, double step) {
     const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
     const int pairs = std::max(1, std::min(kPairs, sms / 2));
@@ -59,8 +58,8 @@ Plan choose(const FfnGemm& g, bool aligned, int kb) {
     }
     return p;
   };
-  take(pair(FFN_CG2_256, 256, 0.40));
-  if (g.layout == FFN_NT && !g.gated) take(pair(FFN_CG2_192, 192, 0.31));
+  take(aligned ? pair(FFN_CG2_256, 256, 0.40) : pair(FFN_CG2_256_GEN, 256, 0.8));
+  if (aligned && g.layout == FFN_NT && !g.gated) take(pair(FFN_CG2_192, 192, 0.31));
   return best;
 }
 
@@ -109,16 +108,15 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   p.partials = g.partials;
   const int slots = plan.cg == 2 ? std::max(1, std::min(kPairs, g.num_sms / 2)) : g.num_sms;
   p.workers = plan.split > 1 ? p.tiles : plan.stream_k ? slots : std::min(p.tiles, slots);
-  p.a_rows = plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
+  p.a_rows = aligned && plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
   p.err = g.err;
   p.residual = g.residual;
   p.vec_res = g.residual.p && rows16(g.residual) && g.N % 8 == 0;
   const int outs = g.row1 == INT_MAX ? 1 : 2;
-  // a TMA store clips at whole 16-byte units: with a ragged width it would write behind the rows
-  p.tma_out = p.tma_pre = g.N % 8 == 0;
+  p.vec_out = p.vec_pre = g.N % 8 == 0;
   for (int i = 0; i < 2; ++i) {
-    if (i < outs) p.tma_out = p.tma_out && rows16(g.out[i]);
-    if (g.pre[i].p) p.tma_pre = p.tma_pre && rows16(g.pre[i]);
+    if (i < outs) p.vec_out = p.vec_out && rows16(g.out[i]);
+    if (g.pre[i].p) p.vec_pre = p.vec_pre && rows16(g.pre[i]);
   }
   const char* why = nullptr;
   bool ok = true;
@@ -131,13 +129,6 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
       ok = ok && (g.layout == FFN_NT ? make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.N, g.K, g.b[i].ld, 64, b_rows, &why)
                                      : make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.K, g.N, g.b[i].ld, 64, b_rows, &why));
   }
-  if (p.tma_out)
-    for (int i = 0; i < outs; ++i)
-      ok = ok && make_tmap_16bit(&p.mout[i], g.fp16, g.out[i].p, i ? g.M - g.row1 : std::min(g.M, g.rows0), g.N, g.out[i].ld,
-                                 32, 32, &why);
-  if (p.tma_pre)
-    for (int i = 0; i < 2; ++i)
-      if (g.pre[i].p) ok = ok && make_tmap_16bit(&p.mpre[i], g.fp16, g.pre[i].p, g.M, g.N, g.pre[i].ld, 32, 32, &why);
   if (!ok) return static_cast<int>(cudaErrorInvalidValue);
   return g.fp16 ? launch_ffn_tc_fp16(plan.cfg, g.layout, g.gated, p, stream)
                 : launch_ffn_tc_bf16(plan.cfg, g.layout, g.gated, p, stream);

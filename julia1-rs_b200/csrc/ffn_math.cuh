@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../../include/j1.h"
+#include "ptx.cuh"
 
 namespace j1rt {
 
@@ -105,6 +106,42 @@ __device__ __forceinline__ float act_value(float p) {
     return h * sigmoid(h);
   }
   return p;
+}
+
+// act of two values. GELU: erf(x) = x P(x^2) / Q(x^2) for |x| <= 4 with P of degree 6 and Q of
+// degree 4 in x^2 (the Eigen / XLA single-precision rational, within 1.2e-7 of erf), evaluated
+// on pairs with packed FP32 arithmetic: no exponential, a reciprocal per value, and half the
+// instructions. x = p / sqrt(2) is folded into the coefficients. Below the clamp the product
+// uses the clamped p, so a far negative p gives 0 (to 4e-7) and not p times an error.
+template <int ACT>
+__device__ __forceinline__ void act_pair(float& a, float& b) {
+  if constexpr (ACT == J1_ACT_GELU) {
+    constexpr float kClamp = 5.656854f;  // 4 sqrt(2)
+    const float la = max_nan(a, -kClamp), lb = max_nan(b, -kClamp);
+    const uint64_t x = f2pack(fminf(la, kClamp), fminf(lb, kClamp));
+    const uint64_t t = mul2(x, x);
+    auto c2 = [](float c) { return f2pack(c, c); };
+    uint64_t p = c2(-3.01199018e-12f);
+    p = fma2(p, t, c2(6.1223987e-10f));
+    p = fma2(p, t, c2(-9.28530142e-08f));
+    p = fma2(p, t, c2(-5.03151205e-06f));
+    p = fma2(p, t, c2(-0.00012992922f));
+    p = fma2(p, t, c2(-0.00104460877f));
+    p = fma2(p, t, c2(-0.011381614f));
+    uint64_t q = c2(-9.10379526e-07f);
+    q = fma2(q, t, c2(-2.6671758e-05f));
+    q = fma2(q, t, c2(-0.000420706754f));
+    q = fma2(q, t, c2(-0.00368666439f));
+    q = fma2(q, t, c2(-0.01426474f));
+    float q0, q1;
+    f2unpack(q, q0, q1);
+    const uint64_t erf = mul2(mul2(x, p), f2pack(recip_approx(q0), recip_approx(q1)));
+    const uint64_t h = mul2(f2pack(la, lb), c2(0.5f));
+    f2unpack(fma2(h, erf, h), a, b);
+  } else {
+    a = act_value<ACT>(a);
+    b = act_value<ACT>(b);
+  }
 }
 
 // act'(p) and act(p). The slopes are constant to FP32 beyond |p| = 40; clamping there keeps

@@ -6,7 +6,7 @@
 namespace j1rt {
 
 struct FfnTc {
-  CUtensorMap ma[2], mb[2], mout[2], mpre[2];
+  CUtensorMap ma[2], mb[2];
   FfnMat a[2], b[2], out[2], pre[2], residual;
   const float* bias[2];
   int M, N, K;              // output rows, columns, contraction per segment
@@ -19,13 +19,13 @@ struct FfnTc {
   int stream_k;             // each worker takes an equal share of all tiles' blocks; FP32 pieces to partials
   float* partials;
   int stages;
-  int tma_out, tma_pre, vec_res;  // 16-byte rows: outputs / stored pre-activations by TMA, residual by 16-byte loads
+  int vec_out, vec_pre, vec_res;  // rows of whole 16-byte units: 16-byte accesses
   int a_rows;               // rows of one A box (K-major A): fewer than 128 when M is smaller
   int* err;
 };
 
 // Configurations: CG (CTAs per tile pair) x BN (accumulator columns of a tile).
-enum FfnCfg : int { FFN_CG2_256 = 0, FFN_CG2_192, FFN_CG1_128, FFN_CG1_64, FFN_CG1_128_GEN };
+enum FfnCfg : int { FFN_CG2_256 = 0, FFN_CG2_192, FFN_CG1_128, FFN_CG1_64, FFN_CG1_128_GEN, FFN_CG2_256_GEN };
 int launch_ffn_tc_bf16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream);
 int launch_ffn_tc_fp16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream);
 
