@@ -52,7 +52,7 @@ Plan choose(const FfnGemm& g, bool aligned, int kb) {
     Plan p = {cfg, 2, bn, 1, false, 0.0};
     p.us = static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 2.5;
     if (g.layout == FFN_TN && bn == 256 && g.partials &&
-        (tiles + pairs) * kPieceBytes <= g.partial_bytes) {  // equal shares, then a pass over the pieces
+        tiles * kb < INT_MAX && tiles * kb >= pairs && (tiles + pairs) * kPieceBytes <= g.partial_bytes) {  // equal shares, then a pass over the pieces
       const double us = static_cast<double>(tiles) * kb * step / pairs + 6.0 + 0.1 * static_cast<double>(tiles + pairs) / 4;
       if (us < p.us) p.stream_k = true, p.us = us;
     }
@@ -104,10 +104,13 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   p.tiles = p.m_tiles * p.n_tiles;
   p.group = 8;
   p.split = plan.split;
+  for (p.split_log2 = 0; (1 << p.split_log2) < plan.split;) ++p.split_log2;
   p.stream_k = plan.stream_k;
   p.partials = g.partials;
   const int slots = plan.cg == 2 ? std::max(1, std::min(kPairs, g.num_sms / 2)) : g.num_sms;
   p.workers = plan.split > 1 ? p.tiles : plan.stream_k ? slots : std::min(p.tiles, slots);
+  p.share = p.tiles * static_cast<long long>(p.kb) / p.workers;
+  p.share_more = static_cast<int>(p.tiles * static_cast<long long>(p.kb) % p.workers);
   p.a_rows = aligned && plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
   p.err = g.err;
   p.residual = g.residual;

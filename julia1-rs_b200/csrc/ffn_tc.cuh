@@ -29,6 +29,11 @@
 // products. The epilogue works on 32-column chunks, one thread per row: FP32 accumulators from
 // TMEM, bias, activation, residual, one rounding, then through a swizzled 32 x 32 box in shared
 // memory to coalesced 16-byte stores (element stores where rows are not 16-byte aligned).
+//
+// Code size counts: a launch of a few microseconds fetches its instructions cold, and a role's
+// loop that does not fit the innermost instruction cache costs about 180 cycles per turn. So the
+// epilogue works in rolled loops of 16 columns, box copies and waiting loops are out of line, and
+// shared memory is addressed with 32-bit addresses throughout.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -51,11 +56,11 @@ __host__ __device__ constexpr int epi_warps(bool gen) { return gen ? 4 : 8; }
 __host__ __device__ constexpr int threads_of(bool gen) { return 32 * (2 + epi_warps(gen) + (gen ? GW : 0)); }
 constexpr uint32_t SLOT = 32 * 32 * 2;  // one 32 x 32 output box
 constexpr uint32_t A_BYTES = BM * BK * 2;
-constexpr uint32_t TAIL_BYTES = 8 * SLOT + 1024 /* bias */ + 256 /* barriers */;
 constexpr uint32_t SMEM_MAX = 232448;
+// bias of the chunk at hand per epilogue warp (two rows of 32 floats), barriers
+constexpr uint32_t BIAS_BYTES = 8 * 2 * 32 * 4, BAR_BYTES = 256;
 
 __host__ __device__ constexpr uint32_t b_bytes(int cg, int bn) { return static_cast<uint32_t>(bn / cg) * BK * 2; }
-__host__ __device__ constexpr uint32_t stage_bytes(int cg, int bn) { return A_BYTES + b_bytes(cg, bn); }
 __host__ __device__ constexpr uint32_t tmem_cols(int bn) { return bn > 128 ? 512 : bn > 64 ? 256 : 128; }
 
 // kind::f16 instruction descriptor (ptx.cuh idesc_bf16) with the element type as a parameter.
@@ -72,10 +77,88 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
   return r != 0;
 }
-// A bounded wait by a whole warp with one outcome.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int site) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, site));
+// ---- shared-memory operations by 32-bit address
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Whether a phase is complete, without waiting.
+__device__ __forceinline__ bool bar_peek(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// The same, suspending the thread for a while.
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// A bounded wait of a whole warp with one outcome, as ptx.cuh's mbar_wait: after J1_WAIT_CYCLES (or
+// once another role of the CTA gave up) the CTA's abort word is set, the site recorded in *err.
+static __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, uint32_t abort_word, int* err, int site) {
+  const long long t0 = clock64();
+  for (;;) {
+    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, lds32(abort_word) != 0)) return false;
+    if (__any_sync(0xffffffffu, clock64() - t0 > J1_WAIT_CYCLES)) {
+      if (lane_id() == 0) {
+        sts32(abort_word, 1u);
+        if (err) atomicCAS(err, 0, 1 | (site << 16));
+      }
+      __syncwarp();
+      return false;
+    }
+  }
+}
+struct Waiter {
+  uint32_t abort_word;
+  int* err;
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity, int site) const {
+    if (__all_sync(0xffffffffu, bar_peek(bar, parity))) return true;
+    return wait_slow(bar, parity, abort_word, err, site);
+  }
+};
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // Arrivals whose writes the other CTA of the pair reads through its tensor core (GEN, CG 2).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
@@ -89,13 +172,38 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
   else
     umma_bf16(d, a, b, id, acc);
 }
-// Arrive on `bar` of CTA `rank` of the pair (CG 1: of this CTA) when this thread's MMAs are done.
+// Arrive on the barrier at this shared address in this CTA (CG 1) or in CTA `rank` of the pair when
+// this thread's MMAs are done.
 template <int CG>
-__device__ __forceinline__ void commit(uint64_t* bar, uint32_t rank) {
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t rank) {
   if constexpr (CG == 2)
-    umma_commit_pair(mapa_shared(smem_u32(bar), rank));
+    umma_commit_pair(mapa_shared(bar, rank));
   else
-    umma_commit(bar);
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// One TMA box to shared address dst, completing on `bar` (CG 2: the leader's, as a cluster address).
+template <int CG>
+__device__ __forceinline__ void tma_box(const CUtensorMap* map, uint32_t bar, uint32_t dst, int x, int y) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+            dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+// 32 TMEM lanes x 16 columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 __device__ __forceinline__ float4 ld_cluster(uint32_t caddr) {
   float4 v;
@@ -107,45 +215,56 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t caddr) {
 }
 
 // A worker's list of (tile, blocks [k0, k1)): whole tiles w, w + workers, ..., or its share of
-// the tile-major block list (stream-K), or its range of one tile (cluster split).
+// the tile-major block list (stream-K), or its range of one tile (cluster split). Everything the
+// loops need is held here, in registers: after every asm statement a parameter would be read again.
 struct Units {
   int tile, k0, k1;
-  long long pos, end;
+  int kb, step, tiles;      // blocks per tile, tiles to the next one, tiles
+  int group, m_tiles, n_tiles;
+  int pos, end;             // stream-K: blocks [pos, end) of the list (below 2^31)
+
+  __device__ __forceinline__ Units(const FfnTc& p, int worker, int rank) {
+    kb = p.kb, step = p.workers, tiles = p.tiles;
+    group = p.group, m_tiles = p.m_tiles, n_tiles = p.n_tiles;
+    tile = worker, k0 = 0, k1 = kb;
+    pos = end = 0;
+    if (p.stream_k) {
+      pos = share_begin(p, worker);
+      end = share_begin(p, worker + 1);
+      step = 0;
+      share();
+    } else if (p.split > 1) {
+      const int per = (kb + p.split - 1) >> p.split_log2;  // blocks per CTA, the last ones one less
+      const int full = kb - (per - 1) * p.split;
+      k0 = rank * per - (rank > full ? rank - full : 0);
+      k1 = k0 + per - (rank >= full ? 1 : 0);
+    }
+  }
+  static __device__ __forceinline__ int share_begin(const FfnTc& p, int worker) {
+    return worker * p.share + min(worker, p.share_more);
+  }
+  __device__ __forceinline__ void share() {
+    tile = pos < end ? pos / kb : tiles;
+    k0 = pos - tile * kb;
+    k1 = min(end - pos, kb - k0) + k0;
+  }
+  __device__ __forceinline__ bool ok() const { return tile < tiles; }
+  __device__ __forceinline__ void next() {
+    tile += step;
+    if (step == 0) {
+      pos += k1 - k0;
+      share();
+    }
+  }
+  __device__ __forceinline__ void at(int& mt, int& nt) const;
 };
-__device__ __forceinline__ bool unit_ok(const FfnTc& p, const Units& u) {
-  return p.stream_k ? u.pos < u.end : u.tile < p.tiles;
-}
-__device__ __forceinline__ void unit_set(const FfnTc& p, Units& u) {
-  if (!p.stream_k) return;
-  u.tile = static_cast<int>(u.pos / p.kb);
-  u.k0 = static_cast<int>(u.pos - static_cast<long long>(u.tile) * p.kb);
-  const long long left = u.end - u.pos;
-  u.k1 = left < p.kb - u.k0 ? u.k0 + static_cast<int>(left) : p.kb;
-}
-__device__ __forceinline__ Units unit_first(const FfnTc& p, int worker, int rank) {
-  Units u = {worker, 0, p.kb, 0, 0};
-  if (p.stream_k) {
-    const long long all = static_cast<long long>(p.tiles) * p.kb;
-    u.pos = all * worker / p.workers;
-    u.end = all * (worker + 1) / p.workers;
-    if (u.pos < u.end) unit_set(p, u);
-  } else if (p.split > 1) {
-    u.k0 = static_cast<int>(static_cast<long long>(p.kb) * rank / p.split);
-    u.k1 = static_cast<int>(static_cast<long long>(p.kb) * (rank + 1) / p.split);
-  }
-  return u;
-}
-__device__ __forceinline__ void unit_next(const FfnTc& p, Units& u) {
-  if (p.stream_k) {
-    u.pos += u.k1 - u.k0;
-    if (u.pos < u.end) unit_set(p, u);
-  } else {
-    u.tile += p.workers;
-  }
-}
 // Tiles are ordered in groups of `group` tile rows, rows fastest inside a group: the tiles in
 // flight share few rows of A and few columns of B, so both stay in L2.
 __host__ __device__ __forceinline__ void tile_at(int tile, int group, int m_tiles, int n_tiles, int& mt, int& nt) {
+  if (m_tiles == 1) {
+    mt = 0, nt = tile;
+    return;
+  }
   const int per = group * n_tiles;
   const int first = tile / per * group;
   const int rows = m_tiles - first < group ? m_tiles - first : group;
@@ -153,6 +272,8 @@ __host__ __device__ __forceinline__ void tile_at(int tile, int group, int m_tile
   mt = first + r % rows;
   nt = r / rows;
 }
+
+__device__ __forceinline__ void Units::at(int& mt, int& nt) const { tile_at(tile, group, m_tiles, n_tiles, mt, nt); }
 
 // ---- GEN loads. A unit is 8 elements (16 bytes of a box row) from address `at`; `n` of them lie
 // inside the matrix's row (n <= 0: none, all zero). The two aligned 16-byte pieces that hold it
@@ -249,7 +370,7 @@ struct GenOperand {
     }
     return slow;
   }
-  __device__ __forceinline__ void store2(const GenUnit (&g)[4], uint32_t slow, int t, int k, uint8_t* dst,
+  __device__ __forceinline__ void store2(const GenUnit (&g)[4], uint32_t slow, int t, int k, uint32_t dst,
                                          const GenOperand& o) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -259,10 +380,10 @@ struct GenOperand {
       int c;
       w.pos(i, k, r, c);
       const uint32_t s = (slow >> j) & 1 ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(w.at(r, c)) & 15u);
-      *reinterpret_cast<uint4*>(dst + br * 128 + ((u ^ (br & 7)) << 4)) = gen_shift(g[j], s, cols - c);
+      sts128(dst + br * 128 + ((u ^ (br & 7)) << 4), gen_shift(g[j], s, cols - c));
     }
   }
-  __device__ __forceinline__ void store(const GenUnit (&g)[4], uint32_t slow, int t, int k, uint8_t* dst) const {
+  __device__ __forceinline__ void store(const GenUnit (&g)[4], uint32_t slow, int t, int k, uint32_t dst) const {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int i = t + j * GW * 32, br = i >> 3, u = i & 7;
@@ -270,7 +391,7 @@ struct GenOperand {
       int c;
       pos(i, k, r, c);
       const uint32_t s = (slow >> j) & 1 ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at(r, c)) & 15u);
-      *reinterpret_cast<uint4*>(dst + br * 128 + ((u ^ (br & 7)) << 4)) = gen_shift(g[j], s, cols - c);
+      sts128(dst + br * 128 + ((u ^ (br & 7)) << 4), gen_shift(g[j], s, cols - c));
     }
   }
 };
@@ -306,128 +427,176 @@ __device__ __forceinline__ void store_row8(const FfnMat& m, bool vec, long long 
   }
 }
 
+// Copies a warp's box (32 rows x 32 columns, 64 bytes a row, unit u of row r at u ^ (r >> 1 & 3)) to rows
+// [row, row + 32) below `rows`, columns [col, col + 32) below N of a matrix.
+static __device__ __noinline__ void copy_out(uint32_t box, void* p, long long ld, int vec, int row, int rows, int col, int N) {
+  const int lane = lane_id();
+  __syncwarp();
+  if (vec) {
+    const int br = lane >> 2, bu = lane & 3;
+    uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row + br) * ld + col + bu * 8;
+    if (col + bu * 8 < N) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = br + 8 * i;
+        if (row + r < rows) *reinterpret_cast<uint4*>(at) = lds128(box + r * 64 + ((bu ^ ((r >> 1) & 3)) << 4));
+        at += 8 * ld;
+      }
+    }
+  } else {
+    const int c = col + lane, n = min(32, rows - row);
+    uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row) * ld + c;
+    if (c < N) {
+#pragma unroll 4
+      for (int r = 0; r < n; ++r) {
+        const uint32_t w = lds32(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 6) * 2);
+        *at = static_cast<uint16_t>(w >> ((lane & 1) * 16));
+        at += ld;
+      }
+    }
+  }
+  __syncwarp();
+}
+// The other way (the residual): vec by asynchronous copies that the reader waits for.
+static __device__ __noinline__ void copy_in(uint32_t box, const void* p, long long ld, int vec, int row, int rows, int col, int N) {
+  const int lane = lane_id();
+  if (vec) {
+    const int br = lane >> 2, bu = lane & 3;
+    const uint16_t* at = static_cast<const uint16_t*>(p) + static_cast<long long>(row + br) * ld + col + bu * 8;
+    if (col + bu * 8 < N) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = br + 8 * i;
+        if (row + r < rows) cp_async16(box + r * 64 + ((bu ^ ((r >> 1) & 3)) << 4), at);
+        at += 8 * ld;
+      }
+    }
+  } else {
+    const int c = col + lane, n = min(32, rows - row);
+    const uint16_t* at = static_cast<const uint16_t*>(p) + static_cast<long long>(row) * ld + c;
+#pragma unroll 4
+    for (int r = 0; r < n; ++r) {
+      const uint16_t v = c < N ? *at : 0;
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2), "h"(v)
+                   : "memory");
+      at += ld;
+    }
+  }
+}
+
 template <typename T, int CG, int BN, int LAYOUT, bool GATED, bool GEN>
 __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_constant__ FfnTc p) {
   constexpr bool A_MN = LAYOUT == FFN_TN, B_MN = LAYOUT != FFN_NT;
   constexpr int EW = epi_warps(GEN);
   constexpr int BROWS = BN / CG;             // output columns of B staged by one CTA
   constexpr int OUTW = GATED ? BN / 2 : BN;  // output columns of a tile
-  constexpr uint32_t B_BYTES = b_bytes(CG, BN), STAGE = stage_bytes(CG, BN);
+  constexpr uint32_t B_BYTES = b_bytes(CG, BN);
   static_assert(!(GATED && LAYOUT != FFN_NT) && !(GEN && BROWS != 128) && OUTW % 64 == 0, "");
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sA = smem;
-  uint8_t* sB = smem + p.stages * A_BYTES;
-  uint8_t* slots = smem + p.stages * STAGE;
-  float* sbias = reinterpret_cast<float*>(slots + 8 * SLOT);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sbias + 8 * 32);
-  uint64_t* empty = full + 8;
-  uint64_t* tfull = empty + 8;
-  uint64_t* tempty = tfull + 2;
-  uint64_t* drain = tempty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const int stages = p.stages;
+  // A boxes hold a_rows rows (128, fewer when M is smaller): an MMA still reads 128, the rows behind
+  // belong to the next box or to B and only reach accumulator rows that nobody reads
+  const uint32_t a_bytes = A_MN ? A_BYTES : static_cast<uint32_t>(p.a_rows) * BK * 2;
+  const uint32_t sA = smem, sB = smem + stages * a_bytes;
+  const uint32_t boxes = smem + p.ring;
+  const uint32_t sbias = boxes + EW * p.boxes * SLOT;
+  const uint32_t full = sbias + BIAS_BYTES, empty = full + 64, tfull = empty + 64, tempty = tfull + 16, drain = tempty + 16;
+  const uint32_t tmem_slot = drain + 8, abort_word = tmem_slot + 4;
 
   grid_dep_launch();
   const int warp = __shfl_sync(0xffffffffu, warp_id(), 0), lane = lane_id();
-  const int crank = CG == 2 || p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int split = p.split;
+  const int crank = CG == 2 || split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const uint32_t rank = CG == 2 ? static_cast<uint32_t>(crank) : 0u;
   const bool leader = rank == 0;
-  const int worker = CG == 2 ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x) / p.split;
-  const bool save = p.pre[0].p != nullptr;
+  const int worker = CG == 2 ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x) >> p.split_log2;
+  const Waiter wait = {abort_word, p.err};
+  uint32_t tmem_base = 0;
 
-  if (warp == 0 && elect_one()) {
-    for (int s = 0; s < p.stages; ++s) {
-      mbar_init(&full[s], GEN ? GW * CG : 1);
-      mbar_init(&empty[s], 1);
+  if (warp == 0) {
+    if (elect_one()) {
+      for (int s = 0; s < stages; ++s) {
+        bar_init(full + s * 8, GEN ? GW * CG : 1);
+        bar_init(empty + s * 8, 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        bar_init(tfull + b * 8, 1);
+        bar_init(tempty + b * 8, EW * CG);
+      }
+      bar_init(drain, 1);
+      sts32(abort_word, 0u);
+      fence_mbar_init();
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], EW * CG);
-    }
-    mbar_init(drain, 1);
-    *abort_flag = 0;
-    fence_mbar_init();
-    if constexpr (!GEN) {
-      tma_prefetch_desc(&p.ma[0]);
-      tma_prefetch_desc(&p.mb[0]);
-      if (GATED || p.segs > 1) tma_prefetch_desc(&p.mb[1]);
-      if (p.segs > 1) tma_prefetch_desc(&p.ma[1]);
-    }
+    __syncwarp();
   }
   if (warp == 1) {
     if constexpr (CG == 2) {
-      tmem_alloc_pair(tmem_slot, tmem_cols(BN));
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(tmem_cols(BN)));
       tmem_relinquish_pair();
     } else {
-      tmem_alloc(tmem_slot, tmem_cols(BN));
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(tmem_cols(BN)));
       tmem_relinquish();
     }
   }
+  // Barriers initialised and TMEM allocated, in both CTAs of a pair. The producer of a single CTA
+  // needs nothing from the other warps: it only arrives and starts to load.
   tc_fence_before();
-  if constexpr (CG == 2)
-    cluster_sync();  // barriers of both CTAs initialised, TMEM allocated in both
-  else
-    __syncthreads();
+  if constexpr (CG == 2) {
+    cluster_sync();
+  } else if (!GEN && warp == 0) {
+    asm volatile("bar.arrive 1, %0;" ::"n"(threads_of(GEN)) : "memory");
+  } else {
+    asm volatile("bar.sync 1, %0;" ::"n"(threads_of(GEN)) : "memory");
+  }
   tc_fence_after();
   grid_dep_wait();
-  const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if constexpr (!GEN) {
-      int stage = 0;
-      uint32_t phase = 0;
+      const int kb_seg = p.kb_seg;
+      int stage = 0, round = 0;
+      uint32_t phase = 1;
       bool ok = true;
-      const uint32_t a_box = A_MN ? A_BYTES : static_cast<uint32_t>(p.a_rows) * BK * 2;
-      for (Units u = unit_first(p, worker, crank); ok && unit_ok(p, u); unit_next(p, u)) {
+      for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
         int mt, nt;
-        tile_at(u.tile, p.group, p.m_tiles, p.n_tiles, mt, nt);
+        u.at(mt, nt);
         const int m0 = (mt * CG + static_cast<int>(rank)) * BM;
+        const int n0 = GATED ? nt * OUTW : nt * BN + static_cast<int>(rank) * BROWS;
+#pragma unroll 1
         for (int kb = u.k0; kb < u.k1; ++kb) {
-          ok = warp_wait(&empty[stage], phase ^ 1, abort_flag, p.err, 31);
-          if (!ok) break;
+          const uint32_t fb = full + stage * 8;
+          if (round && !wait(empty + stage * 8, phase, 31)) {  // in the first round every stage is empty
+            ok = false;
+            break;
+          }
+          const int seg = kb >= kb_seg ? 1 : 0;
+          const int k = (kb - (seg ? kb_seg : 0)) * BK;
+          const uint32_t da = sA + stage * a_bytes, db = sB + stage * B_BYTES;
           if (elect_one()) {
-            if (leader) mbar_arrive_expect_tx(&full[stage], CG * (a_box + B_BYTES));
-            const int seg = kb >= p.kb_seg ? 1 : 0;
-            const int k = (kb - seg * p.kb_seg) * BK;
-            uint8_t* da = sA + stage * A_BYTES;
-            uint8_t* db = sB + stage * B_BYTES;
-            const uint32_t fb = CG == 2 ? mapa_shared(smem_u32(&full[stage]), 0) : 0u;
-            auto load = [&](const CUtensorMap* map, void* dst, int x, int y) {
-              if constexpr (CG == 2)
-                tma_load_2d_pair(map, fb, dst, x, y);
-              else
-                tma_load_2d(map, &full[stage], dst, x, y);
-            };
-            const CUtensorMap* ma = seg ? &p.ma[1] : &p.ma[0];
-            const CUtensorMap* mb = seg ? &p.mb[1] : &p.mb[0];
+            if (leader) bar_expect(fb, CG * (a_bytes + B_BYTES));
+            const uint32_t fc = CG == 2 ? mapa_shared(fb, 0) : fb;
+            const CUtensorMap* ma = &p.ma[0] + seg;
+            const CUtensorMap* mb = &p.mb[0] + (GATED ? static_cast<int>(rank) : seg);
             if constexpr (A_MN) {
-              load(ma, da, m0, k);
-              load(ma, da + A_BYTES / 2, m0 + 64, k);
+              tma_box<CG>(ma, fc, da, m0, k);
+              tma_box<CG>(ma, fc, da + A_BYTES / 2, m0 + 64, k);
             } else {
-              load(ma, da, k, m0);
+              tma_box<CG>(ma, fc, da, k, m0);
             }
-            if constexpr (GATED) {  // the tile's columns: OUTW of B0, then OUTW of B1
-              if constexpr (CG == 2) {
-                load(rank ? &p.mb[1] : &p.mb[0], db, k, nt * OUTW);
-              } else {
-                load(&p.mb[0], db, k, nt * OUTW);
-                load(&p.mb[1], db + B_BYTES / 2, k, nt * OUTW);
-              }
-            } else {
-              const int n0 = nt * BN + static_cast<int>(rank) * BROWS;
-              if constexpr (B_MN) {
+            if constexpr (B_MN) {
 #pragma unroll
-                for (int c = 0; c < BROWS / 64; ++c) load(mb, db + c * 8192, n0 + c * 64, k);
-              } else {
-                load(mb, db, k, n0);
-              }
+              for (int c = 0; c < BROWS / 64; ++c) tma_box<CG>(mb, fc, db + c * 8192, n0 + c * 64, k);
+            } else {  // gated: the tile's columns are OUTW of B0 (CTA 0), then OUTW of B1 (CTA 1)
+              tma_box<CG>(mb, fc, db, k, n0);
+              if constexpr (GATED && CG == 1) tma_box<CG>(mb + 1, fc, db + B_BYTES / 2, k, n0);
             }
           }
           __syncwarp();
-          if (++stage == p.stages) {
+          if (++stage == stages) {
             stage = 0;
+            round = 1;
             phase ^= 1;
           }
         }
@@ -441,81 +610,102 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
+    tmem_base = lds32(tmem_slot);
     if (leader) {
       constexpr uint32_t id = idesc<T>(BM * CG, BN, A_MN, B_MN);
       // descriptors of stage 0; a stage or a step of 16 contraction elements adds to the address
       // field (units of 16 bytes)
-      const uint64_t a_desc = A_MN ? sdesc_sw128(smem_u32(sA), 8192, 1024) : sdesc_sw128(smem_u32(sA), 16, 1024);
-      const uint64_t b_desc = B_MN ? sdesc_sw128(smem_u32(sB), 8192, 1024) : sdesc_sw128(smem_u32(sB), 16, 1024);
+      const uint64_t a_desc = A_MN ? sdesc_sw128(sA, 8192, 1024) : sdesc_sw128(sA, 16, 1024);
+      const uint64_t b_desc = B_MN ? sdesc_sw128(sB, 8192, 1024) : sdesc_sw128(sB, 16, 1024);
       constexpr uint32_t a_step = A_MN ? 2048 / 16 : 32 / 16, b_step = B_MN ? 2048 / 16 : 32 / 16;
       int stage = 0, acc = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (Units u = unit_first(p, worker, crank); ok && unit_ok(p, u); unit_next(p, u)) {
+      // The test of the next stage's barrier is issued before this stage's MMAs: its latency (80
+      // cycles) passes while they are issued.
+      bool ready = bar_peek(full, 0);
+      for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
         const int buf = acc & 1;
-        ok = warp_wait(&tempty[buf], ((acc >> 1) & 1) ^ 1, abort_flag, p.err, 32);
+        if (acc >= 2) ok = wait(tempty + buf * 8, ((acc >> 1) + 1) & 1, 32);
         if (!ok) break;
         tc_fence_after();
         const uint32_t d = tmem_base + buf * BN;
+        uint32_t more = 0;  // 0: the tile's first MMA overwrites the accumulator
+#pragma unroll 1
         for (int kb = u.k0; kb < u.k1; ++kb) {
-          ok = warp_wait(&full[stage], phase, abort_flag, p.err, 33);
-          if (!ok) break;
+          if (!__all_sync(0xffffffffu, ready) && !wait(full + stage * 8, phase, 33)) {
+            ok = false;
+            break;
+          }
+          const int next = stage + 1 == stages ? 0 : stage + 1;
+          const uint32_t next_phase = next ? phase : phase ^ 1;
+          ready = bar_peek(full + next * 8, next_phase);
           if constexpr (GEN && CG == 2) fence_cluster();
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t da = a_desc + static_cast<uint32_t>(stage) * (A_BYTES / 16);
+            const uint64_t da = a_desc + static_cast<uint32_t>(stage) * (a_bytes / 16);
             const uint64_t db = b_desc + static_cast<uint32_t>(stage) * (B_BYTES / 16);
+            mma<CG>(d, da, db, id, more);
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k)
-              mma<CG>(d, da + k * a_step, db + k * b_step, id, (kb > u.k0 || k > 0) ? 1u : 0u);
-            commit<CG>(&empty[stage], 0);
-            if constexpr (CG == 2) commit<CG>(&empty[stage], 1);
-            if (kb + 1 == u.k1) {
-              commit<CG>(&tfull[buf], 0);
-              if constexpr (CG == 2) commit<CG>(&tfull[buf], 1);
-            }
+            for (int k = 1; k < BK / 16; ++k) mma<CG>(d, da + k * a_step, db + k * b_step, id, 1u);
+            commit<CG>(empty + stage * 8, 0);
+            if constexpr (CG == 2) commit<CG>(empty + stage * 8, 1);
           }
           __syncwarp();
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          more = 1;
+          stage = next;
+          phase = next_phase;
         }
+        if (!ok) break;
+        if (elect_one()) {
+          commit<CG>(tfull + buf * 8, 0);
+          if constexpr (CG == 2) commit<CG>(tfull + buf * 8, 1);
+        }
+        __syncwarp();
         ++acc;
       }
-      // All MMAs must have finished before TMEM is released.
-      if (elect_one()) commit<CG>(drain, 0);
-      __syncwarp();
-      volatile int no_abort = 0;
-      mbar_wait(drain, 0, &no_abort, nullptr, 0);
+      // Every tile's accumulators have been read (both CTAs' epilogues arrive here), or, after an
+      // abort, at least every MMA has finished: TMEM may be released.
+      for (int b = 0; ok && b < 2; ++b) {
+        const int uses = (acc + 1 - b) / 2;
+        if (uses > 0) ok = wait(tempty + b * 8, (uses - 1) & 1, 36);
+      }
+      if (!ok) {
+        if (elect_one()) commit<CG>(drain, 0);
+        __syncwarp();
+        const long long t0 = clock64();
+        while (!bar_try(drain, 0) && clock64() - t0 < J1_WAIT_CYCLES) {
+        }
+      }
     }
   } else if (GEN && warp >= 2 + EW) {
     // ------------------------------------------------------------ loader warps (GEN)
     const int t = static_cast<int>(threadIdx.x) - 32 * (2 + EW);
+    const int kb_seg = p.kb_seg, M = p.M, N = p.N, K = p.K;
     int stage = 0;
-    uint32_t phase = 0;
+    uint32_t phase = 1;
     bool ok = true;
     GenUnit ga[4], gb[4];
-    for (Units u = unit_first(p, worker, crank); ok && unit_ok(p, u); unit_next(p, u)) {
+    for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
       int mt, nt;
-      tile_at(u.tile, p.group, p.m_tiles, p.n_tiles, mt, nt);
+      u.at(mt, nt);
       const int m0 = (mt * CG + static_cast<int>(rank)) * BM;
       // operands of block kb; B of a single gated CTA is 64 rows of each weight
       auto seg_k = [&](int kb, int& seg) {
-        seg = kb >= p.kb_seg ? 1 : 0;
-        return (kb - seg * p.kb_seg) * BK;
+        seg = kb >= kb_seg ? 1 : 0;
+        return (kb - (seg ? kb_seg : 0)) * BK;
       };
       auto op_a = [&](int seg) {
-        return A_MN ? GenOperand<A_MN>{seg ? p.a[1] : p.a[0], p.K, p.M, 0, m0}
-                    : GenOperand<A_MN>{seg ? p.a[1] : p.a[0], p.M, p.K, m0, 0};
+        return A_MN ? GenOperand<A_MN>{seg ? p.a[1] : p.a[0], K, M, 0, m0}
+                    : GenOperand<A_MN>{seg ? p.a[1] : p.a[0], M, K, m0, 0};
       };
       auto op_b = [&](int seg) {
-        if constexpr (GATED && CG == 2) return GenOperand<B_MN>{rank ? p.b[1] : p.b[0], p.N, p.K, nt * OUTW, 0};
+        if constexpr (GATED && CG == 2) return GenOperand<B_MN>{rank ? p.b[1] : p.b[0], N, K, nt * OUTW, 0};
         if constexpr (GATED && CG == 1)  // box rows 0..63 from B0, 64..127 from B1: units j < 2, j >= 2
-          return GenOperand<B_MN>{seg ? p.b[1] : p.b[0], p.N, p.K, nt * OUTW - (seg ? 64 : 0), 0};
+          return GenOperand<B_MN>{seg ? p.b[1] : p.b[0], N, K, nt * OUTW - (seg ? 64 : 0), 0};
         const int n0 = nt * BN + static_cast<int>(rank) * BROWS;
-        return B_MN ? GenOperand<B_MN>{seg ? p.b[1] : p.b[0], p.K, p.N, 0, n0}
-                    : GenOperand<B_MN>{seg ? p.b[1] : p.b[0], p.N, p.K, n0, 0};
+        return B_MN ? GenOperand<B_MN>{seg ? p.b[1] : p.b[0], K, N, 0, n0}
+                    : GenOperand<B_MN>{seg ? p.b[1] : p.b[0], N, K, n0, 0};
       };
       uint32_t slow_a = 0, slow_b = 0;
       auto load_a = [&](int kb) {
@@ -533,12 +723,13 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
       };
       load_a(u.k0);
       load_b(u.k0);
+#pragma unroll 1
       for (int kb = u.k0; kb < u.k1; ++kb) {
-        ok = warp_wait(&empty[stage], phase ^ 1, abort_flag, p.err, 34);
+        ok = wait(empty + stage * 8, phase, 34);
         if (!ok) break;
         int seg;
         const int k = seg_k(kb, seg);
-        op_a(seg).store(ga, slow_a, t, k, sA + stage * A_BYTES);
+        op_a(seg).store(ga, slow_a, t, k, sA + stage * a_bytes);
         if (kb + 1 < u.k1) load_a(kb + 1);
         if constexpr (GATED && CG == 1)
           op_b(0).store2(gb, slow_b, t, k, sB + stage * B_BYTES, op_b(1));
@@ -549,11 +740,11 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
         __syncwarp();
         if (lane == 0) {
           if constexpr (CG == 2)
-            mbar_arrive_cluster(mapa_shared(smem_u32(&full[stage]), 0));
+            mbar_arrive_cluster(mapa_shared(full + stage * 8, 0));
           else
-            mbar_arrive(&full[stage]);
+            bar_arrive(full + stage * 8);
         }
-        if (++stage == p.stages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1;
         }
@@ -562,141 +753,54 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
   } else {
     // ------------------------------------------------------------ epilogue warps
     const int e = warp - 2;
-    const int q = warp & 3;              // TMEM lane quarter this warp may access
+    const int q = warp & 3;                // TMEM lane quarter this warp may access
     constexpr int COLS = OUTW / (EW / 4);  // output columns of this warp
     const int c0 = (e >> 2) * COLS;
-    uint8_t* box = slots + static_cast<uint32_t>(e) * SLOT;
-    float* wbias = sbias + e * 32;
+    const int M = p.M, N = p.N, act = p.act;
+    const bool save = p.pre[0].p != nullptr, residual = !GATED && p.residual.p != nullptr;
+    const uint32_t box = boxes + static_cast<uint32_t>(e) * p.boxes * SLOT;  // output, then pre-activations
+    const uint32_t wbias = sbias + e * 256;
+    const uint32_t own = box + lane * 64;  // this thread's row, unit u at own + ((u ^ sw) << 4)
     const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
-    // copying a box out (or in): rows br + 8 i, 16-byte unit bu
-    const int br = lane >> 2, bu = lane & 3;
-    uint4 rv[4];            // residual of the chunk to come
-    float nb0 = 0.f, nb1 = 0.f;  // its biases, one column per lane
+    tmem_base = lds32(tmem_slot);
 
-    // One box holds 32 rows x 32 columns, 64 bytes a row, unit u of row r at (u ^ (r >> 1 & 3)).
-    auto put_row = [&](const float (&v)[32]) {
+    // What the chunk at (row, col) needs beside its accumulators: biases to the warp's bias rows,
+    // the residual to the output box. Called once everything of the chunk before has left the box.
+    auto fetch = [&](int row, int col) {
+      const bool in = col + lane < N;
+      sts32(wbias + lane * 4, p.bias[0] && in ? __float_as_uint(p.bias[0][col + lane]) : 0u);
+      if constexpr (GATED) sts32(wbias + 128 + lane * 4, p.bias[1] && in ? __float_as_uint(p.bias[1][col + lane]) : 0u);
+      if (residual) copy_in(box, p.residual.p, p.residual.ld, p.vec_res, row, M, col, N);
+    };
+    auto add16 = [&](uint32_t bias, const uint32_t (&r)[16], float (&v)[16]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint4 w;
-        w.x = Elem<T>::pack(v[8 * i], v[8 * i + 1]);
-        w.y = Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]);
-        w.z = Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]);
-        w.w = Elem<T>::pack(v[8 * i + 6], v[8 * i + 7]);
-        *reinterpret_cast<uint4*>(box + lane * 64 + ((static_cast<uint32_t>(i) ^ sw) << 4)) = w;
+        const uint4 b = lds128(bias + i * 16);
+        v[4 * i] = __uint_as_float(r[4 * i]) + __uint_as_float(b.x);
+        v[4 * i + 1] = __uint_as_float(r[4 * i + 1]) + __uint_as_float(b.y);
+        v[4 * i + 2] = __uint_as_float(r[4 * i + 2]) + __uint_as_float(b.z);
+        v[4 * i + 3] = __uint_as_float(r[4 * i + 3]) + __uint_as_float(b.w);
       }
     };
-    // v through the box to rows [row, row + 32) below `rows`, columns [col, col + 32) of m.
-    auto send = [&](const FfnMat& m, bool vec, int row, int rows, int col, const float (&v)[32]) {
-      put_row(v);
-      __syncwarp();
-      if (vec) {
-        uint16_t* at = static_cast<uint16_t*>(const_cast<void*>(m.p)) + static_cast<long long>(row + br) * m.ld + col + bu * 8;
-        const bool in = col + bu * 8 < p.N;
+    auto put16 = [&](uint32_t at, int j, const float (&v)[16]) {  // two units of this thread's row
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = br + 8 * i;
-          const uint4 w = *reinterpret_cast<const uint4*>(box + r * 64 + ((bu ^ ((r >> 1) & 3)) << 4));
-          if (in && row + r < rows) *reinterpret_cast<uint4*>(at) = w;
-          at += 8 * m.ld;
-        }
-      } else {
-        const int c = col + lane, n = min(32, rows - row);
-        uint16_t* at = static_cast<uint16_t*>(const_cast<void*>(m.p)) + static_cast<long long>(row) * m.ld + c;
-        if (c < p.N) {
-#pragma unroll 4
-          for (int r = 0; r < n; ++r) {
-            *at = *reinterpret_cast<const uint16_t*>(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
-            at += m.ld;
-          }
-        }
-      }
-      __syncwarp();
-    };
-    auto fetch = [&](int row, int col) {  // what the chunk at (row, col) needs beside its accumulators
-      nb0 = p.bias[0] && col + lane < p.N ? p.bias[0][col + lane] : 0.f;
-      if constexpr (GATED) {
-        nb1 = p.bias[1] && col + lane < p.N ? p.bias[1][col + lane] : 0.f;
-      } else if (p.residual.p && p.vec_res) {
-        const int c = col + bu * 8;
-        const uint16_t* at = static_cast<const uint16_t*>(p.residual.p) + static_cast<long long>(row + br) * p.residual.ld + c;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          rv[i] = make_uint4(0u, 0u, 0u, 0u);
-          if (row + br + 8 * i < p.M && c < p.N) rv[i] = *reinterpret_cast<const uint4*>(at);
-          at += 8 * p.residual.ld;
-        }
-      }
-    };
-    auto add_bias = [&](float b, float (&v)[32]) {
-      wbias[lane] = b;
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 x = reinterpret_cast<const float4*>(wbias)[i];
-        v[4 * i] += x.x;
-        v[4 * i + 1] += x.y;
-        v[4 * i + 2] += x.z;
-        v[4 * i + 3] += x.w;
-      }
-      __syncwarp();
-    };
-    // Accumulators of 32 columns from `col`, row `row + lane` -> results.
-    auto finish = [&](float (&v)[32], float (&g)[32], int row, int col) {
-      if (p.bias[0]) add_bias(nb0, v);
-      if (save) send(p.pre[0], p.vec_pre, row, p.M, col, v);
-      act_all<32>(p.act, v);
-      if constexpr (GATED) {
-        if (p.bias[1]) add_bias(nb1, g);
-        if (save) send(p.pre[1], p.vec_pre, row, p.M, col, g);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= g[i];
-      } else if (p.residual.p) {
-        if (p.vec_res) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = br + 8 * i;
-            *reinterpret_cast<uint4*>(box + r * 64 + ((bu ^ ((r >> 1) & 3)) << 4)) = rv[i];
-          }
-        } else {
-          const int c = col + lane, n = min(32, p.M - row);
-          const uint16_t* at = static_cast<const uint16_t*>(p.residual.p) + static_cast<long long>(row) * p.residual.ld + c;
-#pragma unroll 4
-          for (int r = 0; r < n; ++r) {
-            *reinterpret_cast<uint16_t*>(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) =
-                c < p.N ? *at : 0;
-            at += p.residual.ld;
-          }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 w = *reinterpret_cast<const uint4*>(box + lane * 64 + ((static_cast<uint32_t>(i) ^ sw) << 4));
-          const uint32_t x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 f = Elem<T>::unpack(x[j]);
-            v[8 * i + 2 * j] += f.x;
-            v[8 * i + 2 * j + 1] += f.y;
-          }
-        }
-        __syncwarp();
-      }
-      if (row < p.row1)
-        send(p.out[0], p.vec_out, row, min(p.M, p.rows0), col, v);
-      else
-        send(p.out[1], p.vec_out, row - p.row1, p.M - p.row1, col, v);
+      for (int i = 0; i < 2; ++i)
+        sts128(at + ((static_cast<uint32_t>(2 * j + i) ^ sw) << 4),
+               make_uint4(Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]),
+                          Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7])));
     };
 
     int acc = 0;
     bool ok = true;
-    for (Units u = unit_first(p, worker, crank); ok && unit_ok(p, u); unit_next(p, u), ++acc) {
+    for (Units u(p, worker, crank); ok && u.ok(); u.next(), ++acc) {
       int mt, nt;
-      tile_at(u.tile, p.group, p.m_tiles, p.n_tiles, mt, nt);
+      u.at(mt, nt);
       const int row = (mt * CG + static_cast<int>(rank)) * BM + q * 32;  // this warp's first row
-      const int n0 = nt * OUTW;
-      const int buf = acc & 1;
-      if (p.split == 1 && !p.stream_k && row < p.M && n0 + c0 < p.N) fetch(row, n0 + c0);
-      ok = warp_wait(&tfull[buf], (acc >> 1) & 1, abort_flag, p.err, 35);
+      const int n0 = nt * OUTW + c0;
+      const uint32_t buf = acc & 1;
+      const bool pieces = split > 1 || p.stream_k;
+      if (!pieces && row < M && n0 < N) fetch(row, n0);
+      ok = wait(tfull + buf * 8, (acc >> 1) & 1, 35);
       if (!ok) break;
       tc_fence_after();
       const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
@@ -705,126 +809,191 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
         __syncwarp();
         if (lane == 0) {
           if constexpr (CG == 2)
-            mbar_arrive_remote(mapa_shared(smem_u32(&tempty[buf]), 0));
+            mbar_arrive_remote(mapa_shared(tempty + buf * 8, 0));
           else
-            mbar_arrive(&tempty[buf]);
+            bar_arrive(tempty + buf * 8);
         }
       };
-      if (p.split > 1 || p.stream_k) {
+      if (pieces) {
         // FP32 accumulators as they are, four columns of a row per 16 bytes, lanes side by side:
         // stream-K pieces to the workspace, a cluster's to shared memory (over the idle stages)
-        float4* dst;
-        if (p.stream_k) {
-          const size_t piece = static_cast<size_t>(worker) + u.tile;  // unique and below workers + tiles
-          dst = reinterpret_cast<float4*>(p.partials) + ((piece * CG + rank) * 4 + q) * (BN / 4) * 32;
-        } else {
-          dst = reinterpret_cast<float4*>(smem) + q * (BN / 4) * 32;
-        }
         constexpr int ACC = BN / (EW / 4);  // accumulator columns of this warp
+        // pieces are numbered worker + tile: unique, below workers + tiles
+        float4* dst = reinterpret_cast<float4*>(p.partials) +
+                      (((static_cast<size_t>(worker) + u.tile) * CG + rank) * 4 + q) * (BN / 4) * 32 + lane;
+        const uint32_t sdst = smem + (q * (BN / 4) * 32 + lane) * 16;
 #pragma unroll 1
-        for (int c = (e >> 2) * ACC; c < ((e >> 2) + 1) * ACC; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(tb + c, r);
+        for (int c = (e >> 2) * ACC; row < M && c < ((e >> 2) + 1) * ACC; c += 16) {
+          uint32_t r[16];
+          tmem_ld16(tb + c, r);
           tmem_ld_wait();
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[(c / 4 + i) * 32 + lane] =
-                make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
-                            __uint_as_float(r[4 * i + 3]));
+          for (int i = 0; i < 4; ++i) {
+            if (split > 1)
+              sts128(sdst + (c / 4 + i) * 512, make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]));
+            else
+              dst[(c / 4 + i) * 32] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                                  __uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3]));
+          }
         }
         release();
         continue;
       }
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 32) {
-        uint32_t r0[32], r1[32];
-        tmem_ld32(tb + c0 + c, r0);
-        if constexpr (GATED) tmem_ld32(tb + BN / 2 + c0 + c, r1);
-        tmem_ld_wait();
-        if (c + 32 == COLS) release();
-        if (row >= p.M || n0 + c0 + c >= p.N) continue;
-        float v[32], g[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          v[i] = __uint_as_float(r0[i]);
-          if constexpr (GATED) g[i] = __uint_as_float(r1[i]);
+        const int col = n0 + c;
+        const bool in = row < M && col < N;
+        if (in) {
+          if (residual) cp_async_wait();
+          __syncwarp();  // biases and residual are in place
         }
-        finish(v, g, row, n0 + c0 + c);
-        if (c + 32 < COLS && n0 + c0 + c + 32 < p.N) fetch(row, n0 + c0 + c + 32);
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j) {
+          uint32_t r0[16], r1[16];
+          tmem_ld16(tb + c0 + c + 16 * j, r0);
+          if constexpr (GATED) tmem_ld16(tb + BN / 2 + c0 + c + 16 * j, r1);
+          tmem_ld_wait();
+          if (j == 1 && c + 32 == COLS) release();
+          if (!in) continue;
+          float v[16];
+          add16(wbias + j * 64, r0, v);
+          if (save) put16(own + SLOT, j, v);
+          act_all<16>(act, v);
+          if constexpr (GATED) {
+            float g[16];
+            add16(wbias + 128 + j * 64, r1, g);
+            if (save) put16(own + 2 * SLOT, j, g);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] *= g[i];
+          } else if (residual) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint4 w = lds128(own + ((static_cast<uint32_t>(2 * j + i) ^ sw) << 4));
+              const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = Elem<T>::unpack(x[k]);
+                v[8 * i + 2 * k] += f.x;
+                v[8 * i + 2 * k + 1] += f.y;
+              }
+            }
+          }
+          put16(own, j, v);
+        }
+        if (!in) continue;
+        if (save) {
+          copy_out(box + SLOT, const_cast<void*>(p.pre[0].p), p.pre[0].ld, p.vec_pre, row, M, col, N);
+          if (GATED) copy_out(box + 2 * SLOT, const_cast<void*>(p.pre[1].p), p.pre[1].ld, p.vec_pre, row, M, col, N);
+        }
+        const bool second = row >= p.row1;
+        copy_out(box, const_cast<void*>(second ? p.out[1].p : p.out[0].p), second ? p.out[1].ld : p.out[0].ld, p.vec_out,
+                 second ? row - p.row1 : row, second ? M - p.row1 : min(M, p.rows0), col, N);
+        if (c + 32 < COLS && col + 32 < N) fetch(row, col + 32);
       }
     }
     if constexpr (CG == 1) {
-      if (p.split > 1) {
+      if (split > 1) {
         // All accumulators of the cluster are in shared memory. Units of 32 rows x 8 columns are
         // dealt to the cluster's epilogue warps; a unit's pieces are added in rank order.
+        int mt, nt;
+        tile_at(worker, p.group, p.m_tiles, p.n_tiles, mt, nt);
+        const int quarters = min(4, (M - mt * BM + 31) / 32);  // that hold rows
+        const int units = quarters * (OUTW / 8);
+        const int first = (e << p.split_log2) + crank;
+        auto unit_bias = [&](const float* bias, int unit) {  // lane i < 8: column i
+          const int c = nt * OUTW + unit / quarters * 8 + lane;
+          return bias && lane < 8 && unit < units && c < N ? bias[c] : 0.f;
+        };
+        float b0 = unit_bias(p.bias[0], first), b1 = GATED ? unit_bias(p.bias[1], first) : 0.f;
         cluster_sync();
+        bool left = false;  // this warp has arrived for its last remote read
         if (ok) {
-          int mt, nt;
-          tile_at(worker, p.group, p.m_tiles, p.n_tiles, mt, nt);
 #pragma unroll 1
-          for (int unit = e * p.split + crank; unit < 4 * (OUTW / 8); unit += EW * p.split) {
-            const int uq = unit & 3, c = (unit >> 2) * 8;
+          for (int unit = first; unit < units; unit += EW << p.split_log2) {
+            const int uq = unit % quarters, c = unit / quarters * 8;
             const int row = mt * BM + uq * 32 + lane, col = nt * OUTW + c;
-            if (mt * BM + uq * 32 >= p.M || col >= p.N) continue;
+            if (unit != first) {
+              b0 = unit_bias(p.bias[0], unit);
+              if (GATED) b1 = unit_bias(p.bias[1], unit);
+            }
+            const bool last = unit + (EW << p.split_log2) >= units;
+            if (col >= N) continue;
             float v[8], g[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = g[i] = 0.f;
-            const uint32_t at = static_cast<uint32_t>((uq * (BN / 4) + c / 4) * 512 + lane * 16);
-#pragma unroll 4
-            for (int s = 0; s < p.split; ++s) {
-              const uint32_t base = mapa_shared(smem_u32(smem), s) + at;
+            const uint32_t at = smem + static_cast<uint32_t>((uq * (BN / 4) + c / 4) * 512 + lane * 16);
+#pragma unroll 1
+            for (int s0 = 0; s0 < split; s0 += 2) {  // two CTAs' pieces in flight (split is even)
+              float4 x[2][2], y[2][2];
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const float4 x = ld_cluster(base + i * 512);
-                v[4 * i] += x.x;
-                v[4 * i + 1] += x.y;
-                v[4 * i + 2] += x.z;
-                v[4 * i + 3] += x.w;
-                if constexpr (GATED) {
-                  const float4 y = ld_cluster(base + (BN / 8 + i) * 512);
-                  g[4 * i] += y.x;
-                  g[4 * i + 1] += y.y;
-                  g[4 * i + 2] += y.z;
-                  g[4 * i + 3] += y.w;
+              for (int s = 0; s < 2; ++s) {
+                const uint32_t base = mapa_shared(at, s0 + s);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  x[s][i] = ld_cluster(base + i * 512);
+                  if constexpr (GATED) y[s][i] = ld_cluster(base + (BN / 8 + i) * 512);
                 }
               }
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                  v[4 * i] += x[s][i].x;
+                  v[4 * i + 1] += x[s][i].y;
+                  v[4 * i + 2] += x[s][i].z;
+                  v[4 * i + 3] += x[s][i].w;
+                  if constexpr (GATED) {
+                    g[4 * i] += y[s][i].x;
+                    g[4 * i + 1] += y[s][i].y;
+                    g[4 * i + 2] += y[s][i].z;
+                    g[4 * i + 3] += y[s][i].w;
+                  }
+                }
+            }
+            if (last) {
+              cluster_arrive();
+              left = true;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              if (p.bias[0] && col + i < p.N) v[i] += p.bias[0][col + i];
-              if (GATED && p.bias[1] && col + i < p.N) g[i] += p.bias[1][col + i];
+              v[i] += __shfl_sync(0xffffffffu, b0, i);
+              if constexpr (GATED) g[i] += __shfl_sync(0xffffffffu, b1, i);
             }
-            if (row < p.M) {
-              if (save) store_row8<T>(p.pre[0], p.vec_pre, row, col, p.N, v);
-              if (GATED && save) store_row8<T>(p.pre[1], p.vec_pre, row, col, p.N, g);
-              act_all<8>(p.act, v);
+            if (row < M) {
+              if (save) store_row8<T>(p.pre[0], p.vec_pre, row, col, N, v);
+              if (GATED && save) store_row8<T>(p.pre[1], p.vec_pre, row, col, N, g);
+              act_all<8>(act, v);
               if constexpr (GATED) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] *= g[i];
-              } else if (p.residual.p) {
+              } else if (residual) {
                 const long long at_r = static_cast<long long>(row) * p.residual.ld + col;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                  if (col + i < p.N) v[i] += Elem<T>::load(p.residual.p, at_r + i);
+                  if (col + i < N) v[i] += Elem<T>::load(p.residual.p, at_r + i);
               }
               const int orow = row < p.row1 ? row : row - p.row1;
               if (row >= p.row1 || row < p.rows0)
-                store_row8<T>(row < p.row1 ? p.out[0] : p.out[1], p.vec_out, orow, col, p.N, v);
+                store_row8<T>(row < p.row1 ? p.out[0] : p.out[1], p.vec_out, orow, col, N, v);
             }
           }
         }
+        if (!left) cluster_arrive();
       }
     }
   }
-  if (CG == 1 && p.split > 1 && (warp < 2 || warp >= 2 + EW)) cluster_sync();  // meets the epilogue warps' one
 
-  tc_fence_before();
-  if (CG == 2 || p.split > 1)
-    cluster_sync();  // every role of every CTA is done, the MMAs have drained
-  else
-    __syncthreads();
-  tc_fence_after();
+  // The epilogue warps end here: nothing below waits for their stores. What is left is to free
+  // TMEM once they have read it, and to stay until no CTA of the cluster needs this one.
+  if (warp >= 2) return;
+  if constexpr (CG == 2) {
+    cluster_sync();
+  } else if (split > 1) {
+    cluster_sync();  // meets the arrivals before the sums ...
+    cluster_sync();  // ... and after them
+  }
   if (warp == 1) {
+    tc_fence_after();
     if constexpr (CG == 2)
       tmem_dealloc_pair(tmem_base, tmem_cols(BN));
     else
@@ -846,14 +1015,11 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Ffn
   const int row = mt * CG * BM + rq * 32, col = nt * BN + chunk * 32;
   grid_dep_wait();
   if (row >= p.M || col >= p.N) return;
-  const long long all = static_cast<long long>(p.tiles) * p.kb, b0 = static_cast<long long>(tile) * p.kb, b1 = b0 + p.kb;
-  // worker w holds blocks [all w / W, all (w + 1) / W): the one that holds block b0 first
-  int w = static_cast<int>(b0 * p.workers / all);
-  while (all * (w + 1) / p.workers <= b0) ++w;
-  while (w > 0 && all * w / p.workers > b0) --w;
+  // the workers whose shares [share_begin(w), share_begin(w + 1)) meet the tile's blocks [b0, b1)
+  const int b0 = tile * p.kb, b1 = b0 + p.kb;
+  int w = b0 < (p.share + 1) * p.share_more ? b0 / (p.share + 1) : (b0 - p.share_more) / p.share;
   float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (; w < p.workers && all * w / p.workers < b1; ++w) {
-    if (all * (w + 1) / p.workers == all * w / p.workers) continue;
+  for (; w < p.workers && Units::share_begin(p, w) < b1; ++w) {
     const float4 x = reinterpret_cast<const float4*>(
         p.partials)[(((static_cast<size_t>(w) + tile) * CG + rq / 4) * 4 + rq % 4) * (BN / 4) * 32 + (chunk * 8 + cg) * 32 + lane];
     t.x += x.x;
@@ -883,16 +1049,20 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
   auto kern = tc_kernel<T, CG, BN, LAYOUT, GATED, GEN>;
   cudaError_t e = set_smem_once(kern, SMEM_MAX, configured);
   if (e != cudaSuccess) return static_cast<int>(e);
-  // no more stages than blocks a CTA will see: a small CTA can share the SM with the kernel before
-  const uint32_t fixed = 1024 + TAIL_BYTES;
-  const int room = static_cast<int>((SMEM_MAX - fixed) / stage_bytes(CG, BN));
+  // no more stages than blocks a CTA will see: a small CTA can share the SM with the kernel before.
+  // A cluster's CTAs leave their accumulators (BM x BN floats) over the stages.
+  p.boxes = 1 + (p.pre[0].p ? (GATED ? 2 : 1) : 0);
+  const uint32_t fixed = 1024 + epi_warps(GEN) * p.boxes * SLOT + BIAS_BYTES + BAR_BYTES;
+  const uint32_t stage = (LAYOUT == FFN_TN ? BM : static_cast<uint32_t>(p.a_rows)) * BK * 2 + b_bytes(CG, BN);
+  const int room = static_cast<int>((SMEM_MAX - fixed) / stage);
   const long long blocks = (static_cast<long long>(p.tiles) * p.kb + p.workers - 1) / p.workers;
   const long long mine = p.split > 1 ? (p.kb + p.split - 1) / p.split : blocks;
-  p.stages = static_cast<int>(std::min<long long>(std::min(room, 8), std::max<long long>(mine, p.split > 1 ? 4 : 2)));
+  p.stages = static_cast<int>(std::min<long long>(std::min(room, 8), std::max<long long>(mine, 2)));
+  p.ring = std::max<uint32_t>(p.stages * stage, std::max<uint32_t>(p.split > 1 ? BM * BN * 4 : 0, A_BYTES + b_bytes(CG, BN)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(CG == 2 ? 2 * p.workers : p.workers * p.split));
   cfg.blockDim = dim3(threads_of(GEN));
-  cfg.dynamicSmemBytes = fixed + p.stages * stage_bytes(CG, BN);
+  cfg.dynamicSmemBytes = fixed + p.ring;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

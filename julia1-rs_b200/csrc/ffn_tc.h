@@ -15,10 +15,14 @@ struct FfnTc {
   int row1, rows0;          // see FfnGemm
   int m_tiles, n_tiles, tiles, group;
   int workers;              // CTAs (CG 1) or CTA pairs (CG 2) that walk the tiles; cluster splits: tiles
+  int split_log2;           // log2 of:
   int split;                // CTAs of a cluster that share a tile's contraction (CG 1), else 1
   int stream_k;             // each worker takes an equal share of all tiles' blocks; FP32 pieces to partials
+  int share, share_more;    // stream-K: blocks of a worker, and how many workers take one more
   float* partials;
   int stages;
+  int boxes;                // 32 x 32 boxes per epilogue warp
+  uint32_t ring;            // shared memory of the stages
   int vec_out, vec_pre, vec_res;  // rows of whole 16-byte units: 16-byte accesses
   int a_rows;               // rows of one A box (K-major A): fewer than 128 when M is smaller
   int* err;
