@@ -65,110 +65,94 @@ __device__ __forceinline__ float recip_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + exp(-x)): relative error about 1e-6 on both tails (exp(-x) may overflow: 1 / inf = 0).
-__device__ __forceinline__ float sigmoid(float x) {
-  return recip_approx(1.f + exp2_approx(-1.4426950408889634f * x));
-}
-// The normal distribution function Phi(h) and density phi(h) from one exponential:
-// erf(x) = 1 - t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2), t = 1 / (1 + p x), x >= 0,
-// absolute error below 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26).
-__device__ __forceinline__ void normal(float h, float& cdf, float& pdf) {
-  const float x = fabsf(h) * 0.70710678118654752f;
-  const float t = recip_approx(fmaf(0.3275911f, x, 1.f));
-  const float e = exp2_approx(-1.4426950408889634f * x * x);
-  float s = fmaf(t, 1.061405429f, -1.453152027f);
-  s = fmaf(t, s, 1.421413741f);
-  s = fmaf(t, s, -0.284496736f);
-  s = fmaf(t, s, 0.254829592f);
-  s = 0.5f * s * t * e;  // Phi(-|h|)
-  cdf = h < 0.f ? s : 1.f - s;
-  pdf = 0.3989422804014327f * e;
+// 1 / (1 + 2^x), the logistic function of -x ln 2: relative error about 1e-6 on both tails (2^x may
+// overflow: 1 / inf = 0).
+__device__ __forceinline__ float logistic2(float x) { return recip_approx(1.f + exp2_approx(x)); }
+
+// Every activation here but ReLU is p times a logistic function of an odd polynomial of p, and all
+// are evaluated that way, with one exponential and one reciprocal per value:
+//   silu       p / (1 + 2^(-p log2 e))
+//   gelu_tanh  0.5 (1 + tanh z) = 1 / (1 + 2^(-2 z log2 e)),  z = sqrt(2/pi) (p + 0.044715 p^3)
+//   gelu       Phi(p) = 1 / (1 + 2^(-p R(p^2))): R(p^2) = log2(Phi / (1 - Phi)) / p is smooth and even; a
+//              polynomial of degree 6 in p^2, fitted here by reweighted least squares on |p| <= 6 to the
+//              smallest maximal error of Phi, is within 3e-8 of Phi (5e-8 in FP32 arithmetic), and its
+//              leading coefficient keeps it growing beyond.
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTanhA = -2.302208198144325f;                // -2 sqrt(2 / pi) log2(e)
+constexpr float kTanhB = -2.302208198144325f * 0.044715f;
+__host__ __device__ constexpr float gelu_coef(int k) {  // minus the coefficient of p^(2 k) in R
+  return k == 0   ? -2.3022093772888184f
+         : k == 1 ? -0.10483512282371521f
+         : k == 2 ? 9.404900629306212e-05f
+         : k == 3 ? 1.5958001313265413e-04f
+         : k == 4 ? -1.1439842637628317e-05f
+         : k == 5 ? 3.8163187809914234e-07f
+                  : -5.06724973092787e-09f;
 }
 
-constexpr float kTanhScale2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-
-// act(p). The negative tails go to 0 also where p itself overflows to -inf; NaN stays NaN.
+// Minus the exponent (log2) of the logistic function, of a value t = p^2 beside p.
 template <int ACT>
-__device__ __forceinline__ float act_value(float p) {
-  if constexpr (ACT == J1_ACT_RELU) return p < 0.f ? 0.f : p;
+__device__ __forceinline__ float logit2(float p, float t) {
   if constexpr (ACT == J1_ACT_GELU) {
-    float cdf, pdf;
-    const float h = max_nan(p, -40.f);
-    normal(h, cdf, pdf);
-    return h * cdf;
-  }
-  if constexpr (ACT == J1_ACT_GELU_TANH) {  // 0.5 (1 + tanh z) = sigmoid(2 z)
-    const float h = max_nan(p, -40.f);
-    return h * sigmoid(kTanhScale2 * fmaf(0.044715f * h * h, h, h));
-  }
-  if constexpr (ACT == J1_ACT_SILU) {
-    const float h = max_nan(p, -200.f);
-    return h * sigmoid(h);
-  }
-  return p;
-}
-
-// act of two values. GELU: erf(x) = x P(x^2) / Q(x^2) for |x| <= 4 with P of degree 6 and Q of
-// degree 4 in x^2 (the Eigen / XLA single-precision rational, within 1.2e-7 of erf), evaluated
-// on pairs with packed FP32 arithmetic: no exponential, a reciprocal per value, and half the
-// instructions. x = p / sqrt(2) is folded into the coefficients. Below the clamp the product
-// uses the clamped p, so a far negative p gives 0 (to 4e-7) and not p times an error.
-template <int ACT>
-__device__ __forceinline__ void act_pair(float& a, float& b) {
-  if constexpr (ACT == J1_ACT_GELU) {
-    constexpr float kClamp = 5.656854f;  // 4 sqrt(2)
-    const float la = max_nan(a, -kClamp), lb = max_nan(b, -kClamp);
-    const uint64_t x = f2pack(fminf(la, kClamp), fminf(lb, kClamp));
-    const uint64_t t = mul2(x, x);
-    auto c2 = [](float c) { return f2pack(c, c); };
-    uint64_t p = c2(-3.01199018e-12f);
-    p = fma2(p, t, c2(6.1223987e-10f));
-    p = fma2(p, t, c2(-9.28530142e-08f));
-    p = fma2(p, t, c2(-5.03151205e-06f));
-    p = fma2(p, t, c2(-0.00012992922f));
-    p = fma2(p, t, c2(-0.00104460877f));
-    p = fma2(p, t, c2(-0.011381614f));
-    uint64_t q = c2(-9.10379526e-07f);
-    q = fma2(q, t, c2(-2.6671758e-05f));
-    q = fma2(q, t, c2(-0.000420706754f));
-    q = fma2(q, t, c2(-0.00368666439f));
-    q = fma2(q, t, c2(-0.01426474f));
-    float q0, q1;
-    f2unpack(q, q0, q1);
-    const uint64_t erf = mul2(mul2(x, p), f2pack(recip_approx(q0), recip_approx(q1)));
-    const uint64_t h = mul2(f2pack(la, lb), c2(0.5f));
-    f2unpack(fma2(h, erf, h), a, b);
+    float r = gelu_coef(6);
+#pragma unroll
+    for (int k = 5; k >= 0; --k) r = fmaf(r, t, gelu_coef(k));
+    return r * p;
+  } else if constexpr (ACT == J1_ACT_GELU_TANH) {
+    return p * fmaf(kTanhB, t, kTanhA);
   } else {
-    a = act_value<ACT>(a);
-    b = act_value<ACT>(b);
+    return -kLog2e * p;
   }
 }
 
-// act'(p) and act(p). The slopes are constant to FP32 beyond |p| = 40; clamping there keeps
-// 0 * inf out of them.
+// act of a pair of values (packed FP32 arithmetic around the exponentials and reciprocals).
+template <int ACT>
+__device__ __forceinline__ uint64_t act_pair(uint64_t p) {
+  if constexpr (ACT == J1_ACT_NONE) return p;
+  float a, b;
+  if constexpr (ACT == J1_ACT_RELU) {
+    f2unpack(p, a, b);
+    return f2pack(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);  // keeps NaN
+  }
+  auto c2 = [](float c) { return f2pack(c, c); };
+  uint64_t x;
+  if constexpr (ACT == J1_ACT_GELU) {
+    const uint64_t t = mul2(p, p);
+    x = c2(gelu_coef(6));
+#pragma unroll
+    for (int k = 5; k >= 0; --k) x = fma2(x, t, c2(gelu_coef(k)));
+    x = mul2(x, p);
+  } else if constexpr (ACT == J1_ACT_GELU_TANH) {
+    x = mul2(p, fma2(mul2(p, p), c2(kTanhB), c2(kTanhA)));
+  } else {
+    x = mul2(p, c2(-kLog2e));
+  }
+  f2unpack(x, a, b);
+  f2unpack(add2(f2pack(exp2_approx(a), exp2_approx(b)), c2(1.f)), a, b);
+  return mul2(p, f2pack(recip_approx(a), recip_approx(b)));
+}
+
+// act'(p) and act(p). With s the logistic function and x(p) its argument, act = p s and act' = s +
+// p s (1 - s) x'(p); for gelu p s (1 - s) x' is p phi(p), taken from the density itself. The slopes
+// are constant to FP32 beyond |p| = 40; clamping there keeps 0 * inf out of them.
 template <int ACT>
 __device__ __forceinline__ void act_slope(float p, float& slope, float& value) {
-  const float h = min_nan(max_nan(p, -40.f), 40.f);
-  if constexpr (ACT == J1_ACT_RELU) {
-    slope = p > 0.f ? 1.f : 0.f;
-    value = p < 0.f ? 0.f : p;
-  } else if constexpr (ACT == J1_ACT_GELU) {
-    float cdf, pdf;
-    normal(h, cdf, pdf);
-    slope = fmaf(h, pdf, cdf);
-    value = max_nan(p, -40.f) * cdf;
-  } else if constexpr (ACT == J1_ACT_GELU_TANH) {
-    const float h2 = h * h;
-    const float s = sigmoid(kTanhScale2 * fmaf(0.044715f * h2, h, h));
-    slope = fmaf(h * (s * (1.f - s)), kTanhScale2 * fmaf(3.f * 0.044715f, h2, 1.f), s);
-    value = max_nan(p, -40.f) * s;
-  } else if constexpr (ACT == J1_ACT_SILU) {
-    const float s = sigmoid(h);
-    slope = fmaf(h * s, 1.f - s, s);
-    value = max_nan(p, -40.f) * s;
-  } else {
+  if constexpr (ACT == J1_ACT_NONE) {
     slope = 1.f;
     value = p;
+  } else if constexpr (ACT == J1_ACT_RELU) {
+    slope = p > 0.f ? 1.f : 0.f;
+    value = p < 0.f ? 0.f : p;
+  } else {
+    const float low = max_nan(p, -40.f), h = min_nan(low, 40.f), t = h * h;
+    const float s = logistic2(logit2<ACT>(h, t));
+    value = low * s;
+    if constexpr (ACT == J1_ACT_GELU)
+      slope = fmaf(h, 0.3989422804014327f * exp2_approx(-0.5f * kLog2e * t), s);
+    else if constexpr (ACT == J1_ACT_GELU_TANH)
+      slope = fmaf(h * (s * (1.f - s)), 1.5957691216057308f * fmaf(3.f * 0.044715f, t, 1.f), s);
+    else
+      slope = fmaf(h * s, 1.f - s, s);
   }
 }
 

@@ -19,7 +19,7 @@
 //   in the accumulator's own layout and a second kernel adds a tile's pieces in order.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocator and MMA issuer (even CTA), then the
-// epilogue warps (eight: two per TMEM lane quarter, each on half of the tile's columns). GEN:
+// epilogue warps (four to sixteen: those of a TMEM lane quarter take its 32-column chunks in turn). GEN:
 // operands whose rows do not start on 16-byte boundaries cannot be read by TMA; eight loader
 // warps (and four epilogue warps) load aligned 16-byte pieces, shift them into place and store
 // the boxes a TMA load would have written.
@@ -52,13 +52,19 @@ namespace ffn {
 constexpr int BM = 128;  // rows of a tile per CTA
 constexpr int BK = 64;   // contraction elements per stage
 constexpr int GW = 8;    // loader warps (GEN): each thread owns 4 units of A and 4 of B
-__host__ __device__ constexpr int epi_warps(bool gen) { return gen ? 4 : 8; }
-__host__ __device__ constexpr int threads_of(bool gen) { return 32 * (2 + epi_warps(gen) + (gen ? GW : 0)); }
+// Epilogue warps. A linear forward tile on a pair has up to 32,768 activations per CTA, each with an
+// exponential and a reciprocal: with two warps per SM sub-partition their latencies were not hidden
+// (131072 x 1152 x 768 with GELU 326 us, without 182 us), with four they are (219 us). Gated tiles
+// have half of them, products without an activation none: eight warps leave room for more stages.
+__host__ __device__ constexpr int epi_warps(int cg, int bn, int layout, bool gated, bool gen) {
+  return gen ? 4 : cg == 2 && layout == FFN_NT && !gated ? (bn == 192 ? 12 : 16) : 8;
+}
+__host__ __device__ constexpr int threads_of(int ew, bool gen) { return 32 * (2 + ew + (gen ? GW : 0)); }
 constexpr uint32_t SLOT = 32 * 32 * 2;  // one 32 x 32 output box
 constexpr uint32_t A_BYTES = BM * BK * 2;
 constexpr uint32_t SMEM_MAX = 232448;
 // bias of the chunk at hand per epilogue warp (two rows of 32 floats), barriers
-constexpr uint32_t BIAS_BYTES = 8 * 2 * 32 * 4, BAR_BYTES = 256;
+constexpr uint32_t BIAS_BYTES = 2 * 32 * 4, BAR_BYTES = 256;
 
 __host__ __device__ constexpr uint32_t b_bytes(int cg, int bn) { return static_cast<uint32_t>(bn / cg) * BK * 2; }
 __host__ __device__ constexpr uint32_t tmem_cols(int bn) { return bn > 128 ? 512 : bn > 64 ? 256 : 128; }
@@ -397,12 +403,12 @@ struct GenOperand {
 };
 
 template <int ACT, int W>
-__device__ __forceinline__ void act_all(float (&v)[W]) {
+__device__ __forceinline__ void act_all(uint64_t (&v)[W]) {
 #pragma unroll
-  for (int i = 0; i < W; i += 2) act_pair<ACT>(v[i], v[i + 1]);
+  for (int i = 0; i < W; ++i) v[i] = act_pair<ACT>(v[i]);
 }
 template <int W>
-__device__ __forceinline__ void act_all(int act, float (&v)[W]) {
+__device__ __forceinline__ void act_all(int act, uint64_t (&v)[W]) {
   switch (act) {
     case J1_ACT_RELU: act_all<J1_ACT_RELU, W>(v); break;
     case J1_ACT_GELU: act_all<J1_ACT_GELU, W>(v); break;
@@ -411,13 +417,19 @@ __device__ __forceinline__ void act_all(int act, float (&v)[W]) {
     default: break;
   }
 }
+// A pair of FP32 values rounded to two elements.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(uint64_t v) {
+  float lo, hi;
+  f2unpack(v, lo, hi);
+  return Elem<T>::pack(lo, hi);
+}
 
 // 8 results of one row to m[row, col ...]: 16 bytes, or element by element up to column N.
 template <typename T>
-__device__ __forceinline__ void store_row8(const FfnMat& m, bool vec, long long row, int col, int N, const float (&v)[8]) {
+__device__ __forceinline__ void store_row8(const FfnMat& m, bool vec, long long row, int col, int N, const uint64_t (&v)[4]) {
   uint16_t* at = static_cast<uint16_t*>(const_cast<void*>(m.p)) + row * m.ld + col;
-  const uint32_t w[4] = {Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]),
-                         Elem<T>::pack(v[6], v[7])};
+  const uint32_t w[4] = {pack2<T>(v[0]), pack2<T>(v[1]), pack2<T>(v[2]), pack2<T>(v[3])};
   if (vec) {
     *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
@@ -485,9 +497,9 @@ static __device__ __noinline__ void copy_in(uint32_t box, const void* p, long lo
 }
 
 template <typename T, int CG, int BN, int LAYOUT, bool GATED, bool GEN>
-__global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_constant__ FfnTc p) {
+__global__ void __launch_bounds__(threads_of(epi_warps(CG, BN, LAYOUT, GATED, GEN), GEN), 1) tc_kernel(const __grid_constant__ FfnTc p) {
   constexpr bool A_MN = LAYOUT == FFN_TN, B_MN = LAYOUT != FFN_NT;
-  constexpr int EW = epi_warps(GEN);
+  constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED, GEN);
   constexpr int BROWS = BN / CG;             // output columns of B staged by one CTA
   constexpr int OUTW = GATED ? BN / 2 : BN;  // output columns of a tile
   constexpr uint32_t B_BYTES = b_bytes(CG, BN);
@@ -501,7 +513,7 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
   const uint32_t sA = smem, sB = smem + stages * a_bytes;
   const uint32_t boxes = smem + p.ring;
   const uint32_t sbias = boxes + EW * p.boxes * SLOT;
-  const uint32_t full = sbias + BIAS_BYTES, empty = full + 64, tfull = empty + 64, tempty = tfull + 16, drain = tempty + 16;
+  const uint32_t full = sbias + EW * BIAS_BYTES, empty = full + 64, tfull = empty + 64, tempty = tfull + 16, drain = tempty + 16;
   const uint32_t tmem_slot = drain + 8, abort_word = tmem_slot + 4;
 
   grid_dep_launch();
@@ -545,9 +557,9 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
   if constexpr (CG == 2) {
     cluster_sync();
   } else if (!GEN && warp == 0) {
-    asm volatile("bar.arrive 1, %0;" ::"n"(threads_of(GEN)) : "memory");
+    asm volatile("bar.arrive 1, %0;" ::"n"(threads_of(EW, GEN)) : "memory");
   } else {
-    asm volatile("bar.sync 1, %0;" ::"n"(threads_of(GEN)) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(threads_of(EW, GEN)) : "memory");
   }
   tc_fence_after();
   grid_dep_wait();
@@ -754,12 +766,12 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
     // ------------------------------------------------------------ epilogue warps
     const int e = warp - 2;
     const int q = warp & 3;                // TMEM lane quarter this warp may access
-    constexpr int COLS = OUTW / (EW / 4);  // output columns of this warp
-    const int c0 = (e >> 2) * COLS;
+    constexpr int PER = EW / 4;            // warps of a quarter: they take its 32-column chunks in turn
+    const int c0 = (e >> 2) * 32;
     const int M = p.M, N = p.N, act = p.act;
     const bool save = p.pre[0].p != nullptr, residual = !GATED && p.residual.p != nullptr;
     const uint32_t box = boxes + static_cast<uint32_t>(e) * p.boxes * SLOT;  // output, then pre-activations
-    const uint32_t wbias = sbias + e * 256;
+    const uint32_t wbias = sbias + e * BIAS_BYTES;
     const uint32_t own = box + lane * 64;  // this thread's row, unit u at own + ((u ^ sw) << 4)
     const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
     tmem_base = lds32(tmem_slot);
@@ -772,22 +784,21 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
       if constexpr (GATED) sts32(wbias + 128 + lane * 4, p.bias[1] && in ? __float_as_uint(p.bias[1][col + lane]) : 0u);
       if (residual) copy_in(box, p.residual.p, p.residual.ld, p.vec_res, row, M, col, N);
     };
-    auto add16 = [&](uint32_t bias, const uint32_t (&r)[16], float (&v)[16]) {
+    auto add16 = [&](uint32_t bias, const uint32_t (&r)[16], uint64_t (&v)[8]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 b = lds128(bias + i * 16);
-        v[4 * i] = __uint_as_float(r[4 * i]) + __uint_as_float(b.x);
-        v[4 * i + 1] = __uint_as_float(r[4 * i + 1]) + __uint_as_float(b.y);
-        v[4 * i + 2] = __uint_as_float(r[4 * i + 2]) + __uint_as_float(b.z);
-        v[4 * i + 3] = __uint_as_float(r[4 * i + 3]) + __uint_as_float(b.w);
+        v[2 * i] = add2(f2pack(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])),
+                        f2pack(__uint_as_float(b.x), __uint_as_float(b.y)));
+        v[2 * i + 1] = add2(f2pack(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
+                            f2pack(__uint_as_float(b.z), __uint_as_float(b.w)));
       }
     };
-    auto put16 = [&](uint32_t at, int j, const float (&v)[16]) {  // two units of this thread's row
+    auto put16 = [&](uint32_t at, int j, const uint64_t (&v)[8]) {  // two units of this thread's row
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         sts128(at + ((static_cast<uint32_t>(2 * j + i) ^ sw) << 4),
-               make_uint4(Elem<T>::pack(v[8 * i], v[8 * i + 1]), Elem<T>::pack(v[8 * i + 2], v[8 * i + 3]),
-                          Elem<T>::pack(v[8 * i + 4], v[8 * i + 5]), Elem<T>::pack(v[8 * i + 6], v[8 * i + 7])));
+               make_uint4(pack2<T>(v[4 * i]), pack2<T>(v[4 * i + 1]), pack2<T>(v[4 * i + 2]), pack2<T>(v[4 * i + 3])));
     };
 
     int acc = 0;
@@ -796,10 +807,10 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
       int mt, nt;
       u.at(mt, nt);
       const int row = (mt * CG + static_cast<int>(rank)) * BM + q * 32;  // this warp's first row
-      const int n0 = nt * OUTW + c0;
+      const int n0 = nt * OUTW;
       const uint32_t buf = acc & 1;
       const bool pieces = split > 1 || p.stream_k;
-      if (!pieces && row < M && n0 < N) fetch(row, n0);
+      if (!pieces && row < M && c0 < OUTW && n0 + c0 < N) fetch(row, n0 + c0);
       ok = wait(tfull + buf * 8, (acc >> 1) & 1, 35);
       if (!ok) break;
       tc_fence_after();
@@ -817,7 +828,7 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
       if (pieces) {
         // FP32 accumulators as they are, four columns of a row per 16 bytes, lanes side by side:
         // stream-K pieces to the workspace, a cluster's to shared memory (over the idle stages)
-        constexpr int ACC = BN / (EW / 4);  // accumulator columns of this warp
+        constexpr int ACC = BN / PER;  // accumulator columns of this warp
         // pieces are numbered worker + tile: unique, below workers + tiles
         float4* dst = reinterpret_cast<float4*>(p.partials) +
                       (((static_cast<size_t>(worker) + u.tile) * CG + rank) * 4 + q) * (BN / 4) * 32 + lane;
@@ -839,8 +850,9 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
         release();
         continue;
       }
+      if (c0 >= OUTW) release();  // more warps than chunks
 #pragma unroll 1
-      for (int c = 0; c < COLS; c += 32) {
+      for (int c = c0; c < OUTW; c += 32 * PER) {
         const int col = n0 + c;
         const bool in = row < M && col < N;
         if (in) {
@@ -850,21 +862,21 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
 #pragma unroll 1
         for (int j = 0; j < 2; ++j) {
           uint32_t r0[16], r1[16];
-          tmem_ld16(tb + c0 + c + 16 * j, r0);
-          if constexpr (GATED) tmem_ld16(tb + BN / 2 + c0 + c + 16 * j, r1);
+          tmem_ld16(tb + c + 16 * j, r0);
+          if constexpr (GATED) tmem_ld16(tb + BN / 2 + c + 16 * j, r1);
           tmem_ld_wait();
-          if (j == 1 && c + 32 == COLS) release();
+          if (j == 1 && c + 32 * PER >= OUTW) release();
           if (!in) continue;
-          float v[16];
+          uint64_t v[8];
           add16(wbias + j * 64, r0, v);
           if (save) put16(own + SLOT, j, v);
-          act_all<16>(act, v);
+          act_all<8>(act, v);
           if constexpr (GATED) {
-            float g[16];
+            uint64_t g[8];
             add16(wbias + 128 + j * 64, r1, g);
             if (save) put16(own + 2 * SLOT, j, g);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] *= g[i];
+            for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], g[i]);
           } else if (residual) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -873,8 +885,7 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const float2 f = Elem<T>::unpack(x[k]);
-                v[8 * i + 2 * k] += f.x;
-                v[8 * i + 2 * k + 1] += f.y;
+                v[4 * i + k] = add2(v[4 * i + k], f2pack(f.x, f.y));
               }
             }
           }
@@ -888,7 +899,7 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
         const bool second = row >= p.row1;
         copy_out(box, const_cast<void*>(second ? p.out[1].p : p.out[0].p), second ? p.out[1].ld : p.out[0].ld, p.vec_out,
                  second ? row - p.row1 : row, second ? M - p.row1 : min(M, p.rows0), col, N);
-        if (c + 32 < COLS && col + 32 < N) fetch(row, col + 32);
+        if (c + 32 * PER < OUTW && col + 32 * PER < N) fetch(row, col + 32 * PER);
       }
     }
     if constexpr (CG == 1) {
@@ -918,9 +929,9 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
             }
             const bool last = unit + (EW << p.split_log2) >= units;
             if (col >= N) continue;
-            float v[8], g[8];
+            uint64_t v[4], g[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = g[i] = 0.f;
+            for (int i = 0; i < 4; ++i) v[i] = g[i] = 0ull;
             const uint32_t at = smem + static_cast<uint32_t>((uq * (BN / 4) + c / 4) * 512 + lane * 16);
 #pragma unroll 1
             for (int s0 = 0; s0 < split; s0 += 2) {  // two CTAs' pieces in flight (split is even)
@@ -938,15 +949,11 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
               for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                  v[4 * i] += x[s][i].x;
-                  v[4 * i + 1] += x[s][i].y;
-                  v[4 * i + 2] += x[s][i].z;
-                  v[4 * i + 3] += x[s][i].w;
+                  v[2 * i] = add2(v[2 * i], f2pack(x[s][i].x, x[s][i].y));
+                  v[2 * i + 1] = add2(v[2 * i + 1], f2pack(x[s][i].z, x[s][i].w));
                   if constexpr (GATED) {
-                    g[4 * i] += y[s][i].x;
-                    g[4 * i + 1] += y[s][i].y;
-                    g[4 * i + 2] += y[s][i].z;
-                    g[4 * i + 3] += y[s][i].w;
+                    g[2 * i] = add2(g[2 * i], f2pack(y[s][i].x, y[s][i].y));
+                    g[2 * i + 1] = add2(g[2 * i + 1], f2pack(y[s][i].z, y[s][i].w));
                   }
                 }
             }
@@ -955,22 +962,26 @@ __global__ void __launch_bounds__(threads_of(GEN), 1) tc_kernel(const __grid_con
               left = true;
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              v[i] += __shfl_sync(0xffffffffu, b0, i);
-              if constexpr (GATED) g[i] += __shfl_sync(0xffffffffu, b1, i);
+            for (int i = 0; i < 4; ++i) {
+              v[i] = add2(v[i], f2pack(__shfl_sync(0xffffffffu, b0, 2 * i), __shfl_sync(0xffffffffu, b0, 2 * i + 1)));
+              if constexpr (GATED)
+                g[i] = add2(g[i], f2pack(__shfl_sync(0xffffffffu, b1, 2 * i), __shfl_sync(0xffffffffu, b1, 2 * i + 1)));
             }
             if (row < M) {
               if (save) store_row8<T>(p.pre[0], p.vec_pre, row, col, N, v);
               if (GATED && save) store_row8<T>(p.pre[1], p.vec_pre, row, col, N, g);
-              act_all<8>(act, v);
+              act_all<4>(act, v);
               if constexpr (GATED) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= g[i];
+                for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], g[i]);
               } else if (residual) {
                 const long long at_r = static_cast<long long>(row) * p.residual.ld + col;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                  if (col + i < N) v[i] += Elem<T>::load(p.residual.p, at_r + i);
+                for (int i = 0; i < 4; ++i) {
+                  const float lo = col + 2 * i < N ? Elem<T>::load(p.residual.p, at_r + 2 * i) : 0.f;
+                  const float hi = col + 2 * i + 1 < N ? Elem<T>::load(p.residual.p, at_r + 2 * i + 1) : 0.f;
+                  v[i] = add2(v[i], f2pack(lo, hi));
+                }
               }
               const int orow = row < p.row1 ? row : row - p.row1;
               if (row >= p.row1 || row < p.rows0)
@@ -1045,6 +1056,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Ffn
 
 template <typename T, int CG, int BN, int LAYOUT, bool GATED, bool GEN>
 int launch_one(FfnTc& p, cudaStream_t stream) {
+  constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED, GEN);
   static std::atomic<unsigned long long> configured{0};
   auto kern = tc_kernel<T, CG, BN, LAYOUT, GATED, GEN>;
   cudaError_t e = set_smem_once(kern, SMEM_MAX, configured);
@@ -1052,7 +1064,7 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
   // no more stages than blocks a CTA will see: a small CTA can share the SM with the kernel before.
   // A cluster's CTAs leave their accumulators (BM x BN floats) over the stages.
   p.boxes = 1 + (p.pre[0].p ? (GATED ? 2 : 1) : 0);
-  const uint32_t fixed = 1024 + epi_warps(GEN) * p.boxes * SLOT + BIAS_BYTES + BAR_BYTES;
+  const uint32_t fixed = 1024 + EW * (p.boxes * SLOT + BIAS_BYTES) + BAR_BYTES;
   const uint32_t stage = (LAYOUT == FFN_TN ? BM : static_cast<uint32_t>(p.a_rows)) * BK * 2 + b_bytes(CG, BN);
   const int room = static_cast<int>((SMEM_MAX - fixed) / stage);
   const long long blocks = (static_cast<long long>(p.tiles) * p.kb + p.workers - 1) / p.workers;
@@ -1061,7 +1073,7 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
   p.ring = std::max<uint32_t>(p.stages * stage, std::max<uint32_t>(p.split > 1 ? BM * BN * 4 : 0, A_BYTES + b_bytes(CG, BN)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(CG == 2 ? 2 * p.workers : p.workers * p.split));
-  cfg.blockDim = dim3(threads_of(GEN));
+  cfg.blockDim = dim3(threads_of(EW, GEN));
   cfg.dynamicSmemBytes = fixed + p.ring;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
