@@ -446,20 +446,25 @@ J1_API j1_status j1_op_attention_noalloc(const void* qkv, int64_t t, int32_t hid
 
 /* ---- the feed-forward block for training and serving (no reference counterpart)
  * Row-major matrices of 16-bit elements on device memory, one token per row; `ld*` are row
- * strides in elements (>= the row's width, any alignment of a whole element; rows that start
- * on 16-byte boundaries take the faster path). Any M >= 0, N >= 1, K >= 1. Weights are used as
- * a checkpoint stores them, [N, K]. Products accumulate in FP32, every epilogue works on the
- * unrounded FP32 values, each result is rounded once. Biases and their gradients are FP32.
+ * strides in elements (>= the row's width, any alignment of a whole element). Any M >= 0,
+ * N >= 1, K >= 1. Weights are used as a checkpoint stores them, [N, K]. Products accumulate in
+ * FP32, every epilogue works on the unrounded FP32 values, each result is rounded once. Biases
+ * and their gradients are FP32.
  *
  * All pointers of a call must be memory of the calling thread's current device, and `stream`
  * a stream of it (NULL: its default stream); other pointers give J1_ERR_INVALID_ARG. Results
  * must not overlap each other or any input, except that j1_op_linear's out may be its residual
  * (same pointer and row stride). Elements between a row's width and its stride are neither
- * read nor written. With sync = 0 the calls only enqueue work and may be captured into a CUDA
- * graph; the first call of each kind on a device loads its kernels and should come before any
- * capture. Nothing is allocated. Device-side timeouts of sync = 0 calls are reported by the
- * next of these calls made with sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Equal
- * inputs give equal bits: no result depends on the order in which blocks finish. */
+ * read nor written. Equal inputs give equal bits: no result depends on the order in which
+ * blocks finish.
+ *
+ * With sync = 0 the calls only enqueue work and may be captured into a CUDA graph; the first
+ * call of each kind on a device loads its kernels and should come before any capture.
+ * Device-side timeouts of sync = 0 calls are reported by the next of these calls made with
+ * sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Operands whose rows all start on 16-byte
+ * boundaries are read in place and nothing is allocated; other operands of a product are copied
+ * first, to stream-ordered memory of a pool of the library, which keeps the most it ever needed
+ * at once. */
 typedef enum j1_dtype { J1_DTYPE_BF16 = 0, J1_DTYPE_FP16 = 1 } j1_dtype;
 typedef enum j1_act {
   J1_ACT_NONE = 0,

@@ -1,5 +1,7 @@
 // j1_op_linear, j1_op_gated and their backward passes: argument checks, workspace layout and
-// the launches. Everything here runs on the host; no call allocates device memory.
+// the launches. Everything here runs on the host. Device memory is only taken for operands whose
+// rows do not start on 16-byte boundaries: the products read such an operand from a copy, in
+// stream-ordered memory of the library's own pool (product() below).
 #include <climits>
 #include <cstdint>
 #include <mutex>
@@ -22,6 +24,9 @@ struct FfnDevice {
   cudaError_t rc = cudaSuccess;
   int* err = nullptr;
   int num_sms = 0;
+  std::once_flag pool_once;
+  cudaError_t pool_rc = cudaSuccess;
+  cudaMemPool_t pool = nullptr;
 };
 FfnDevice g_dev[kMaxDevices];
 
@@ -126,6 +131,8 @@ j1_status finish(FfnDevice* d, cudaStream_t st, int sync) {
   return J1_OK;
 }
 
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
 FfnGemm gemm_for(int dtype, int layout, int M, int N, int K, const FfnDevice* d) {
   FfnGemm g = {};
   g.fp16 = dtype == J1_DTYPE_FP16;
@@ -139,9 +146,70 @@ FfnGemm gemm_for(int dtype, int layout, int M, int N, int K, const FfnDevice* d)
   return g;
 }
 
+// The device's pool, which keeps what it has taken (as a model's workspace does).
+cudaError_t device_pool(FfnDevice* d, int dev) {
+  std::call_once(d->pool_once, [d, dev] {
+    cudaMemPoolProps props = {};
+    props.allocType = cudaMemAllocationTypePinned;
+    props.location.type = cudaMemLocationTypeDevice;
+    props.location.id = dev;
+    d->pool_rc = cudaMemPoolCreate(&d->pool, &props);
+    uint64_t keep = UINT64_MAX;
+    if (d->pool_rc == cudaSuccess) d->pool_rc = cudaMemPoolSetAttribute(d->pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  });
+  return d->pool_rc;
+}
+
+// One product. TMA reads rows on 16-byte boundaries only; other operands are copied first. (Reading
+// them in the product instead, loader warps shifting aligned 16-byte pieces into place, kept the
+// tensor cores waiting: 65536 x 771 x 1155 took 527-606 us. A copy costs its bytes twice.) The memory
+// is taken and given back in stream order: calls on several streams, and captured graphs, have
+// their own.
+j1_status product(FfnGemm& g, FfnDevice* d, int dev, cudaStream_t st, const char* what) {
+  FfnMat* operands[4];
+  FfnCopies c = {};
+  size_t bytes = 0, at[4];
+  const int na = g.segs, nb = g.gated ? 2 : g.segs;
+  for (int i = 0; i < na + nb; ++i) {
+    const bool a = i < na;
+    FfnMat& m = a ? g.a[i] : g.b[i - na];
+    FfnCopy& o = c.m[c.n];
+    o.rows = a ? (g.layout == FFN_TN ? g.K : g.M) : (g.layout == FFN_NT ? g.N : g.K);
+    o.cols = a ? (g.layout == FFN_TN ? g.M : g.K) : (g.layout == FFN_NT ? g.K : g.N);
+    if (o.rows == 1) m.ld = (static_cast<long long>(o.cols) + 7) / 8 * 8;  // one row: the stride is never used
+    if (ffn_rows16(m)) continue;
+    o.src = m;
+    o.dst.ld = (static_cast<long long>(o.cols) + 7) / 8 * 8;
+    operands[c.n] = &m;
+    at[c.n++] = bytes;
+    bytes += up256(static_cast<size_t>(o.rows) * o.dst.ld * 2);
+  }
+  void* mem = nullptr;
+  if (c.n) {
+    if (take_fault(J1_FAULT_ALLOC)) return set_error(J1_ERR_OOM, std::string(what) + ": device allocation failed (injected)");
+    cudaError_t e = device_pool(d, dev);
+    if (e == cudaSuccess) e = cudaMallocFromPoolAsync(&mem, bytes, d->pool, st);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_error(e, what);
+    }
+    for (int i = 0; i < c.n; ++i) {
+      c.m[i].dst.p = static_cast<uint8_t*>(mem) + at[i];
+      *operands[i] = c.m[i].dst;
+    }
+  }
+  int rc = take_fault(J1_FAULT_LAUNCH) ? static_cast<int>(cudaErrorLaunchFailure) : 0;
+  if (!rc && c.n) rc = launch_ffn_copies(c, st);
+  if (!rc) rc = launch_ffn_gemm(g, st);
+  if (mem) {
+    const cudaError_t e = cudaFreeAsync(mem, st);
+    if (!rc) rc = e;
+  }
+  return rc ? cuda_error(static_cast<cudaError_t>(rc), what) : J1_OK;
+}
+
 // ---- backward workspace: gradients at the pre-activations (rows padded to 32 elements; the
 // gated pair side by side), slab sums of the bias gradients, partial products of dw.
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 int pad32(int n) { return (n + 31) / 32 * 32; }
 struct Workspace {
   size_t grads, sums, partials, bytes;  // offsets of the three parts, total
@@ -221,7 +289,7 @@ j1_status j1_op_linear(const j1_linear_args* a, void* stream, int sync) {
       g.residual = {a->residual, a->ldr};
       g.out[0] = {a->out, a->ldo};
       g.pre[0] = {a->pre, a->ldp};
-      FFN_LAUNCH(launch_ffn_gemm(g, st), "linear launch");
+      FFN_TRY(product(g, d, dev, st, "linear launch"));
     }
     return finish(d, st, sync);
   });
@@ -257,7 +325,7 @@ j1_status j1_op_gated(const j1_gated_args* a, void* stream, int sync) {
       g.out[0] = {a->out, a->ldo};
       g.pre[0] = {a->pre_a, a->ldpa};
       g.pre[1] = {a->pre_g, a->ldpg};
-      FFN_LAUNCH(launch_ffn_gemm(g, st), "gated launch");
+      FFN_TRY(product(g, d, dev, st, "gated launch"));
     }
     return finish(d, st, sync);
   });
@@ -303,14 +371,15 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
     uint8_t* base = static_cast<uint8_t*>(a->workspace);
     FfnMat dp = {a->dout, a->lddo};
     const bool products = a->dx || a->dw;
-    if ((slope && products) || a->dbias) {
+    const bool copy = products && (slope || !ffn_rows16(dp));  // both products read it
+    if (copy || a->dbias) {
       FfnGrad k = {};
       k.fp16 = a->dtype == J1_DTYPE_FP16;
       k.act = a->act;
       k.M = a->M, k.N = a->N;
       k.dout = {a->dout, a->lddo};
       k.p0 = {slope ? a->pre : nullptr, a->ldp};
-      if (slope && products) k.d0 = dp = {base + ws.grads, ws.ld};
+      if (copy) k.d0 = dp = {base + ws.grads, ws.ld};
       k.sum0 = a->dbias;
       k.partials = reinterpret_cast<float*>(base + ws.sums);
       FFN_LAUNCH(launch_ffn_grad(k, st), "linear gradient launch");
@@ -320,7 +389,7 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       g.a[0] = dp;
       g.b[0] = {a->w, a->ldw};
       g.out[0] = {a->dx, a->lddx};
-      FFN_LAUNCH(launch_ffn_gemm(g, st), "dx launch");
+      FFN_TRY(product(g, d, dev, st, "dx launch"));
     }
     if (a->dw) {
       FfnGemm g = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
@@ -329,7 +398,7 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       g.out[0] = {a->dw, a->lddw};
       g.partials = reinterpret_cast<float*>(base + ws.partials);
       g.partial_bytes = ws.partial_bytes;
-      FFN_LAUNCH(launch_ffn_gemm(g, st), "dw launch");
+      FFN_TRY(product(g, d, dev, st, "dw launch"));
     }
     return finish(d, st, sync);
   });
@@ -396,7 +465,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
       g.b[0] = {a->wa, a->ldwa};
       g.b[1] = {a->wg, a->ldwg};
       g.out[0] = {a->dx, a->lddx};
-      FFN_LAUNCH(launch_ffn_gemm(g, st), "dx launch");
+      FFN_TRY(product(g, d, dev, st, "dx launch"));
     }
     if (a->dwa) {  // both weights' gradients as one product: rows [0, np) of da | dg are dwa's
       FfnGemm g = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
@@ -408,7 +477,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
       g.out[1] = {a->dwg, a->lddwg};
       g.partials = reinterpret_cast<float*>(base + ws.partials);
       g.partial_bytes = ws.partial_bytes;
-      FFN_LAUNCH(launch_ffn_gemm(g, st), "dw launch");
+      FFN_TRY(product(g, d, dev, st, "dw launch"));
     }
     return finish(d, st, sync);
   });

@@ -13,6 +13,8 @@ struct FfnMat {
   const void* p;
   long long ld;
 };
+// Rows on 16-byte boundaries: what TMA and 16-byte accesses need.
+inline bool ffn_rows16(const FfnMat& m) { return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0; }
 
 // How the operands of out[M, N] = A . B lie in memory (K: the contraction).
 enum FfnLayout : int {
@@ -42,11 +44,23 @@ struct FfnGemm {
   int num_sms;
 };
 
+// The operands a and b must have rows on 16-byte boundaries (ffn_rows16).
 int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream);
 // Workspace that a split contraction of these sizes may take (host arithmetic only).
 size_t ffn_partial_bytes(int M, int N, int K);
 // Device address of the operators' error word on the current device.
 cudaError_t ffn_error_word(int** p);
+
+// Copies of matrices to rows on 16-byte boundaries (dst.ld a multiple of 8).
+struct FfnCopy {
+  FfnMat src, dst;
+  int rows, cols;
+};
+struct FfnCopies {
+  FfnCopy m[4];
+  int n;
+};
+int launch_ffn_copies(const FfnCopies& c, cudaStream_t stream);
 
 // dp = dout * act'(pre) (linear), or da = dout * g * act'(a), dg = dout * act(a) (gated): the
 // gradients at the pre-activations, rounded to the element type, with the column sums of the

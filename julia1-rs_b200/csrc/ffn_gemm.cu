@@ -16,9 +16,6 @@ __device__ int g_ffn_error;
 constexpr int kPairs = 74;                        // most CTA pairs a stream-K product uses
 constexpr size_t kPieceBytes = 256 * 256 * 4;     // FP32 accumulators of a pair
 
-// Rows on 16-byte boundaries: what TMA and 16-byte accesses need.
-bool rows16(const FfnMat& m) { return reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0; }
-
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 struct Plan {
@@ -29,7 +26,7 @@ struct Plan {
 
 // Microseconds per 64-block of a tile and CTA (or pair) and the fixed part of a tile that
 // nothing hides (first loads, last epilogue).
-Plan choose(const FfnGemm& g, bool aligned, int kb) {
+Plan choose(const FfnGemm& g, int kb) {
   const int sms = g.num_sms;
   const auto single = [&](int cfg, int bn, double step) {
     const long long tiles = ceil_div(g.M, 128) * ceil_div(g.N, g.gated ? bn / 2 : bn);
@@ -41,11 +38,11 @@ Plan choose(const FfnGemm& g, bool aligned, int kb) {
     }
     return best;
   };
-  Plan best = aligned ? single(FFN_CG1_128, 128, 0.22) : single(FFN_CG1_128_GEN, 128, 0.6);
+  Plan best = single(FFN_CG1_128, 128, 0.22);
   const auto take = [&](const Plan& p) {
     if (p.us < best.us) best = p;
   };
-  if (aligned && !g.gated) take(single(FFN_CG1_64, 64, 0.13));
+  if (!g.gated) take(single(FFN_CG1_64, 64, 0.13));
   const auto pair = [&](int cfg, int bn, double step) {
     const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
     const int pairs = std::max(1, std::min(kPairs, sms / 2));
@@ -58,8 +55,8 @@ Plan choose(const FfnGemm& g, bool aligned, int kb) {
     }
     return p;
   };
-  take(aligned ? pair(FFN_CG2_256, 256, 0.40) : pair(FFN_CG2_256_GEN, 256, 0.8));
-  if (aligned && g.layout == FFN_NT && !g.gated) take(pair(FFN_CG2_192, 192, 0.31));
+  take(pair(FFN_CG2_256, 256, 0.40));
+  if (g.layout == FFN_NT && !g.gated) take(pair(FFN_CG2_192, 192, 0.31));
   return best;
 }
 
@@ -82,19 +79,14 @@ size_t ffn_partial_bytes(int M, int N, int K) {
 
 int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   FfnTc p = {};
-  bool aligned = true;
   const int nb = g.gated ? 2 : g.segs;
-  for (int i = 0; i < 2; ++i) {
-    p.a[i] = g.a[i], p.b[i] = g.b[i], p.out[i] = g.out[i], p.pre[i] = g.pre[i], p.bias[i] = g.bias[i];
-    if (i < g.segs) aligned = aligned && rows16(g.a[i]);
-    if (i < nb) aligned = aligned && rows16(g.b[i]);
-  }
+  for (int i = 0; i < 2; ++i) p.out[i] = g.out[i], p.pre[i] = g.pre[i], p.bias[i] = g.bias[i];
   p.M = g.M, p.N = g.N, p.K = g.K;
   p.segs = g.segs;
   p.kb_seg = static_cast<int>(ceil_div(g.K, 64));
   if (static_cast<long long>(p.kb_seg) * g.segs > INT_MAX) return static_cast<int>(cudaErrorInvalidValue);
   p.kb = p.kb_seg * g.segs;
-  const Plan plan = choose(g, aligned, p.kb);
+  const Plan plan = choose(g, p.kb);
   p.act = g.act;
   p.row1 = g.row1, p.rows0 = g.rows0;
   const long long m_tiles = ceil_div(g.M, 128 * plan.cg);
@@ -111,27 +103,25 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   p.workers = plan.split > 1 ? p.tiles : plan.stream_k ? slots : std::min(p.tiles, slots);
   p.share = p.tiles * static_cast<long long>(p.kb) / p.workers;
   p.share_more = static_cast<int>(p.tiles * static_cast<long long>(p.kb) % p.workers);
-  p.a_rows = aligned && plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
+  p.a_rows = plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
   p.err = g.err;
   p.residual = g.residual;
-  p.vec_res = g.residual.p && rows16(g.residual) && g.N % 8 == 0;
+  p.vec_res = g.residual.p && ffn_rows16(g.residual) && g.N % 8 == 0;
   const int outs = g.row1 == INT_MAX ? 1 : 2;
   p.vec_out = p.vec_pre = g.N % 8 == 0;
   for (int i = 0; i < 2; ++i) {
-    if (i < outs) p.vec_out = p.vec_out && rows16(g.out[i]);
-    if (g.pre[i].p) p.vec_pre = p.vec_pre && rows16(g.pre[i]);
+    if (i < outs) p.vec_out = p.vec_out && ffn_rows16(g.out[i]);
+    if (g.pre[i].p) p.vec_pre = p.vec_pre && ffn_rows16(g.pre[i]);
   }
   const char* why = nullptr;
   bool ok = true;
-  if (aligned) {
-    for (int i = 0; i < g.segs; ++i)
-      ok = ok && (g.layout == FFN_TN ? make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.K, g.M, g.a[i].ld, 64, 64, &why)
-                                     : make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.M, g.K, g.a[i].ld, 64, p.a_rows, &why));
-    const uint32_t b_rows = g.layout != FFN_NT ? 64 : g.gated ? plan.bn / 2 : plan.bn / plan.cg;
-    for (int i = 0; i < nb; ++i)
-      ok = ok && (g.layout == FFN_NT ? make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.N, g.K, g.b[i].ld, 64, b_rows, &why)
-                                     : make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.K, g.N, g.b[i].ld, 64, b_rows, &why));
-  }
+  for (int i = 0; i < g.segs; ++i)
+    ok = ok && (g.layout == FFN_TN ? make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.K, g.M, g.a[i].ld, 64, 64, &why)
+                                   : make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.M, g.K, g.a[i].ld, 64, p.a_rows, &why));
+  const uint32_t b_rows = g.layout != FFN_NT ? 64 : g.gated ? plan.bn / 2 : plan.bn / plan.cg;
+  for (int i = 0; i < nb; ++i)
+    ok = ok && (g.layout == FFN_NT ? make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.N, g.K, g.b[i].ld, 64, b_rows, &why)
+                                   : make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.K, g.N, g.b[i].ld, 64, b_rows, &why));
   if (!ok) return static_cast<int>(cudaErrorInvalidValue);
   return g.fp16 ? launch_ffn_tc_fp16(plan.cfg, g.layout, g.gated, p, stream)
                 : launch_ffn_tc_bf16(plan.cfg, g.layout, g.gated, p, stream);

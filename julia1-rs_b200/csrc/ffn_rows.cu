@@ -137,7 +137,28 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* partials, in
   }
 }
 
-bool vec_ok(const FfnMat& m) { return !m.p || (reinterpret_cast<uintptr_t>(m.p) % 16 == 0 && m.ld % 8 == 0); }
+bool vec_ok(const FfnMat& m) { return !m.p || ffn_rows16(m); }
+
+// Copies matrices to rows on 16-byte boundaries. A warp takes 256 columns of a row; 2-byte accesses,
+// neighbouring lanes on neighbouring elements, any alignment. Block (8 warps): 8 rows.
+__global__ void __launch_bounds__(256) copies_kernel(const FfnCopies c) {
+  grid_dep_launch();
+  const FfnCopy& m = c.m[blockIdx.z];
+  const int lane = threadIdx.x & 31;
+  grid_dep_wait();
+  for (long long r = static_cast<long long>(blockIdx.y) * 8 + (threadIdx.x >> 5); r < m.rows; r += gridDim.y * 8ll) {
+    const uint16_t* src = static_cast<const uint16_t*>(m.src.p) + r * m.src.ld;
+    uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(m.dst.p)) + r * m.dst.ld;
+    for (int c0 = blockIdx.x * 256; c0 < m.cols; c0 += gridDim.x * 256) {
+      uint16_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c0 + i * 32 + lane < m.cols ? src[c0 + i * 32 + lane] : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + i * 32 + lane < m.cols) dst[c0 + i * 32 + lane] = v[i];
+    }
+  }
+}
 
 template <typename T, bool GATED, int ACT>
 cudaError_t launch_grad(const FfnGrad& g, bool vec, dim3 grid, int slab_rows, cudaStream_t st) {
@@ -156,6 +177,17 @@ cudaError_t launch_grad(const FfnGrad& g, bool vec, dim3 grid, int slab_rows, cu
 }
 
 }  // namespace
+
+int launch_ffn_copies(const FfnCopies& c, cudaStream_t st) {
+  long long rows = 1, cols = 1;
+  for (int i = 0; i < c.n; ++i) {
+    rows = rows > c.m[i].rows ? rows : c.m[i].rows;
+    cols = cols > c.m[i].cols ? cols : c.m[i].cols;
+  }
+  const long long by = (rows + 7) / 8, bx = (cols + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(bx < 64 ? bx : 64), static_cast<unsigned>(by < 32768 ? by : 32768), c.n);
+  return static_cast<int>(launch_kernel(copies_kernel, grid, dim3(256), 0, st, c));
+}
 
 // About eight blocks per SM over both dimensions, at least 32 rows each, at most 512 slabs.
 int ffn_grad_slabs(int M, int N) {

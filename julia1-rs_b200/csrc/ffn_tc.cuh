@@ -19,10 +19,7 @@
 //   in the accumulator's own layout and a second kernel adds a tile's pieces in order.
 //
 // Roles per CTA: warp 0 TMA producer, warp 1 TMEM allocator and MMA issuer (even CTA), then the
-// epilogue warps (four to sixteen: those of a TMEM lane quarter take its 32-column chunks in turn). GEN:
-// operands whose rows do not start on 16-byte boundaries cannot be read by TMA; eight loader
-// warps (and four epilogue warps) load aligned 16-byte pieces, shift them into place and store
-// the boxes a TMA load would have written.
+// epilogue warps (eight to sixteen: those of a TMEM lane quarter take its 32-column chunks in turn).
 // Producer and issuer run as whole warps with one elected lane issuing: with a lane-dependent
 // branch around the loop instead, an MMA step (four MMAs and a commit) took 600 cycles to issue.
 // The accumulator is double buffered in TMEM, so a tile's epilogue runs under the next tile's
@@ -51,15 +48,13 @@ namespace ffn {
 
 constexpr int BM = 128;  // rows of a tile per CTA
 constexpr int BK = 64;   // contraction elements per stage
-constexpr int GW = 8;    // loader warps (GEN): each thread owns 4 units of A and 4 of B
 // Epilogue warps. A linear forward tile on a pair has up to 32,768 activations per CTA, each with an
 // exponential and a reciprocal: with two warps per SM sub-partition their latencies were not hidden
 // (131072 x 1152 x 768 with GELU 326 us, without 182 us), with four they are (219 us). Gated tiles
 // have half of them, products without an activation none: eight warps leave room for more stages.
-__host__ __device__ constexpr int epi_warps(int cg, int bn, int layout, bool gated, bool gen) {
-  return gen ? 4 : cg == 2 && layout == FFN_NT && !gated ? (bn == 192 ? 12 : 16) : 8;
+__host__ __device__ constexpr int epi_warps(int cg, int bn, int layout, bool gated) {
+  return cg == 2 && layout == FFN_NT && !gated ? (bn == 192 ? 12 : 16) : 8;
 }
-__host__ __device__ constexpr int threads_of(int ew, bool gen) { return 32 * (2 + ew + (gen ? GW : 0)); }
 constexpr uint32_t SLOT = 32 * 32 * 2;  // one 32 x 32 output box
 constexpr uint32_t A_BYTES = BM * BK * 2;
 constexpr uint32_t SMEM_MAX = 232448;
@@ -165,12 +160,6 @@ struct Waiter {
 };
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-// Arrivals whose writes the other CTA of the pair reads through its tensor core (GEN, CG 2).
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr) : "memory");
-}
-__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
-
 template <int CG>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
   if constexpr (CG == 2)
@@ -281,127 +270,6 @@ __host__ __device__ __forceinline__ void tile_at(int tile, int group, int m_tile
 
 __device__ __forceinline__ void Units::at(int& mt, int& nt) const { tile_at(tile, group, m_tiles, n_tiles, mt, nt); }
 
-// ---- GEN loads. A unit is 8 elements (16 bytes of a box row) from address `at`; `n` of them lie
-// inside the matrix's row (n <= 0: none, all zero). The two aligned 16-byte pieces that hold it
-// are loaded whole when they lie inside the matrix's memory [lo, hi), else the unit is loaded by
-// elements (`slow`, only at the matrix's first and last bytes).
-struct GenUnit {
-  uint4 x, y;
-};
-__device__ __forceinline__ bool gen_load(GenUnit& g, const char* at, int n, const char* lo, const char* hi) {
-  g.x = g.y = make_uint4(0u, 0u, 0u, 0u);
-  if (n <= 0) return false;
-  const uint32_t s = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at) & 15u);
-  const char* c0 = at - s;
-  if (c0 >= lo && c0 + (s ? 32 : 16) <= hi) {
-    g.x = *reinterpret_cast<const uint4*>(c0);
-    if (s) g.y = *reinterpret_cast<const uint4*>(c0 + 16);
-    return false;
-  }
-  const uint16_t* e = reinterpret_cast<const uint16_t*>(at);
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t l = 2 * i < n ? e[2 * i] : 0u, h = 2 * i + 1 < n ? e[2 * i + 1] : 0u;
-    w[i] = l | (h << 16);
-  }
-  g.x = make_uint4(w[0], w[1], w[2], w[3]);
-  return true;
-}
-// The unit's 16 bytes: the two pieces shifted by s bytes (even), elements past n zero.
-__device__ __forceinline__ uint4 gen_shift(const GenUnit& g, uint32_t s, int n) {
-  uint32_t w[8] = {g.x.x, g.x.y, g.x.z, g.x.w, g.y.x, g.y.y, g.y.z, g.y.w};
-#pragma unroll
-  for (int i = 0; i < 6; ++i) w[i] = (s & 8) ? w[i + 2] : w[i];
-#pragma unroll
-  for (int i = 0; i < 5; ++i) w[i] = (s & 4) ? w[i + 1] : w[i];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], (s & 2) * 8);
-  if (n < 8) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (2 * i >= n) w[i] = 0u;
-      else if (2 * i + 1 >= n) w[i] &= 0xffffu;
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// One operand of a stage as this thread sees it: 4 units i = t + 256 j, j < 4, of 128 box rows x
-// 8 units. K-major (MN false): box row = output index, units along the contraction, a step of 64
-// moves 128 bytes along the row. MN-major: two chunks of 64 box rows; box row = contraction
-// index, units along the output index, a step moves 64 rows. Either step keeps an address's
-// offset from its 16-byte boundary, so the shift of a unit is fixed for a tile.
-template <bool MN>
-struct GenOperand {
-  FfnMat m;
-  int rows, cols, r0, c0;  // matrix extents and the tile's first row and column
-  __device__ __forceinline__ void pos(int i, int k, long long& r, int& c) const {
-    const int br = i >> 3, u = i & 7;
-    if constexpr (MN) {
-      r = k + (br & 63);
-      c = c0 + (br >> 6) * 64 + u * 8;
-    } else {
-      r = static_cast<long long>(r0) + br;
-      c = k + u * 8;
-    }
-  }
-  __device__ __forceinline__ const char* at(long long r, int c) const {
-    return static_cast<const char*>(m.p) + (r * m.ld + c) * 2;
-  }
-  __device__ __forceinline__ uint32_t load(GenUnit (&g)[4], int t, int k) const {
-    const char* lo = static_cast<const char*>(m.p);
-    const char* hi = lo + (static_cast<long long>(rows - 1) * m.ld + cols) * 2;
-    uint32_t slow = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      long long r;
-      int c;
-      pos(t + j * GW * 32, k, r, c);
-      if (gen_load(g[j], at(r, c), r < rows ? cols - c : 0, lo, hi)) slow |= 1u << j;
-    }
-    return slow;
-  }
-  // The first 64 box rows of this operand, the last 64 of `o` (units j < 2 and j >= 2).
-  __device__ __forceinline__ uint32_t load2(GenUnit (&g)[4], int t, int k, const GenOperand& o) const {
-    uint32_t slow = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const GenOperand& w = j < 2 ? *this : o;
-      const char* lo = static_cast<const char*>(w.m.p);
-      const char* hi = lo + (static_cast<long long>(rows - 1) * w.m.ld + cols) * 2;
-      long long r;
-      int c;
-      w.pos(t + j * GW * 32, k, r, c);
-      if (gen_load(g[j], w.at(r, c), r < rows ? cols - c : 0, lo, hi)) slow |= 1u << j;
-    }
-    return slow;
-  }
-  __device__ __forceinline__ void store2(const GenUnit (&g)[4], uint32_t slow, int t, int k, uint32_t dst,
-                                         const GenOperand& o) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const GenOperand& w = j < 2 ? *this : o;
-      const int i = t + j * GW * 32, br = i >> 3, u = i & 7;
-      long long r;
-      int c;
-      w.pos(i, k, r, c);
-      const uint32_t s = (slow >> j) & 1 ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(w.at(r, c)) & 15u);
-      sts128(dst + br * 128 + ((u ^ (br & 7)) << 4), gen_shift(g[j], s, cols - c));
-    }
-  }
-  __device__ __forceinline__ void store(const GenUnit (&g)[4], uint32_t slow, int t, int k, uint32_t dst) const {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = t + j * GW * 32, br = i >> 3, u = i & 7;
-      long long r;
-      int c;
-      pos(i, k, r, c);
-      const uint32_t s = (slow >> j) & 1 ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(at(r, c)) & 15u);
-      sts128(dst + br * 128 + ((u ^ (br & 7)) << 4), gen_shift(g[j], s, cols - c));
-    }
-  }
-};
-
 template <int ACT, int W>
 __device__ __forceinline__ void act_all(uint64_t (&v)[W]) {
 #pragma unroll
@@ -447,22 +315,27 @@ static __device__ __noinline__ void copy_out(uint32_t box, void* p, long long ld
   if (vec) {
     const int br = lane >> 2, bu = lane & 3;
     uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row + br) * ld + col + bu * 8;
+    uint4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = lds128(box + (br + 8 * i) * 64 + ((bu ^ ((br >> 1) & 3)) << 4));
     if (col + bu * 8 < N) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = br + 8 * i;
-        if (row + r < rows) *reinterpret_cast<uint4*>(at) = lds128(box + r * 64 + ((bu ^ ((r >> 1) & 3)) << 4));
+        if (row + br + 8 * i < rows) *reinterpret_cast<uint4*>(at) = w[i];
         at += 8 * ld;
       }
     }
   } else {
     const int c = col + lane, n = min(32, rows - row);
     uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row) * ld + c;
-    if (c < N) {
-#pragma unroll 4
-      for (int r = 0; r < n; ++r) {
-        const uint32_t w = lds32(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 6) * 2);
-        *at = static_cast<uint16_t>(w >> ((lane & 1) * 16));
+#pragma unroll 1
+    for (int r0 = 0; r0 < n; r0 += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = lds32(box + (r0 + i) * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 6) * 2);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (r0 + i < n && c < N) *at = static_cast<uint16_t>(w[i] >> ((lane & 1) * 16));
         at += ld;
       }
     }
@@ -496,14 +369,14 @@ static __device__ __noinline__ void copy_in(uint32_t box, const void* p, long lo
   }
 }
 
-template <typename T, int CG, int BN, int LAYOUT, bool GATED, bool GEN>
-__global__ void __launch_bounds__(threads_of(epi_warps(CG, BN, LAYOUT, GATED, GEN), GEN), 1) tc_kernel(const __grid_constant__ FfnTc p) {
+template <typename T, int CG, int BN, int LAYOUT, bool GATED>
+__global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1) tc_kernel(const __grid_constant__ FfnTc p) {
   constexpr bool A_MN = LAYOUT == FFN_TN, B_MN = LAYOUT != FFN_NT;
-  constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED, GEN);
+  constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED);
   constexpr int BROWS = BN / CG;             // output columns of B staged by one CTA
   constexpr int OUTW = GATED ? BN / 2 : BN;  // output columns of a tile
   constexpr uint32_t B_BYTES = b_bytes(CG, BN);
-  static_assert(!(GATED && LAYOUT != FFN_NT) && !(GEN && BROWS != 128) && OUTW % 64 == 0, "");
+  static_assert(!(GATED && LAYOUT != FFN_NT) && OUTW % 64 == 0, "");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int stages = p.stages;
@@ -529,7 +402,7 @@ __global__ void __launch_bounds__(threads_of(epi_warps(CG, BN, LAYOUT, GATED, GE
   if (warp == 0) {
     if (elect_one()) {
       for (int s = 0; s < stages; ++s) {
-        bar_init(full + s * 8, GEN ? GW * CG : 1);
+        bar_init(full + s * 8, 1);
         bar_init(empty + s * 8, 1);
       }
       for (int b = 0; b < 2; ++b) {
@@ -556,69 +429,67 @@ __global__ void __launch_bounds__(threads_of(epi_warps(CG, BN, LAYOUT, GATED, GE
   tc_fence_before();
   if constexpr (CG == 2) {
     cluster_sync();
-  } else if (!GEN && warp == 0) {
-    asm volatile("bar.arrive 1, %0;" ::"n"(threads_of(EW, GEN)) : "memory");
+  } else if (warp == 0) {
+    asm volatile("bar.arrive 1, %0;" ::"n"(32 * (2 + EW)) : "memory");
   } else {
-    asm volatile("bar.sync 1, %0;" ::"n"(threads_of(EW, GEN)) : "memory");
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * (2 + EW)) : "memory");
   }
   tc_fence_after();
   grid_dep_wait();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if constexpr (!GEN) {
-      const int kb_seg = p.kb_seg;
-      int stage = 0, round = 0;
-      uint32_t phase = 1;
-      bool ok = true;
-      for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
-        int mt, nt;
-        u.at(mt, nt);
-        const int m0 = (mt * CG + static_cast<int>(rank)) * BM;
-        const int n0 = GATED ? nt * OUTW : nt * BN + static_cast<int>(rank) * BROWS;
+    const int kb_seg = p.kb_seg;
+    int stage = 0, round = 0;
+    uint32_t phase = 1;
+    bool ok = true;
+    for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
+      int mt, nt;
+      u.at(mt, nt);
+      const int m0 = (mt * CG + static_cast<int>(rank)) * BM;
+      const int n0 = GATED ? nt * OUTW : nt * BN + static_cast<int>(rank) * BROWS;
 #pragma unroll 1
-        for (int kb = u.k0; kb < u.k1; ++kb) {
-          const uint32_t fb = full + stage * 8;
-          if (round && !wait(empty + stage * 8, phase, 31)) {  // in the first round every stage is empty
-            ok = false;
-            break;
+      for (int kb = u.k0; kb < u.k1; ++kb) {
+        const uint32_t fb = full + stage * 8;
+        if (round && !wait(empty + stage * 8, phase, 31)) {  // in the first round every stage is empty
+          ok = false;
+          break;
+        }
+        const int seg = kb >= kb_seg ? 1 : 0;
+        const int k = (kb - (seg ? kb_seg : 0)) * BK;
+        const uint32_t da = sA + stage * a_bytes, db = sB + stage * B_BYTES;
+        if (elect_one()) {
+          if (leader) bar_expect(fb, CG * (a_bytes + B_BYTES));
+          const uint32_t fc = CG == 2 ? mapa_shared(fb, 0) : fb;
+          const CUtensorMap* ma = &p.ma[0] + seg;
+          const CUtensorMap* mb = &p.mb[0] + (GATED ? static_cast<int>(rank) : seg);
+          if constexpr (A_MN) {
+            tma_box<CG>(ma, fc, da, m0, k);
+            tma_box<CG>(ma, fc, da + A_BYTES / 2, m0 + 64, k);
+          } else {
+            tma_box<CG>(ma, fc, da, k, m0);
           }
-          const int seg = kb >= kb_seg ? 1 : 0;
-          const int k = (kb - (seg ? kb_seg : 0)) * BK;
-          const uint32_t da = sA + stage * a_bytes, db = sB + stage * B_BYTES;
-          if (elect_one()) {
-            if (leader) bar_expect(fb, CG * (a_bytes + B_BYTES));
-            const uint32_t fc = CG == 2 ? mapa_shared(fb, 0) : fb;
-            const CUtensorMap* ma = &p.ma[0] + seg;
-            const CUtensorMap* mb = &p.mb[0] + (GATED ? static_cast<int>(rank) : seg);
-            if constexpr (A_MN) {
-              tma_box<CG>(ma, fc, da, m0, k);
-              tma_box<CG>(ma, fc, da + A_BYTES / 2, m0 + 64, k);
-            } else {
-              tma_box<CG>(ma, fc, da, k, m0);
-            }
-            if constexpr (B_MN) {
+          if constexpr (B_MN) {
 #pragma unroll
-              for (int c = 0; c < BROWS / 64; ++c) tma_box<CG>(mb, fc, db + c * 8192, n0 + c * 64, k);
-            } else {  // gated: the tile's columns are OUTW of B0 (CTA 0), then OUTW of B1 (CTA 1)
-              tma_box<CG>(mb, fc, db, k, n0);
-              if constexpr (GATED && CG == 1) tma_box<CG>(mb + 1, fc, db + B_BYTES / 2, k, n0);
-            }
-          }
-          __syncwarp();
-          if (++stage == stages) {
-            stage = 0;
-            round = 1;
-            phase ^= 1;
+            for (int c = 0; c < BROWS / 64; ++c) tma_box<CG>(mb, fc, db + c * 8192, n0 + c * 64, k);
+          } else {  // gated: the tile's columns are OUTW of B0 (CTA 0), then OUTW of B1 (CTA 1)
+            tma_box<CG>(mb, fc, db, k, n0);
+            if constexpr (GATED && CG == 1) tma_box<CG>(mb + 1, fc, db + B_BYTES / 2, k, n0);
           }
         }
+        __syncwarp();
+        if (++stage == stages) {
+          stage = 0;
+          round = 1;
+          phase ^= 1;
+        }
       }
-      if (!ok) {
-        // Unwinding after a timeout: copies in flight may complete on the other CTA's barrier,
-        // so give them ample time to land before shared memory is released.
-        const long long t0 = clock64();
-        while (clock64() - t0 < 2000000) __nanosleep(1000);
-      }
+    }
+    if (!ok) {
+      // Unwinding after a timeout: copies in flight may complete on the other CTA's barrier,
+      // so give them ample time to land before shared memory is released.
+      const long long t0 = clock64();
+      while (clock64() - t0 < 2000000) __nanosleep(1000);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (even CTA)
@@ -652,7 +523,6 @@ __global__ void __launch_bounds__(threads_of(epi_warps(CG, BN, LAYOUT, GATED, GE
           const int next = stage + 1 == stages ? 0 : stage + 1;
           const uint32_t next_phase = next ? phase : phase ^ 1;
           ready = bar_peek(full + next * 8, next_phase);
-          if constexpr (GEN && CG == 2) fence_cluster();
           tc_fence_after();
           if (elect_one()) {
             const uint64_t da = a_desc + static_cast<uint32_t>(stage) * (a_bytes / 16);
@@ -687,78 +557,6 @@ __global__ void __launch_bounds__(threads_of(epi_warps(CG, BN, LAYOUT, GATED, GE
         __syncwarp();
         const long long t0 = clock64();
         while (!bar_try(drain, 0) && clock64() - t0 < J1_WAIT_CYCLES) {
-        }
-      }
-    }
-  } else if (GEN && warp >= 2 + EW) {
-    // ------------------------------------------------------------ loader warps (GEN)
-    const int t = static_cast<int>(threadIdx.x) - 32 * (2 + EW);
-    const int kb_seg = p.kb_seg, M = p.M, N = p.N, K = p.K;
-    int stage = 0;
-    uint32_t phase = 1;
-    bool ok = true;
-    GenUnit ga[4], gb[4];
-    for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
-      int mt, nt;
-      u.at(mt, nt);
-      const int m0 = (mt * CG + static_cast<int>(rank)) * BM;
-      // operands of block kb; B of a single gated CTA is 64 rows of each weight
-      auto seg_k = [&](int kb, int& seg) {
-        seg = kb >= kb_seg ? 1 : 0;
-        return (kb - (seg ? kb_seg : 0)) * BK;
-      };
-      auto op_a = [&](int seg) {
-        return A_MN ? GenOperand<A_MN>{seg ? p.a[1] : p.a[0], K, M, 0, m0}
-                    : GenOperand<A_MN>{seg ? p.a[1] : p.a[0], M, K, m0, 0};
-      };
-      auto op_b = [&](int seg) {
-        if constexpr (GATED && CG == 2) return GenOperand<B_MN>{rank ? p.b[1] : p.b[0], N, K, nt * OUTW, 0};
-        if constexpr (GATED && CG == 1)  // box rows 0..63 from B0, 64..127 from B1: units j < 2, j >= 2
-          return GenOperand<B_MN>{seg ? p.b[1] : p.b[0], N, K, nt * OUTW - (seg ? 64 : 0), 0};
-        const int n0 = nt * BN + static_cast<int>(rank) * BROWS;
-        return B_MN ? GenOperand<B_MN>{seg ? p.b[1] : p.b[0], K, N, 0, n0}
-                    : GenOperand<B_MN>{seg ? p.b[1] : p.b[0], N, K, n0, 0};
-      };
-      uint32_t slow_a = 0, slow_b = 0;
-      auto load_a = [&](int kb) {
-        int seg;
-        const int k = seg_k(kb, seg);
-        slow_a = op_a(seg).load(ga, t, k);
-      };
-      auto load_b = [&](int kb) {
-        int seg;
-        const int k = seg_k(kb, seg);
-        if constexpr (GATED && CG == 1)
-          slow_b = op_b(0).load2(gb, t, k, op_b(1));
-        else
-          slow_b = op_b(seg).load(gb, t, k);
-      };
-      load_a(u.k0);
-      load_b(u.k0);
-#pragma unroll 1
-      for (int kb = u.k0; kb < u.k1; ++kb) {
-        ok = wait(empty + stage * 8, phase, 34);
-        if (!ok) break;
-        int seg;
-        const int k = seg_k(kb, seg);
-        op_a(seg).store(ga, slow_a, t, k, sA + stage * a_bytes);
-        if (kb + 1 < u.k1) load_a(kb + 1);
-        if constexpr (GATED && CG == 1)
-          op_b(0).store2(gb, slow_b, t, k, sB + stage * B_BYTES, op_b(1));
-        else
-          op_b(seg).store(gb, slow_b, t, k, sB + stage * B_BYTES);
-        if (kb + 1 < u.k1) load_b(kb + 1);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 2)
-            mbar_arrive_cluster(mapa_shared(full + stage * 8, 0));
-          else
-            bar_arrive(full + stage * 8);
-        }
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
         }
       }
     }
@@ -1054,11 +852,11 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Ffn
       Elem<T>::store(const_cast<void*>(p.out[o].p), static_cast<long long>(orow + r) * p.out[o].ld + col + lane, box[r][lane]);
 }
 
-template <typename T, int CG, int BN, int LAYOUT, bool GATED, bool GEN>
+template <typename T, int CG, int BN, int LAYOUT, bool GATED>
 int launch_one(FfnTc& p, cudaStream_t stream) {
-  constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED, GEN);
+  constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED);
   static std::atomic<unsigned long long> configured{0};
-  auto kern = tc_kernel<T, CG, BN, LAYOUT, GATED, GEN>;
+  auto kern = tc_kernel<T, CG, BN, LAYOUT, GATED>;
   cudaError_t e = set_smem_once(kern, SMEM_MAX, configured);
   if (e != cudaSuccess) return static_cast<int>(e);
   // no more stages than blocks a CTA will see: a small CTA can share the SM with the kernel before.
@@ -1073,7 +871,7 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
   p.ring = std::max<uint32_t>(p.stages * stage, std::max<uint32_t>(p.split > 1 ? BM * BN * 4 : 0, A_BYTES + b_bytes(CG, BN)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(CG == 2 ? 2 * p.workers : p.workers * p.split));
-  cfg.blockDim = dim3(threads_of(EW, GEN));
+  cfg.blockDim = dim3(32 * (2 + EW));
   cfg.dynamicSmemBytes = fixed + p.ring;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1093,16 +891,14 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
 template <typename T, int LAYOUT, bool GATED>
 int launch_cfg(int cfg, FfnTc& p, cudaStream_t stream) {
   switch (cfg) {
-    case FFN_CG2_256: return launch_one<T, 2, 256, LAYOUT, GATED, false>(p, stream);
+    case FFN_CG2_256: return launch_one<T, 2, 256, LAYOUT, GATED>(p, stream);
     case FFN_CG2_192:
-      if constexpr (LAYOUT == FFN_NT && !GATED) return launch_one<T, 2, 192, LAYOUT, GATED, false>(p, stream);
+      if constexpr (LAYOUT == FFN_NT && !GATED) return launch_one<T, 2, 192, LAYOUT, GATED>(p, stream);
       break;
-    case FFN_CG1_128: return launch_one<T, 1, 128, LAYOUT, GATED, false>(p, stream);
+    case FFN_CG1_128: return launch_one<T, 1, 128, LAYOUT, GATED>(p, stream);
     case FFN_CG1_64:
-      if constexpr (!GATED) return launch_one<T, 1, 64, LAYOUT, GATED, false>(p, stream);
+      if constexpr (!GATED) return launch_one<T, 1, 64, LAYOUT, GATED>(p, stream);
       break;
-    case FFN_CG1_128_GEN: return launch_one<T, 1, 128, LAYOUT, GATED, true>(p, stream);
-    case FFN_CG2_256_GEN: return launch_one<T, 2, 256, LAYOUT, GATED, true>(p, stream);
   }
   return static_cast<int>(cudaErrorInvalidValue);
 }

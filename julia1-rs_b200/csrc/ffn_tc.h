@@ -29,7 +29,7 @@ struct FfnTc {
 };
 
 // Configurations: CG (CTAs per tile pair) x BN (accumulator columns of a tile).
-enum FfnCfg : int { FFN_CG2_256 = 0, FFN_CG2_192, FFN_CG1_128, FFN_CG1_64, FFN_CG1_128_GEN, FFN_CG2_256_GEN };
+enum FfnCfg : int { FFN_CG2_256 = 0, FFN_CG2_192, FFN_CG1_128, FFN_CG1_64 };
 int launch_ffn_tc_bf16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream);
 int launch_ffn_tc_fp16(int cfg, int layout, int gated, FfnTc& p, cudaStream_t stream);
 
