@@ -24,39 +24,45 @@ struct Plan {
   double us;
 };
 
-// Microseconds per 64-block of a tile and CTA (or pair) and the fixed part of a tile that
-// nothing hides (first loads, last epilogue).
+// The tile shape and split with the least time by a model of both sides' measurements: microseconds
+// per 64-block of a tile with all SMs busy (single CTAs are bound by what they load through L2, 32 KB
+// per 128 x 128 block against 64 KB per 256 x 256 for a pair, so their blocks cost three quarters of a
+// pair's for a quarter of the work), fewer when few are, plus what a launch does not overlap.
+// Measured: 8192 x 8192 x 8192 CG 2 x 256 0.67-0.75 ms, x 192 0.80, CG 1 x 128 1.04; 512 x 768 x 768 11.8, 11,
+// 7.3 us and CG 1 x 64 5.6 us; 16 x 8192 x 8192 CG 1 x 128 30 us, in clusters of two 26 us.
 Plan choose(const FfnGemm& g, int kb) {
-  const int sms = g.num_sms;
-  const auto single = [&](int cfg, int bn, double step) {
-    const long long tiles = ceil_div(g.M, 128) * ceil_div(g.N, g.gated ? bn / 2 : bn);
-    Plan best = {cfg, 1, bn, 1, false, 0.0};
-    best.us = static_cast<double>(ceil_div(tiles, sms)) * kb * step + 1.5;
-    for (int s = 2; s <= 8 && s <= kb; s *= 2) {
-      const double us = static_cast<double>(ceil_div(tiles * s, sms)) * (static_cast<double>(ceil_div(kb, s)) * step + 1.5) + 1.0;
-      if (us < best.us) best.split = s, best.us = us;
-    }
-    return best;
-  };
-  Plan best = single(FFN_CG1_128, 128, 0.22);
+  const int sms = g.num_sms, pairs = std::max(1, std::min(kPairs, sms / 2));
+  Plan best = {};
+  best.us = 1e30;
   const auto take = [&](const Plan& p) {
     if (p.us < best.us) best = p;
   };
-  if (!g.gated) take(single(FFN_CG1_64, 64, 0.13));
-  const auto pair = [&](int cfg, int bn, double step) {
-    const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
-    const int pairs = std::max(1, std::min(kPairs, sms / 2));
-    Plan p = {cfg, 2, bn, 1, false, 0.0};
-    p.us = static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 2.5;
-    if (g.layout == FFN_TN && bn == 256 && g.partials &&
-        tiles * kb < INT_MAX && tiles * kb >= pairs && (tiles + pairs) * kPieceBytes <= g.partial_bytes) {  // equal shares, then a pass over the pieces
-      const double us = static_cast<double>(tiles) * kb * step / pairs + 6.0 + 0.1 * static_cast<double>(tiles + pairs) / 4;
-      if (us < p.us) p.stream_k = true, p.us = us;
+  // busy: microseconds per block when every SM works, lone: when few do
+  const auto single = [&](int cfg, int bn, double busy, double lone) {
+    const long long tiles = ceil_div(g.M, 128) * ceil_div(g.N, g.gated ? bn / 2 : bn);
+    const double rows = std::min<double>(g.M, 128.0) / 128.0;  // small A boxes load less
+    for (int s = 1; s <= 8 && s <= kb; s *= 2) {
+      const long long ctas = tiles * s;
+      if (s > 1 && ctas > sms) break;
+      const double load = std::min(1.0, static_cast<double>(ctas) / sms);
+      const double step = lone + (busy * (bn + 128 * rows) / (bn + 128) - lone) * load;
+      const double per = static_cast<double>(ceil_div(kb, s)) * std::max(step, lone);
+      take({cfg, 1, bn, s, false, static_cast<double>(ceil_div(ctas, sms)) * per + 2.8 + (s > 1 ? 1.0 + 0.05 * s : 0.0)});
     }
-    return p;
   };
-  take(pair(FFN_CG2_256, 256, 0.40));
-  if (g.layout == FFN_NT && !g.gated) take(pair(FFN_CG2_192, 192, 0.31));
+  single(FFN_CG1_128, 128, 0.30, 0.15);
+  if (!g.gated) single(FFN_CG1_64, 64, 0.17, 0.13);
+  const auto pair = [&](int cfg, int bn, double busy, double lone) {
+    const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
+    const double load = std::min(1.0, static_cast<double>(tiles) / pairs);
+    const double step = lone + (busy - lone) * load;
+    take({cfg, 2, bn, 1, false, static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 5.0});
+    if (g.layout == FFN_TN && bn == 256 && g.partials && tiles * kb < INT_MAX && tiles * kb >= pairs &&
+        (tiles + pairs) * kPieceBytes <= g.partial_bytes)  // equal shares, then a pass over the pieces
+      take({cfg, 2, bn, 1, true, static_cast<double>(tiles) * kb * busy / pairs + 9.0 + 0.03 * static_cast<double>(tiles + pairs)});
+  };
+  pair(FFN_CG2_256, 256, 0.40, 0.28);
+  if (g.layout == FFN_NT && !g.gated) pair(FFN_CG2_192, 192, 0.335, 0.22);
   return best;
 }
 

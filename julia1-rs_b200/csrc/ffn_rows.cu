@@ -76,27 +76,40 @@ __global__ void __launch_bounds__(GC) grad_kernel(const FfnGrad g, int slab_rows
   const long long r1 = min(r0 + slab_rows, static_cast<long long>(g.M));
   float s0[8] = {}, s1[8] = {};
   grid_dep_wait();
-  for (long long r = r0 + ty; r < r1; r += GR) {
-    float d[8], p[8], q[8], x[8];
-    load8<T, VEC>(g.dout, r, c0, lane, g.N, d);
-    if constexpr (GATED || ACT != J1_ACT_NONE) load8<T, VEC>(g.p0, r, c0, lane, g.N, p);
-    if constexpr (GATED) load8<T, VEC>(g.p1, r, c0, lane, g.N, q);
+  // RI rows of a thread at once, all loads before the arithmetic
+  constexpr int RI = 2;
+  for (long long r = r0 + ty; r < r1; r += GR * RI) {
+    float d[RI][8], p[RI][8], q[RI][8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float slope = 1.f, value = 0.f;
-      if constexpr (GATED || ACT != J1_ACT_NONE) act_slope<ACT>(p[i], slope, value);
-      if constexpr (GATED) {
-        x[i] = d[i] * value;
-        d[i] = d[i] * q[i] * slope;
-        s1[i] += x[i];
-      } else {
-        d[i] = d[i] * slope;
-      }
-      s0[i] += d[i];
+    for (int j = 0; j < RI; ++j) {
+      const long long row = r + j * GR;
+      const int n = row < r1 ? g.N : 0;  // no columns of a row behind the slab
+      load8<T, VEC>(g.dout, row, c0, lane, n, d[j]);
+      if constexpr (GATED || ACT != J1_ACT_NONE) load8<T, VEC>(g.p0, row, c0, lane, n, p[j]);
+      if constexpr (GATED) load8<T, VEC>(g.p1, row, c0, lane, n, q[j]);
     }
-    if (g.d0.p) store8<T, VEC>(g.d0, r, c0, lane, g.N, d);
-    if constexpr (GATED) {
-      if (g.d1.p) store8<T, VEC>(g.d1, r, c0, lane, g.N, x);
+#pragma unroll
+    for (int j = 0; j < RI; ++j) {
+      const long long row = r + j * GR;
+      const int n = row < r1 ? g.N : 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float slope = 1.f, value = 0.f;
+        if constexpr (GATED || ACT != J1_ACT_NONE) act_slope<ACT>(p[j][i], slope, value);
+        if constexpr (GATED) {
+          const float a = d[j][i] * q[j][i] * slope;
+          q[j][i] = d[j][i] * value;
+          d[j][i] = a;
+          s1[i] += q[j][i];
+        } else {
+          d[j][i] = d[j][i] * slope;
+        }
+        s0[i] += d[j][i];
+      }
+      if (g.d0.p) store8<T, VEC>(g.d0, row, c0, lane, n, d[j]);
+      if constexpr (GATED) {
+        if (g.d1.p) store8<T, VEC>(g.d1, row, c0, lane, n, q[j]);
+      }
     }
   }
   if (!g.partials) return;
@@ -114,11 +127,11 @@ __global__ void __launch_bounds__(GC) grad_kernel(const FfnGrad g, int slab_rows
   }
 }
 
-// sum[c] = partials[0][c] + partials[1][c] + ... : 32 columns per block, 8 slab strides at once,
+// sum[c] = partials[0][c] + partials[1][c] + ... : 32 columns per block, 32 slab strides at once with
+// four loads in flight each (one stride of eight and a load at a time took 10 us for 395 slabs),
 // joined in a fixed order.
-__global__ void __launch_bounds__(256) slab_sum_kernel(const float* partials, int slabs, int N, float* sum0,
-                                                       float* sum1) {
-  __shared__ float red[8][32];
+__global__ void __launch_bounds__(1024) slab_sum_kernel(const float* partials, int slabs, int N, float* sum0, float* sum1) {
+  __shared__ float red[32][33];
   grid_dep_launch();
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
@@ -127,35 +140,54 @@ __global__ void __launch_bounds__(256) slab_sum_kernel(const float* partials, in
   float t = 0.f;
   grid_dep_wait();
   if (c < N)
-    for (int s = ty; s < slabs; s += 8) t += p[static_cast<size_t>(s) * N + c];
+    for (int s = ty; s < slabs; s += 128) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = s + 32 * i < slabs ? p[static_cast<size_t>(s + 32 * i) * N + c] : 0.f;
+      t += (v[0] + v[1]) + (v[2] + v[3]);
+    }
   red[ty][lane] = t;
   __syncthreads();
-  if (ty == 0 && c < N && sum) {
+  t = red[lane][ty];  // warp ty: the 32 strides of column ty
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += red[k][lane];
-    sum[c] = t;
-  }
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if (lane == 0 && blockIdx.x * 32 + ty < N && sum) sum[blockIdx.x * 32 + ty] = t;
 }
 
 bool vec_ok(const FfnMat& m) { return !m.p || ffn_rows16(m); }
 
-// Copies matrices to rows on 16-byte boundaries. A warp takes 256 columns of a row; 2-byte accesses,
-// neighbouring lanes on neighbouring elements, any alignment. Block (8 warps): 8 rows.
+// Copies matrices to rows on 16-byte boundaries. A warp takes 256 columns of a row: it reads 2-byte
+// elements (neighbouring lanes on neighbouring elements, any alignment), lane l keeps elements l,
+// l + 32, ..., and writes pairs as words after an exchange with its neighbour, half as many stores.
+// Four rows of a warp are in flight. Block (8 warps): 32 rows.
 __global__ void __launch_bounds__(256) copies_kernel(const FfnCopies c) {
   grid_dep_launch();
-  const FfnCopy& m = c.m[blockIdx.z];
-  const int lane = threadIdx.x & 31;
+  const FfnCopy m = c.m[blockIdx.z];
+  const int lane = threadIdx.x & 31, c0 = blockIdx.x * 256;
+  const long long rows = m.rows;
   grid_dep_wait();
-  for (long long r = static_cast<long long>(blockIdx.y) * 8 + (threadIdx.x >> 5); r < m.rows; r += gridDim.y * 8ll) {
-    const uint16_t* src = static_cast<const uint16_t*>(m.src.p) + r * m.src.ld;
-    uint16_t* dst = static_cast<uint16_t*>(const_cast<void*>(m.dst.p)) + r * m.dst.ld;
-    for (int c0 = blockIdx.x * 256; c0 < m.cols; c0 += gridDim.x * 256) {
-      uint16_t v[8];
+  if (c0 >= m.cols) return;
+  for (long long r = static_cast<long long>(blockIdx.y) * 32 + (threadIdx.x >> 5) * 4; r < rows; r += gridDim.y * 32ll) {
+    uint32_t v[4][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = c0 + i * 32 + lane < m.cols ? src[c0 + i * 32 + lane] : 0;
+    for (int j = 0; j < 4; ++j) {
+      const uint16_t* src = static_cast<const uint16_t*>(m.src.p) + (r + j) * m.src.ld + c0 + lane;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c0 + i * 32 + lane < m.cols) dst[c0 + i * 32 + lane] = v[i];
+      for (int i = 0; i < 8; ++i) v[j][i] = r + j < rows && c0 + i * 32 + lane < m.cols ? src[i * 32] : 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // dst.ld is a multiple of 8: the words of a row up to its stride are ours, elements behind cols stay 0
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(const_cast<void*>(m.dst.p)) + (r + j) * m.dst.ld + c0);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        // even lanes: word lane / 2 of columns [32 i, +32), odd lanes: of [32 (i + 1), +32)
+        const uint32_t keep = lane & 1 ? v[j][i + 1] : v[j][i], give = lane & 1 ? v[j][i] : v[j][i + 1];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
+        const uint32_t word = lane & 1 ? got | (keep << 16) : keep | (got << 16);
+        const int col = (i + (lane & 1)) * 32 + (lane & ~1);
+        if (r + j < rows && c0 + col < m.dst.ld) dst[col / 2] = word;
+      }
     }
   }
 }
@@ -184,8 +216,8 @@ int launch_ffn_copies(const FfnCopies& c, cudaStream_t st) {
     rows = rows > c.m[i].rows ? rows : c.m[i].rows;
     cols = cols > c.m[i].cols ? cols : c.m[i].cols;
   }
-  const long long by = (rows + 7) / 8, bx = (cols + 255) / 256;
-  const dim3 grid(static_cast<unsigned>(bx < 64 ? bx : 64), static_cast<unsigned>(by < 32768 ? by : 32768), c.n);
+  const long long by = (rows + 31) / 32, bx = (cols + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(bx), static_cast<unsigned>(by < 32768 ? by : 32768), c.n);
   return static_cast<int>(launch_kernel(copies_kernel, grid, dim3(256), 0, st, c));
 }
 
@@ -214,7 +246,7 @@ int launch_ffn_grad(const FfnGrad& g, cudaStream_t st) {
     e = g.gated ? launch_grad<__nv_bfloat16, true>(k, vec, grid, slab_rows, st)
                 : launch_grad<__nv_bfloat16, false>(k, vec, grid, slab_rows, st);
   if (e != cudaSuccess || !k.partials) return static_cast<int>(e);
-  return static_cast<int>(launch_kernel(slab_sum_kernel, dim3((g.N + 31) / 32, g.gated ? 2 : 1), dim3(256), 0, st,
+  return static_cast<int>(launch_kernel(slab_sum_kernel, dim3((g.N + 31) / 32, g.gated ? 2 : 1), dim3(1024), 0, st,
                                         static_cast<const float*>(k.partials), slabs, g.N, g.sum0, g.sum1));
 }
 

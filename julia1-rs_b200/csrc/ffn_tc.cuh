@@ -424,6 +424,10 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
       tmem_relinquish();
     }
   }
+  // The list of units needs parameters only: its divisions pass while the others set up.
+  Units u(p, worker, crank);
+  int mt, nt;
+  u.at(mt, nt);
   // Barriers initialised and TMEM allocated, in both CTAs of a pair. The producer of a single CTA
   // needs nothing from the other warps: it only arrives and starts to load.
   tc_fence_before();
@@ -443,9 +447,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
     int stage = 0, round = 0;
     uint32_t phase = 1;
     bool ok = true;
-    for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
-      int mt, nt;
-      u.at(mt, nt);
+    for (; ok && u.ok(); u.next(), u.at(mt, nt)) {
       const int m0 = (mt * CG + static_cast<int>(rank)) * BM;
       const int n0 = GATED ? nt * OUTW : nt * BN + static_cast<int>(rank) * BROWS;
 #pragma unroll 1
@@ -507,7 +509,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
       // The test of the next stage's barrier is issued before this stage's MMAs: its latency (80
       // cycles) passes while they are issued.
       bool ready = bar_peek(full, 0);
-      for (Units u(p, worker, crank); ok && u.ok(); u.next()) {
+      for (; ok && u.ok(); u.next()) {
         const int buf = acc & 1;
         if (acc >= 2) ok = wait(tempty + buf * 8, ((acc >> 1) + 1) & 1, 32);
         if (!ok) break;
@@ -574,12 +576,18 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
     const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
     tmem_base = lds32(tmem_slot);
 
-    // What the chunk at (row, col) needs beside its accumulators: biases to the warp's bias rows,
-    // the residual to the output box. Called once everything of the chunk before has left the box.
-    auto fetch = [&](int row, int col) {
+    // What the chunk at (row, col) needs beside its accumulators: one column's biases per lane, loaded
+    // a chunk ahead (load), then put to the warp's bias rows, and the residual to the output box, once
+    // everything of the chunk before has left them (place).
+    float nb0 = 0.f, nb1 = 0.f;
+    auto load = [&](int col) {
       const bool in = col + lane < N;
-      sts32(wbias + lane * 4, p.bias[0] && in ? __float_as_uint(p.bias[0][col + lane]) : 0u);
-      if constexpr (GATED) sts32(wbias + 128 + lane * 4, p.bias[1] && in ? __float_as_uint(p.bias[1][col + lane]) : 0u);
+      nb0 = p.bias[0] && in ? p.bias[0][col + lane] : 0.f;
+      if constexpr (GATED) nb1 = p.bias[1] && in ? p.bias[1][col + lane] : 0.f;
+    };
+    auto place = [&](int row, int col) {
+      sts32(wbias + lane * 4, __float_as_uint(nb0));
+      if constexpr (GATED) sts32(wbias + 128 + lane * 4, __float_as_uint(nb1));
       if (residual) copy_in(box, p.residual.p, p.residual.ld, p.vec_res, row, M, col, N);
     };
     auto add16 = [&](uint32_t bias, const uint32_t (&r)[16], uint64_t (&v)[8]) {
@@ -601,14 +609,15 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
 
     int acc = 0;
     bool ok = true;
-    for (Units u(p, worker, crank); ok && u.ok(); u.next(), ++acc) {
-      int mt, nt;
-      u.at(mt, nt);
+    for (; ok && u.ok(); u.next(), u.at(mt, nt), ++acc) {
       const int row = (mt * CG + static_cast<int>(rank)) * BM + q * 32;  // this warp's first row
       const int n0 = nt * OUTW;
       const uint32_t buf = acc & 1;
       const bool pieces = split > 1 || p.stream_k;
-      if (!pieces && row < M && c0 < OUTW && n0 + c0 < N) fetch(row, n0 + c0);
+      if (!pieces && row < M && c0 < OUTW && n0 + c0 < N) {
+        load(n0 + c0);
+        place(row, n0 + c0);
+      }
       ok = wait(tfull + buf * 8, (acc >> 1) & 1, 35);
       if (!ok) break;
       tc_fence_after();
@@ -657,6 +666,8 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           if (residual) cp_async_wait();
           __syncwarp();  // biases and residual are in place
         }
+        const bool more = c + 32 * PER < OUTW && col + 32 * PER < N;
+        if (more) load(col + 32 * PER);
 #pragma unroll 1
         for (int j = 0; j < 2; ++j) {
           uint32_t r0[16], r1[16];
@@ -697,29 +708,30 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
         const bool second = row >= p.row1;
         copy_out(box, const_cast<void*>(second ? p.out[1].p : p.out[0].p), second ? p.out[1].ld : p.out[0].ld, p.vec_out,
                  second ? row - p.row1 : row, second ? M - p.row1 : min(M, p.rows0), col, N);
-        if (c + 32 * PER < OUTW && col + 32 * PER < N) fetch(row, col + 32 * PER);
+        if (more) place(row, col + 32 * PER);
       }
     }
     if constexpr (CG == 1) {
       if (split > 1) {
         // All accumulators of the cluster are in shared memory. Units of 32 rows x 8 columns are
         // dealt to the cluster's epilogue warps; a unit's pieces are added in rank order.
-        int mt, nt;
         tile_at(worker, p.group, p.m_tiles, p.n_tiles, mt, nt);
-        const int quarters = min(4, (M - mt * BM + 31) / 32);  // that hold rows
-        const int units = quarters * (OUTW / 8);
+        const int rows = M - mt * BM;
+        const int qlog = rows > 64 ? 2 : rows > 32 ? 1 : 0;  // log2 of the quarters that may hold rows
+        const int units = (OUTW / 8) << qlog;
         const int first = (e << p.split_log2) + crank;
         auto unit_bias = [&](const float* bias, int unit) {  // lane i < 8: column i
-          const int c = nt * OUTW + unit / quarters * 8 + lane;
+          const int c = nt * OUTW + (unit >> qlog) * 8 + lane;
           return bias && lane < 8 && unit < units && c < N ? bias[c] : 0.f;
         };
         float b0 = unit_bias(p.bias[0], first), b1 = GATED ? unit_bias(p.bias[1], first) : 0.f;
         cluster_sync();
+        constexpr int FLY = 4;
         bool left = false;  // this warp has arrived for its last remote read
         if (ok) {
 #pragma unroll 1
           for (int unit = first; unit < units; unit += EW << p.split_log2) {
-            const int uq = unit % quarters, c = unit / quarters * 8;
+            const int uq = unit & ((1 << qlog) - 1), c = (unit >> qlog) * 8;
             const int row = mt * BM + uq * 32 + lane, col = nt * OUTW + c;
             if (unit != first) {
               b0 = unit_bias(p.bias[0], unit);
@@ -732,11 +744,11 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
             for (int i = 0; i < 4; ++i) v[i] = g[i] = 0ull;
             const uint32_t at = smem + static_cast<uint32_t>((uq * (BN / 4) + c / 4) * 512 + lane * 16);
 #pragma unroll 1
-            for (int s0 = 0; s0 < split; s0 += 2) {  // two CTAs' pieces in flight (split is even)
-              float4 x[2][2], y[2][2];
+            for (int s0 = 0; s0 < split; s0 += FLY) {  // FLY CTAs' pieces in flight
+              float4 x[FLY][2], y[FLY][2];
 #pragma unroll
-              for (int s = 0; s < 2; ++s) {
-                const uint32_t base = mapa_shared(at, s0 + s);
+              for (int s = 0; s < FLY; ++s) {
+                const uint32_t base = mapa_shared(at, s0 + s < split ? s0 + s : s0);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                   x[s][i] = ld_cluster(base + i * 512);
@@ -744,9 +756,10 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
                 }
               }
 #pragma unroll
-              for (int s = 0; s < 2; ++s)
+              for (int s = 0; s < FLY; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
+                  if (s0 + s >= split) continue;
                   v[2 * i] = add2(v[2 * i], f2pack(x[s][i].x, x[s][i].y));
                   v[2 * i + 1] = add2(v[2 * i + 1], f2pack(x[s][i].z, x[s][i].w));
                   if constexpr (GATED) {
