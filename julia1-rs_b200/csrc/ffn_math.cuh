@@ -65,12 +65,9 @@ __device__ __forceinline__ float recip_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 1 / (1 + 2^x), the logistic function of -x ln 2: relative error about 1e-6 on both tails (2^x may
-// overflow: 1 / inf = 0).
-__device__ __forceinline__ float logistic2(float x) { return recip_approx(1.f + exp2_approx(x)); }
-
 // Every activation here but ReLU is p times a logistic function of an odd polynomial of p, and all
-// are evaluated that way, with one exponential and one reciprocal per value:
+// are evaluated that way, with one exponential and one reciprocal per value (the exponential may
+// overflow on the far side: 1 / inf = 0):
 //   silu       p / (1 + 2^(-p log2 e))
 //   gelu_tanh  0.5 (1 + tanh z) = 1 / (1 + 2^(-2 z log2 e)),  z = sqrt(2/pi) (p + 0.044715 p^3)
 //   gelu       Phi(p) = 1 / (1 + 2^(-p R(p^2))): R(p^2) = log2(Phi / (1 - Phi)) / p is smooth and even; a
@@ -88,21 +85,6 @@ __host__ __device__ constexpr float gelu_coef(int k) {  // minus the coefficient
          : k == 4 ? -1.1439842637628317e-05f
          : k == 5 ? 3.8163187809914234e-07f
                   : -5.06724973092787e-09f;
-}
-
-// Minus the exponent (log2) of the logistic function, of a value t = p^2 beside p.
-template <int ACT>
-__device__ __forceinline__ float logit2(float p, float t) {
-  if constexpr (ACT == J1_ACT_GELU) {
-    float r = gelu_coef(6);
-#pragma unroll
-    for (int k = 5; k >= 0; --k) r = fmaf(r, t, gelu_coef(k));
-    return r * p;
-  } else if constexpr (ACT == J1_ACT_GELU_TANH) {
-    return p * fmaf(kTanhB, t, kTanhA);
-  } else {
-    return -kLog2e * p;
-  }
 }
 
 // act of a pair of values (packed FP32 arithmetic around the exponentials and reciprocals).
@@ -132,27 +114,51 @@ __device__ __forceinline__ uint64_t act_pair(uint64_t p) {
   return mul2(p, f2pack(recip_approx(a), recip_approx(b)));
 }
 
-// act'(p) and act(p). With s the logistic function and x(p) its argument, act = p s and act' = s +
-// p s (1 - s) x'(p); for gelu p s (1 - s) x' is p phi(p), taken from the density itself. The slopes
-// are constant to FP32 beyond |p| = 40; clamping there keeps 0 * inf out of them.
+// act'(p) and act(p) of a pair. With s the logistic function and x(p) its argument, act = p s and
+// act' = s + p s (1 - s) x'(p); for gelu p s (1 - s) x' is p phi(p), taken from the density itself.
+// The tanh form's slope is constant to FP32 beyond |p| = 40; clamping there keeps 0 * inf out of it.
 template <int ACT>
-__device__ __forceinline__ void act_slope(float p, float& slope, float& value) {
+__device__ __forceinline__ void act_slope(uint64_t p, uint64_t& slope, uint64_t& value) {
+  auto c2 = [](float c) { return f2pack(c, c); };
+  float a, b;
   if constexpr (ACT == J1_ACT_NONE) {
-    slope = 1.f;
+    slope = c2(1.f);
     value = p;
   } else if constexpr (ACT == J1_ACT_RELU) {
-    slope = p > 0.f ? 1.f : 0.f;
-    value = p < 0.f ? 0.f : p;
+    f2unpack(p, a, b);
+    slope = f2pack(a > 0.f ? 1.f : 0.f, b > 0.f ? 1.f : 0.f);
+    value = f2pack(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);
   } else {
-    const float low = max_nan(p, -40.f), h = min_nan(low, 40.f), t = h * h;
-    const float s = logistic2(logit2<ACT>(h, t));
-    value = low * s;
-    if constexpr (ACT == J1_ACT_GELU)
-      slope = fmaf(h, 0.3989422804014327f * exp2_approx(-0.5f * kLog2e * t), s);
-    else if constexpr (ACT == J1_ACT_GELU_TANH)
-      slope = fmaf(h * (s * (1.f - s)), 1.5957691216057308f * fmaf(3.f * 0.044715f, t, 1.f), s);
-    else
-      slope = fmaf(h * s, 1.f - s, s);
+    uint64_t h = p, x;
+    if constexpr (ACT == J1_ACT_GELU_TANH) {
+      f2unpack(p, a, b);
+      h = f2pack(min_nan(max_nan(a, -40.f), 40.f), min_nan(max_nan(b, -40.f), 40.f));
+    }
+    const uint64_t t = mul2(h, h);
+    if constexpr (ACT == J1_ACT_GELU) {
+      x = c2(gelu_coef(6));
+#pragma unroll
+      for (int k = 5; k >= 0; --k) x = fma2(x, t, c2(gelu_coef(k)));
+      x = mul2(x, h);
+    } else if constexpr (ACT == J1_ACT_GELU_TANH) {
+      x = mul2(h, fma2(t, c2(kTanhB), c2(kTanhA)));
+    } else {
+      x = mul2(h, c2(-kLog2e));
+    }
+    f2unpack(x, a, b);
+    f2unpack(add2(f2pack(exp2_approx(a), exp2_approx(b)), c2(1.f)), a, b);
+    const uint64_t s = f2pack(recip_approx(a), recip_approx(b));
+    value = mul2(p, s);
+    if constexpr (ACT == J1_ACT_GELU) {
+      f2unpack(mul2(t, c2(-0.5f * kLog2e)), a, b);
+      slope = fma2(mul2(h, c2(0.3989422804014327f)), f2pack(exp2_approx(a), exp2_approx(b)), s);
+    } else {
+      const uint64_t rest = fma2(s, c2(-1.f), c2(1.f));  // 1 - s
+      if constexpr (ACT == J1_ACT_GELU_TANH)
+        slope = fma2(mul2(mul2(h, s), rest), fma2(t, c2(3.f * 0.044715f * 1.5957691216057308f), c2(1.5957691216057308f)), s);
+      else
+        slope = fma2(mul2(h, s), rest, s);
+    }
   }
 }
 
