@@ -9,6 +9,7 @@ raise J1Error.
 """
 import ctypes as C
 import os
+import struct
 from dataclasses import dataclass, field
 from typing import List, Optional, Sequence
 
@@ -1145,6 +1146,8 @@ def op_geglu_interleave(src_f32, dst_bf16, inter, k, stream=None):
 
 # ---- the feed-forward block (include/j1.h, "the feed-forward block for training and serving"):
 # 2-D bf16 or fp16 tensors whose rows are contiguous (any row stride), float32 biases.
+# A small call takes 5 us on the GPU, so the wrappers keep their own work short: sizes, strides and
+# pointers are read once and packed into the argument struct's bytes (the layout of the J1*Args classes).
 _ffn_dtypes = {}  # torch dtype -> j1_dtype
 
 
@@ -1158,38 +1161,64 @@ def _ffn_dtype(t):
     return d
 
 
+def _ffn_bad(name, t, what):
+    shape = tuple(t.shape)
+    raise J1Error(INVALID_ARG, "%s: expected %s, got %s of %s with strides %s" % (name, what, t.dtype, shape, t.stride()))
+
+
 def _ffn_mat(name, t, rows, cols, dtype):
-    """(pointer, row stride) of a [rows, cols] matrix of `dtype`; None: (None, 0)."""
+    """(pointer, row stride) of a [rows, cols] matrix of `dtype`; None: (0, 0)."""
     if t is None:
-        return None, 0
-    if t.shape != (rows, cols) or t.dtype != dtype:
-        raise J1Error(INVALID_ARG, "%s: expected %s of shape (%d, %d), got %s of %s" % (
-            name, dtype, rows, cols, t.dtype, tuple(t.shape)))
-    s = t.stride()
-    if s[1] != 1 and cols > 1:
-        raise J1Error(INVALID_ARG, "%s: the elements of a row must be contiguous (strides %s)" % (name, s))
-    return t.data_ptr(), s[0] if rows > 1 else max(s[0], cols)
+        return 0, 0
+    if t.dtype is not dtype or t.shape != (rows, cols):
+        _ffn_bad(name, t, "%s of shape (%d, %d)" % (dtype, rows, cols))
+    ld, one = t.stride()
+    if one != 1 and cols > 1:
+        _ffn_bad(name, t, "contiguous elements in a row")
+    return t.data_ptr(), ld if rows > 1 or ld > cols else cols
+
+
+_ffn_float = None  # torch.float32, once seen
 
 
 def _ffn_vec(name, t, n):
+    global _ffn_float
     if t is None:
-        return None
-    if t.shape != (n,) or str(t.dtype) != "torch.float32" or (n > 1 and t.stride(0) != 1):
-        raise J1Error(INVALID_ARG, "%s: expected contiguous float32 of shape (%d,), got %s of %s" % (
-            name, n, t.dtype, tuple(t.shape)))
+        return 0
+    if t.dtype is not _ffn_float:
+        if str(t.dtype) != "torch.float32":
+            _ffn_bad(name, t, "float32 of shape (%d,)" % n)
+        _ffn_float = t.dtype
+    if t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        _ffn_bad(name, t, "contiguous float32 of shape (%d,)" % n)
     return t.data_ptr()
 
 
 def _ffn_sizes(x, w):
     if x.dim() != 2 or w.dim() != 2:
         raise J1Error(INVALID_ARG, "matrices must have two dimensions")
-    if max(x.shape[0], w.shape[0], w.shape[1]) > 1 << 30:
+    M, K = x.shape
+    N = w.shape[0]
+    if M > 1 << 30 or N > 1 << 30 or K > 1 << 30:
         raise J1Error(UNSUPPORTED, "sizes above 2^30")
-    return x.shape[0], w.shape[0], w.shape[1]
+    return M, N, K
 
 
 def _ffn_workspace(t):
-    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+    return (0, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+
+
+_ffn_ops = {}
+
+
+def _ffn_op(name, args):
+    s = struct.Struct("@" + "".join({C.c_int32: "i", C.c_int64: "q", C.c_void_p: "Q", C.c_size_t: "Q"}[t]
+                                    for _, t in args._fields_))
+    assert s.size == C.sizeof(args)
+    f = lib()["j1_op_" + name]  # a function object of its own: the packed bytes go in as a char pointer
+    f.argtypes, f.restype = [C.c_char_p, C.c_void_p, C.c_int], C.c_int
+    _ffn_ops[name] = op = s.pack, f
+    return op
 
 
 def op_linear(x, w, out, bias=None, act=ACT_NONE, residual=None, pre=None, stream=None, sync=True):
@@ -1197,10 +1226,10 @@ def op_linear(x, w, out, bias=None, act=ACT_NONE, residual=None, pre=None, strea
     x [M, K], w [N, K], out / residual / pre [M, N] (out may be residual), bias float32 [N]."""
     M, N, K = _ffn_sizes(x, w)
     d = x.dtype
-    a = J1LinearArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("x", x, M, K, d), *_ffn_mat("w", w, N, K, d),
-                     _ffn_vec("bias", bias, N), *_ffn_mat("residual", residual, M, N, d),
-                     *_ffn_mat("out", out, M, N, d), *_ffn_mat("pre", pre, M, N, d))
-    check(lib().j1_op_linear(a, stream, 1 if sync else 0))
+    pack, call = _ffn_ops.get("linear") or _ffn_op("linear", J1LinearArgs)
+    check(call(pack(_ffn_dtype(x), act, M, N, K, *_ffn_mat("x", x, M, K, d), *_ffn_mat("w", w, N, K, d),
+                    _ffn_vec("bias", bias, N), *_ffn_mat("residual", residual, M, N, d),
+                    *_ffn_mat("out", out, M, N, d), *_ffn_mat("pre", pre, M, N, d)), stream, 1 if sync else 0))
 
 
 def op_linear_backward_workspace(M, N, K):
@@ -1217,10 +1246,11 @@ def op_linear_backward(dout, x, w, pre=None, act=ACT_NONE, dx=None, dw=None, dbi
     op_linear_backward_workspace(M, N, K) bytes."""
     M, N, K = _ffn_sizes(x, w)
     d = x.dtype
-    a = J1LinearGradArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("dout", dout, M, N, d), *_ffn_mat("x", x, M, K, d),
-                         *_ffn_mat("w", w, N, K, d), *_ffn_mat("pre", pre, M, N, d), *_ffn_mat("dx", dx, M, K, d),
-                         *_ffn_mat("dw", dw, N, K, d), _ffn_vec("dbias", dbias, N), *_ffn_workspace(workspace))
-    check(lib().j1_op_linear_backward(a, stream, 1 if sync else 0))
+    pack, call = _ffn_ops.get("linear_backward") or _ffn_op("linear_backward", J1LinearGradArgs)
+    check(call(pack(_ffn_dtype(x), act, M, N, K, *_ffn_mat("dout", dout, M, N, d), *_ffn_mat("x", x, M, K, d),
+                    *_ffn_mat("w", w, N, K, d), *_ffn_mat("pre", pre, M, N, d), *_ffn_mat("dx", dx, M, K, d),
+                    *_ffn_mat("dw", dw, N, K, d), _ffn_vec("dbias", dbias, N), *_ffn_workspace(workspace)),
+               stream, 1 if sync else 0))
 
 
 def op_gated(x, wa, wg, out, ba=None, bg=None, act=ACT_GELU, pre_a=None, pre_g=None, stream=None, sync=True):
@@ -1229,11 +1259,11 @@ def op_gated(x, wa, wg, out, ba=None, bg=None, act=ACT_GELU, pre_a=None, pre_g=N
     out / pre_a / pre_g [M, N], ba / bg float32 [N]."""
     M, N, K = _ffn_sizes(x, wa)
     d = x.dtype
-    a = J1GatedArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("x", x, M, K, d), *_ffn_mat("wa", wa, N, K, d),
+    pack, call = _ffn_ops.get("gated") or _ffn_op("gated", J1GatedArgs)
+    check(call(pack(_ffn_dtype(x), act, M, N, K, *_ffn_mat("x", x, M, K, d), *_ffn_mat("wa", wa, N, K, d),
                     *_ffn_mat("wg", wg, N, K, d), _ffn_vec("ba", ba, N), _ffn_vec("bg", bg, N),
                     *_ffn_mat("out", out, M, N, d), *_ffn_mat("pre_a", pre_a, M, N, d),
-                    *_ffn_mat("pre_g", pre_g, M, N, d))
-    check(lib().j1_op_gated(a, stream, 1 if sync else 0))
+                    *_ffn_mat("pre_g", pre_g, M, N, d)), stream, 1 if sync else 0))
 
 
 def op_gated_backward_workspace(M, N, K):
@@ -1250,9 +1280,9 @@ def op_gated_backward(dout, x, wa, wg, pre_a, pre_g, act=ACT_GELU, dx=None, dwa=
     op_gated_backward_workspace(M, N, K) bytes."""
     M, N, K = _ffn_sizes(x, wa)
     d = x.dtype
-    a = J1GatedGradArgs(_ffn_dtype(x), act, M, N, K, *_ffn_mat("dout", dout, M, N, d), *_ffn_mat("x", x, M, K, d),
-                        *_ffn_mat("wa", wa, N, K, d), *_ffn_mat("wg", wg, N, K, d),
-                        *_ffn_mat("pre_a", pre_a, M, N, d), *_ffn_mat("pre_g", pre_g, M, N, d),
-                        *_ffn_mat("dx", dx, M, K, d), *_ffn_mat("dwa", dwa, N, K, d), *_ffn_mat("dwg", dwg, N, K, d),
-                        _ffn_vec("dba", dba, N), _ffn_vec("dbg", dbg, N), *_ffn_workspace(workspace))
-    check(lib().j1_op_gated_backward(a, stream, 1 if sync else 0))
+    pack, call = _ffn_ops.get("gated_backward") or _ffn_op("gated_backward", J1GatedGradArgs)
+    check(call(pack(_ffn_dtype(x), act, M, N, K, *_ffn_mat("dout", dout, M, N, d), *_ffn_mat("x", x, M, K, d),
+                    *_ffn_mat("wa", wa, N, K, d), *_ffn_mat("wg", wg, N, K, d), *_ffn_mat("pre_a", pre_a, M, N, d),
+                    *_ffn_mat("pre_g", pre_g, M, N, d), *_ffn_mat("dx", dx, M, K, d),
+                    *_ffn_mat("dwa", dwa, N, K, d), *_ffn_mat("dwg", dwg, N, K, d), _ffn_vec("dba", dba, N),
+                    _ffn_vec("dbg", dbg, N), *_ffn_workspace(workspace)), stream, 1 if sync else 0))
