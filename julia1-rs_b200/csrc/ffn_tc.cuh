@@ -271,17 +271,17 @@ __host__ __device__ __forceinline__ void tile_at(int tile, int group, int m_tile
 __device__ __forceinline__ void Units::at(int& mt, int& nt) const { tile_at(tile, group, m_tiles, n_tiles, mt, nt); }
 
 template <int ACT, int W>
-__device__ __forceinline__ void act_all(uint64_t (&v)[W]) {
+__device__ __forceinline__ void act_all(uint64_t (&v)[W], const ActConst& k) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) v[i] = act_pair<ACT>(v[i]);
+  for (int i = 0; i < W; ++i) v[i] = act_pair<ACT>(v[i], k);
 }
 template <int W>
-__device__ __forceinline__ void act_all(int act, uint64_t (&v)[W]) {
+__device__ __forceinline__ void act_all(int act, uint64_t (&v)[W], const ActConst& k) {
   switch (act) {
-    case J1_ACT_RELU: act_all<J1_ACT_RELU, W>(v); break;
-    case J1_ACT_GELU: act_all<J1_ACT_GELU, W>(v); break;
-    case J1_ACT_GELU_TANH: act_all<J1_ACT_GELU_TANH, W>(v); break;
-    case J1_ACT_SILU: act_all<J1_ACT_SILU, W>(v); break;
+    case J1_ACT_RELU: act_all<J1_ACT_RELU, W>(v, k); break;
+    case J1_ACT_GELU: act_all<J1_ACT_GELU, W>(v, k); break;
+    case J1_ACT_GELU_TANH: act_all<J1_ACT_GELU_TANH, W>(v, k); break;
+    case J1_ACT_SILU: act_all<J1_ACT_SILU, W>(v, k); break;
     default: break;
   }
 }
@@ -574,23 +574,30 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
     const uint32_t wbias = sbias + e * BIAS_BYTES;
     const uint32_t own = box + lane * 64;  // this thread's row, unit u at own + ((u ^ sw) << 4)
     const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
+    const ActConst k(act);
     tmem_base = lds32(tmem_slot);
 
     // What the chunk at (row, col) needs beside its accumulators: one column's biases per lane, loaded
     // a chunk ahead (load), then put to the warp's bias rows, and the residual to the output box, once
     // everything of the chunk before has left them (place).
+    const bool bias0 = p.bias[0] != nullptr, bias1 = p.bias[1] != nullptr;
     float nb0 = 0.f, nb1 = 0.f;
     auto load = [&](int col) {
       const bool in = col + lane < N;
-      nb0 = p.bias[0] && in ? p.bias[0][col + lane] : 0.f;
-      if constexpr (GATED) nb1 = p.bias[1] && in ? p.bias[1][col + lane] : 0.f;
+      if (bias0) nb0 = in ? p.bias[0][col + lane] : 0.f;
+      if (GATED && bias1) nb1 = in ? p.bias[1][col + lane] : 0.f;
     };
     auto place = [&](int row, int col) {
-      sts32(wbias + lane * 4, __float_as_uint(nb0));
-      if constexpr (GATED) sts32(wbias + 128 + lane * 4, __float_as_uint(nb1));
+      if (bias0) sts32(wbias + lane * 4, __float_as_uint(nb0));
+      if (GATED && bias1) sts32(wbias + 128 + lane * 4, __float_as_uint(nb1));
       if (residual) copy_in(box, p.residual.p, p.residual.ld, p.vec_res, row, M, col, N);
     };
-    auto add16 = [&](uint32_t bias, const uint32_t (&r)[16], uint64_t (&v)[8]) {
+    auto add16 = [&](bool add, uint32_t bias, const uint32_t (&r)[16], uint64_t (&v)[8]) {
+      if (!add) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = f2pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 b = lds128(bias + i * 16);
@@ -677,12 +684,12 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           if (j == 1 && c + 32 * PER >= OUTW) release();
           if (!in) continue;
           uint64_t v[8];
-          add16(wbias + j * 64, r0, v);
+          add16(bias0, wbias + j * 64, r0, v);
           if (save) put16(own + SLOT, j, v);
-          act_all<8>(act, v);
+          act_all<8>(act, v, k);
           if constexpr (GATED) {
             uint64_t g[8];
-            add16(wbias + 128 + j * 64, r1, g);
+            add16(bias1, wbias + 128 + j * 64, r1, g);
             if (save) put16(own + 2 * SLOT, j, g);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], g[i]);
@@ -692,9 +699,9 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
               const uint4 w = lds128(own + ((static_cast<uint32_t>(2 * j + i) ^ sw) << 4));
               const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const float2 f = Elem<T>::unpack(x[k]);
-                v[4 * i + k] = add2(v[4 * i + k], f2pack(f.x, f.y));
+              for (int c4 = 0; c4 < 4; ++c4) {
+                const float2 f = Elem<T>::unpack(x[c4]);
+                v[4 * i + c4] = add2(v[4 * i + c4], f2pack(f.x, f.y));
               }
             }
           }
@@ -781,7 +788,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
             if (row < M) {
               if (save) store_row8<T>(p.pre[0], p.vec_pre, row, col, N, v);
               if (GATED && save) store_row8<T>(p.pre[1], p.vec_pre, row, col, N, g);
-              act_all<4>(act, v);
+              act_all<4>(act, v, k);
               if constexpr (GATED) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], g[i]);
