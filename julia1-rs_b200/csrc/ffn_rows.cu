@@ -140,7 +140,12 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
     float t = 0.f;
 #pragma unroll
     for (int k = 0; k < GR; ++k) t += red[k][threadIdx.x];
-    if (c < g.N) g.partials[(static_cast<size_t>(h) * gridDim.y + blockIdx.y) * g.N + c] = t;
+    if (gridDim.y == 1) {  // the only slab: its sums are the result
+      float* sum = h ? g.sum1 : g.sum0;
+      if (c < g.N && sum) sum[c] = t;
+    } else if (c < g.N) {
+      g.partials[(static_cast<size_t>(h) * gridDim.y + blockIdx.y) * g.N + c] = t;
+    }
   }
 }
 
@@ -259,11 +264,12 @@ int launch_ffn_copies(const FfnCopies& c, cudaStream_t st) {
   return static_cast<int>(launch_kernel(copies_kernel, grid, dim3(256), 0, st, c));
 }
 
-// About eight blocks per SM over both dimensions, at least 32 rows each, at most 512 slabs.
+// About eight blocks per SM over both dimensions, at least 32 rows each, at most 512 slabs; up to 64
+// rows in one slab, which saves the second kernel (2 us) for two more turns of the first (1 us).
 int ffn_grad_slabs(int M, int N) {
   const long long cols = (static_cast<long long>(N) + GC - 1) / GC;
   long long slabs = (1184 + cols - 1) / cols;
-  const long long most = (static_cast<long long>(M) + 31) / 32;
+  const long long most = M <= 64 ? 1 : (static_cast<long long>(M) + 31) / 32;
   if (slabs > most) slabs = most;
   if (slabs > 512) slabs = 512;
   return slabs < 1 ? 1 : static_cast<int>(slabs);
@@ -283,7 +289,7 @@ int launch_ffn_grad(const FfnGrad& g, cudaStream_t st) {
   else
     e = g.gated ? launch_grad<__nv_bfloat16, true>(k, vec, grid, slab_rows, st)
                 : launch_grad<__nv_bfloat16, false>(k, vec, grid, slab_rows, st);
-  if (e != cudaSuccess || !k.partials) return static_cast<int>(e);
+  if (e != cudaSuccess || !k.partials || slabs == 1) return static_cast<int>(e);
   return static_cast<int>(launch_kernel(slab_sum_kernel, dim3((g.N + 31) / 32, g.gated ? 2 : 1), dim3(1024), 0, st,
                                         static_cast<const float*>(k.partials), slabs, g.N, g.sum0, g.sum1));
 }

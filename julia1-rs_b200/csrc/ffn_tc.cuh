@@ -326,17 +326,33 @@ static __device__ __noinline__ void copy_out(uint32_t box, void* p, long long ld
       }
     }
   } else {
-    const int c = col + lane, n = min(32, rows - row);
-    uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row) * ld + c;
+    // two rows at a time, 16 lanes each: words where the row's columns start on one, else the words
+    // between them (elements 2 h + 1, 2 h + 2) and the first and last element by themselves
+    const int h = lane & 15, n = min(32, rows - row), left = min(32, N - col);  // columns of the matrix in the box
+    uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row + (lane >> 4)) * ld + col;
 #pragma unroll 1
-    for (int r0 = 0; r0 < n; r0 += 8) {
-      uint32_t w[8];
+    for (int r0 = lane >> 4; r0 < 32; r0 += 8) {
+      uint32_t w[4], next[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = lds32(box + (r0 + i) * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 6) * 2);
+      for (int i = 0; i < 4; ++i) {
+        const int r = r0 + 2 * i;
+        w[i] = lds32(box + r * 64 + (((h >> 2) ^ ((r >> 1) & 3)) << 4) + (h & 3) * 4);
+      }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (r0 + i < n && c < N) *at = static_cast<uint16_t>(w[i] >> ((lane & 1) * 16));
-        at += ld;
+      for (int i = 0; i < 4; ++i) next[i] = __shfl_down_sync(0xffffffffu, w[i], 1, 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (r0 + 2 * i < n) {
+          const bool odd = (reinterpret_cast<uintptr_t>(at) & 2u) != 0;
+          const int e = odd ? 2 * h + 1 : 2 * h;  // first element of this lane's word
+          const uint32_t v = odd ? __funnelshift_r(w[i], next[i], 16) : w[i];
+          if (e + 1 < left && e < 31)
+            *reinterpret_cast<uint32_t*>(at + e) = v;
+          else if (e < left)
+            at[e] = static_cast<uint16_t>(v);
+          if (odd && h == 0) at[0] = static_cast<uint16_t>(w[i]);
+        }
+        at += 2 * ld;
       }
     }
   }
@@ -359,12 +375,19 @@ static __device__ __noinline__ void copy_in(uint32_t box, const void* p, long lo
   } else {
     const int c = col + lane, n = min(32, rows - row);
     const uint16_t* at = static_cast<const uint16_t*>(p) + static_cast<long long>(row) * ld + c;
-#pragma unroll 4
-    for (int r = 0; r < n; ++r) {
-      const uint16_t v = c < N ? *at : 0;
-      asm volatile("st.shared.u16 [%0], %1;" ::"r"(box + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2), "h"(v)
-                   : "memory");
-      at += ld;
+#pragma unroll 1
+    for (int r0 = 0; r0 < n; r0 += 16) {
+      uint16_t v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        v[i] = c < N && r0 + i < n ? *at : 0;
+        at += ld;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(box + (r0 + i) * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) + (lane & 7) * 2),
+                     "h"(v[i])
+                     : "memory");
     }
   }
 }

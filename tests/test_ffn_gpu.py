@@ -59,6 +59,8 @@ def mat(rows, cols, dtype, gen=None, std=1.0, pad=0, fill=float("nan")):
 def pad_untouched(v, fill=float("nan")):
     """Nothing was written behind the rows of v (a view of mat())."""
     base = v._base
+    if base is not None and base.dim() == 1:  # a matrix somewhere in a buffer: what lies before it
+        return bool(base[:v.storage_offset()].isnan().all())
     if base is None or base.shape[1] == v.shape[1]:
         return True
     rest = base[:, v.shape[1]:].float()
@@ -431,7 +433,7 @@ def test_same_bits_again(torch_cuda):
 
 def test_two_streams_at_once(torch_cuda):
     """Blocks with a workspace each on two streams, interleaved, give what they give alone."""
-    blocks = [_block(1500, 768, 384, BF, 17), _block(700, 520, 264, HF, 19)]
+    blocks = [_block(1500, 768, 384, BF, 17), _block(700, 520, 264, HF, 19), _block(600, 333, 129, BF, 20)]
     refs = []
     for b in blocks:
         _step(b, sync=True)
@@ -449,9 +451,11 @@ def test_two_streams_at_once(torch_cuda):
             assert torch.equal(b[k], ref[k]), k
 
 
-def test_captured_and_replayed(torch_cuda):
-    """A whole step in a CUDA graph, replayed on new inputs in the same buffers."""
-    b = _block(600, 384, 256, BF, 23)
+@pytest.mark.parametrize("M,N,K", [(600, 384, 256), (333, 259, 131), (5, 200, 96)])
+def test_captured_and_replayed(torch_cuda, M, N, K):
+    """A whole step in a CUDA graph, replayed on new inputs in the same buffers; also where operands
+    are copied to aligned rows first (odd widths)."""
+    b = _block(M, N, K, BF, 23)
     _step(b, sync=True)
     s = torch.cuda.Stream()
     graph = torch.cuda.CUDAGraph()
@@ -468,6 +472,78 @@ def test_captured_and_replayed(torch_cuda):
         _step(b, sync=True)
         for k in RESULTS:
             assert torch.equal(b[k], got[k]), k
+
+
+def test_two_graphs_and_an_eager_call(torch_cuda):
+    """Two captured steps with a workspace each, replayed at once on two streams while a third step runs
+    eagerly, all with copied operands."""
+    blocks = [_block(257, 131, 67, BF, 31), _block(300, 203, 77, HF, 32), _block(129, 99, 101, BF, 33)]
+    refs = []
+    for b in blocks:
+        _step(b, sync=True)
+        refs.append({k: b[k].clone() for k in RESULTS})
+    graphs = []
+    for b in blocks[:2]:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            _step(b, stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+    for b in blocks:
+        for k in RESULTS:
+            b[k].fill_(float("nan"))
+    streams = [torch.cuda.Stream() for _ in blocks]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        _step(blocks[2], stream=streams[2].cuda_stream)
+    torch.cuda.synchronize()
+    for b, ref in zip(blocks, refs):
+        for k in RESULTS:
+            assert torch.equal(b[k], ref[k]), k
+
+
+def test_unaligned_bases(torch_cuda):
+    """Operands and results that start anywhere in a buffer, at its first and last elements too: the
+    copies to aligned rows read nothing outside them."""
+    for off, (M, N, K) in enumerate(((70, 40, 64), (33, 130, 72), (129, 65, 257), (1, 9, 300), (17, 8, 8), (64, 3, 5)), 1):
+        g = gen(off)
+
+        def at(rows, cols, std=1.0):
+            buf = torch.full((rows * cols + off,), float("nan"), device="cuda", dtype=BF)
+            v = buf[off:].view(rows, cols)
+            v.copy_(torch.randn((rows, cols), generator=g, device="cuda") * std)
+            return v
+
+        x, w, r, out, dout = at(M, K), at(N, K, K ** -0.5), at(M, N), at(M, N), at(M, N)
+        j1.op_linear(x, w, out, residual=r)
+        p, e = affine64(x, w, None)
+        ref = p + r.double()
+        close("out", out, ref, unit(BF) * (ref.abs() + e) + e + 2.0 ** -23 * ref.abs())
+        dx, dw = at(M, K), at(N, K)
+        j1.op_linear_backward(dout, x, w, dx=dx, dw=dw, workspace=scratch(j1.op_linear_backward_workspace(M, N, K)))
+        d = dout.double()
+        check_grads(BF, x, [d], [torch.zeros_like(d)], [w], dx, [dw], [])
+
+
+def test_copies_allocation_failure(torch_cuda):
+    x, w, out = (torch.ones(s, device="cuda", dtype=BF) for s in ((4, 17), (8, 17), (4, 8)))
+    j1.inject_fault(j1.FAULT_ALLOC, 1)
+    try:
+        with pytest.raises(j1.J1Error) as e:
+            j1.op_linear(x, w, out)
+    finally:
+        j1.inject_fault(j1.FAULT_ALLOC, 0)
+    assert e.value.status == j1.OOM
+    j1.op_linear(x, w, out)
+    assert bool((out == 17).all())
+    j1.inject_fault(j1.FAULT_ALLOC, 1)  # nothing is allocated for aligned rows
+    try:
+        j1.op_linear(x[:, :16].contiguous(), w[:, :16].contiguous(), out)
+    finally:
+        j1.inject_fault(j1.FAULT_ALLOC, 0)
+    assert bool((out == 16).all())
 
 
 def test_refused_pointers(torch_cuda):
