@@ -22,6 +22,7 @@ struct Plan {
   int cfg, cg, bn, split;
   bool stream_k;
   double us;
+  int sk_q, sk_r, group;  // stream-K groups; order of the tiles (tile_at)
 };
 
 // The tile shape and split with the least time by a model of both sides' measurements: microseconds
@@ -47,7 +48,7 @@ Plan choose(const FfnGemm& g, int kb) {
       const double load = std::min(1.0, static_cast<double>(ctas) / sms);
       const double step = lone + (busy * (bn + 128 * rows) / (bn + 128) - lone) * load;
       const double per = static_cast<double>(ceil_div(kb, s)) * std::max(step, lone);
-      take({cfg, 1, bn, s, false, static_cast<double>(ceil_div(ctas, sms)) * per + 2.8 + (s > 1 ? 1.0 + 0.05 * s : 0.0)});
+      take({cfg, 1, bn, s, false, static_cast<double>(ceil_div(ctas, sms)) * per + 2.8 + (s > 1 ? 1.0 + 0.05 * s : 0.0), 1, 1, 8});
     }
   };
   single(FFN_CG1_128, 128, 0.30, 0.15);
@@ -56,10 +57,24 @@ Plan choose(const FfnGemm& g, int kb) {
     const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
     const double load = std::min(1.0, static_cast<double>(tiles) / pairs);
     const double step = lone + (busy - lone) * load;
-    take({cfg, 2, bn, 1, false, static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 5.0});
+    take({cfg, 2, bn, 1, false, static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 5.0, 1, 1, 8});
     if (g.layout == FFN_TN && bn == 256 && g.partials && tiles * kb < INT_MAX && tiles * kb >= pairs &&
-        (tiles + pairs) * kPieceBytes <= g.partial_bytes)  // equal shares, then a pass over the pieces
-      take({cfg, 2, bn, 1, true, static_cast<double>(tiles) * kb * busy / pairs + 9.0 + 0.03 * static_cast<double>(tiles + pairs)});
+        (tiles + pairs) * kPieceBytes <= g.partial_bytes) {
+      // q workers for every r tiles, then a pass over the pieces. Tiles of the same place in their group
+      // walk the contraction together: with r dividing the tile rows, rows fastest, that is every r-th
+      // row for all columns, and each of the r walks reads (rows / r + columns) x 256 columns of the
+      // operands; with r dividing the tile columns the other way round.
+      const long long mt = ceil_div(g.M, 256), nt = ceil_div(g.N, 256);
+      for (int order = 0; order < 2; ++order)
+        for (int r = 1; r <= 8; ++r) {
+          const long long side = order ? nt : mt, other = order ? mt : nt, q = pairs * static_cast<long long>(r) / tiles;
+          if (side % r || q < 1) continue;
+          const double compute = static_cast<double>(tiles) * kb * busy / static_cast<double>(q * (tiles / r));
+          const double memory = static_cast<double>(side + r * other) * kb * (64 * 256 * 2) / 6.0e6;
+          take({cfg, 2, bn, 1, true, std::max(compute, memory) + 9.0 + 0.03 * static_cast<double>(tiles + pairs),
+                static_cast<int>(q), r, static_cast<int>(order ? 1 : mt)});
+        }
+    }
   };
   pair(FFN_CG2_256, 256, 0.40, 0.28);
   if (g.layout == FFN_NT && !g.gated) pair(FFN_CG2_192, 192, 0.335, 0.22);
@@ -100,15 +115,14 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   if (m_tiles * n_tiles * plan.split > INT_MAX / 64) return static_cast<int>(cudaErrorInvalidValue);
   p.m_tiles = static_cast<int>(m_tiles), p.n_tiles = static_cast<int>(n_tiles);
   p.tiles = p.m_tiles * p.n_tiles;
-  p.group = 8;
   p.split = plan.split;
   for (p.split_log2 = 0; (1 << p.split_log2) < plan.split;) ++p.split_log2;
   p.stream_k = plan.stream_k;
   p.partials = g.partials;
   const int slots = plan.cg == 2 ? std::max(1, std::min(kPairs, g.num_sms / 2)) : g.num_sms;
-  p.workers = plan.split > 1 ? p.tiles : plan.stream_k ? slots : std::min(p.tiles, slots);
-  p.share = p.tiles * static_cast<long long>(p.kb) / p.workers;
-  p.share_more = static_cast<int>(p.tiles * static_cast<long long>(p.kb) % p.workers);
+  p.sk_q = plan.sk_q, p.sk_r = plan.sk_r;
+  p.workers = plan.split > 1 ? p.tiles : plan.stream_k ? plan.sk_q * (p.tiles / plan.sk_r) : std::min(p.tiles, slots);
+  p.group = plan.stream_k ? plan.group : 8;
   p.a_rows = plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
   p.err = g.err;
   p.residual = g.residual;

@@ -18,7 +18,7 @@ struct FfnTc {
   int split_log2;           // log2 of:
   int split;                // CTAs of a cluster that share a tile's contraction (CG 1), else 1
   int stream_k;             // each worker takes an equal share of all tiles' blocks; FP32 pieces to partials
-  int share, share_more;    // stream-K: blocks of a worker, and how many workers take one more
+  int sk_q, sk_r;           // stream-K: workers per group of tiles, tiles per group
   float* partials;
   int stages;
   int boxes;                // 32 x 32 boxes per epilogue warp
