@@ -68,7 +68,7 @@ Plan choose(const FfnGemm& g, int kb) {
       for (int order = 0; order < 2; ++order)
         for (int r = 1; r <= 8; ++r) {
           const long long side = order ? nt : mt, other = order ? mt : nt, q = pairs * static_cast<long long>(r) / tiles;
-          if (side % r || q < 1) continue;
+          if (side % r || q < 1 || q * r * kb >= (1ll << 32)) continue;
           const double compute = static_cast<double>(tiles) * kb * busy / static_cast<double>(q * (tiles / r));
           const double memory = static_cast<double>(side + r * other) * kb * (64 * 256 * 2) / 6.0e6;
           take({cfg, 2, bn, 1, true, std::max(compute, memory) + 9.0 + 0.03 * static_cast<double>(tiles + pairs),

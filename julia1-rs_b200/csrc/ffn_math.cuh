@@ -87,49 +87,30 @@ __host__ __device__ constexpr float gelu_coef(int k) {  // minus the coefficient
                   : -5.06724973092787e-09f;
 }
 
-// Packed constants of an activation, kept in registers: a loop that names them as literals builds each
-// pair anew (two moves) at every use.
-struct ActConst {
-  uint64_t c[7], one;
-  static __device__ __forceinline__ uint64_t keep(float v) {
-    uint64_t r;
-    asm volatile("mov.b64 %0, {%1, %1};" : "=l"(r) : "f"(v));
-    return r;
-  }
-  __device__ __forceinline__ explicit ActConst(int act) {
-#pragma unroll
-    for (int k = 0; k < 7; ++k) {
-      float v = gelu_coef(k);
-      if (k == 0) v = act == J1_ACT_SILU ? -kLog2e : act == J1_ACT_GELU_TANH ? kTanhA : v;
-      if (k == 1) v = act == J1_ACT_GELU_TANH ? kTanhB : v;
-      c[k] = keep(v);
-    }
-    one = keep(1.f);
-  }
-};
-
 // act of a pair of values (packed FP32 arithmetic around the exponentials and reciprocals).
 template <int ACT>
-__device__ __forceinline__ uint64_t act_pair(uint64_t p, const ActConst& k) {
+__device__ __forceinline__ uint64_t act_pair(uint64_t p) {
+  if constexpr (ACT == J1_ACT_NONE) return p;
   float a, b;
   if constexpr (ACT == J1_ACT_RELU) {
     f2unpack(p, a, b);
     return f2pack(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);  // keeps NaN
   }
+  auto c2 = [](float c) { return f2pack(c, c); };
   uint64_t x;
   if constexpr (ACT == J1_ACT_GELU) {
     const uint64_t t = mul2(p, p);
-    x = k.c[6];
+    x = c2(gelu_coef(6));
 #pragma unroll
-    for (int i = 5; i >= 0; --i) x = fma2(x, t, k.c[i]);
+    for (int k = 5; k >= 0; --k) x = fma2(x, t, c2(gelu_coef(k)));
     x = mul2(x, p);
   } else if constexpr (ACT == J1_ACT_GELU_TANH) {
-    x = mul2(p, fma2(mul2(p, p), k.c[1], k.c[0]));
+    x = mul2(p, fma2(mul2(p, p), c2(kTanhB), c2(kTanhA)));
   } else {
-    x = mul2(p, k.c[0]);
+    x = mul2(p, c2(-kLog2e));
   }
   f2unpack(x, a, b);
-  f2unpack(add2(f2pack(exp2_approx(a), exp2_approx(b)), k.one), a, b);
+  f2unpack(add2(f2pack(exp2_approx(a), exp2_approx(b)), c2(1.f)), a, b);
   return mul2(p, f2pack(recip_approx(a), recip_approx(b)));
 }
 

@@ -238,10 +238,10 @@ struct Units {
       k1 = k0 + per - (rank >= full ? 1 : 0);
     }
   }
-  // Stream-K: every sk_q workers share sk_r neighbouring tiles in equal parts.
+  // Stream-K: every sk_q workers share sk_r neighbouring tiles in equal parts (sk_q sk_r kb < 2^32).
   static __device__ __forceinline__ int share_begin(const FfnTc& p, int worker) {
-    const int blocks = p.sk_r * p.kb, g = worker / p.sk_q;
-    return g * blocks + static_cast<int>(static_cast<long long>(worker - g * p.sk_q) * blocks / p.sk_q);
+    const uint32_t q = p.sk_q, blocks = static_cast<uint32_t>(p.sk_r) * p.kb, g = static_cast<uint32_t>(worker) / q;
+    return static_cast<int>(g * blocks + (worker - g * q) * blocks / q);
   }
   __device__ __forceinline__ void share() {
     tile = pos < end ? pos / kb : tiles;
@@ -276,17 +276,17 @@ __host__ __device__ __forceinline__ void tile_at(int tile, int group, int m_tile
 __device__ __forceinline__ void Units::at(int& mt, int& nt) const { tile_at(tile, group, m_tiles, n_tiles, mt, nt); }
 
 template <int ACT, int W>
-__device__ __forceinline__ void act_all(uint64_t (&v)[W], const ActConst& k) {
+__device__ __forceinline__ void act_all(uint64_t (&v)[W]) {
 #pragma unroll
-  for (int i = 0; i < W; ++i) v[i] = act_pair<ACT>(v[i], k);
+  for (int i = 0; i < W; ++i) v[i] = act_pair<ACT>(v[i]);
 }
 template <int W>
-__device__ __forceinline__ void act_all(int act, uint64_t (&v)[W], const ActConst& k) {
+__device__ __forceinline__ void act_all(int act, uint64_t (&v)[W]) {
   switch (act) {
-    case J1_ACT_RELU: act_all<J1_ACT_RELU, W>(v, k); break;
-    case J1_ACT_GELU: act_all<J1_ACT_GELU, W>(v, k); break;
-    case J1_ACT_GELU_TANH: act_all<J1_ACT_GELU_TANH, W>(v, k); break;
-    case J1_ACT_SILU: act_all<J1_ACT_SILU, W>(v, k); break;
+    case J1_ACT_RELU: act_all<J1_ACT_RELU, W>(v); break;
+    case J1_ACT_GELU: act_all<J1_ACT_GELU, W>(v); break;
+    case J1_ACT_GELU_TANH: act_all<J1_ACT_GELU_TANH, W>(v); break;
+    case J1_ACT_SILU: act_all<J1_ACT_SILU, W>(v); break;
     default: break;
   }
 }
@@ -331,9 +331,11 @@ static __device__ __noinline__ void copy_out(uint32_t box, void* p, long long ld
       }
     }
   } else {
-    // two rows at a time, 16 lanes each: words where the row's columns start on one, else the words
-    // between them (elements 2 h + 1, 2 h + 2) and the first and last element by themselves
+    // Two rows at a time, 16 lanes each: words where the row's columns start on one, else the words
+    // between them (elements 2 h + 1, 2 h + 2) and the first and last element by themselves. A lane reads
+    // the word behind its own as well: a shuffle in this function cost the kernel a third more code.
     const int h = lane & 15, n = min(32, rows - row), left = min(32, N - col);  // columns of the matrix in the box
+    const int h1 = (h + 1) & 15;
     uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row + (lane >> 4)) * ld + col;
 #pragma unroll 1
     for (int r0 = lane >> 4; r0 < 32; r0 += 8) {
@@ -341,10 +343,10 @@ static __device__ __noinline__ void copy_out(uint32_t box, void* p, long long ld
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = r0 + 2 * i;
-        w[i] = lds32(box + r * 64 + (((h >> 2) ^ ((r >> 1) & 3)) << 4) + (h & 3) * 4);
+        const uint32_t at_r = box + r * 64, s = (r >> 1) & 3;
+        w[i] = lds32(at_r + (((h >> 2) ^ s) << 4) + (h & 3) * 4);
+        next[i] = lds32(at_r + (((h1 >> 2) ^ s) << 4) + (h1 & 3) * 4);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) next[i] = __shfl_down_sync(0xffffffffu, w[i], 1, 16);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (r0 + 2 * i < n) {
@@ -602,7 +604,6 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
     const uint32_t wbias = sbias + e * BIAS_BYTES;
     const uint32_t own = box + lane * 64;  // this thread's row, unit u at own + ((u ^ sw) << 4)
     const uint32_t sw = static_cast<uint32_t>((lane >> 1) & 3);
-    const ActConst k(act);
     tmem_base = lds32(tmem_slot);
 
     // What the chunk at (row, col) needs beside its accumulators: one column's biases per lane, loaded
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           uint64_t v[8];
           add16(bias0, wbias + j * 64, r0, v);
           if (save) put16(own + SLOT, j, v);
-          act_all<8>(act, v, k);
+          act_all<8>(act, v);
           if constexpr (GATED) {
             uint64_t g[8];
             add16(bias1, wbias + 128 + j * 64, r1, g);
@@ -816,7 +817,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
             if (row < M) {
               if (save) store_row8<T>(p.pre[0], p.vec_pre, row, col, N, v);
               if (GATED && save) store_row8<T>(p.pre[1], p.vec_pre, row, col, N, g);
-              act_all<4>(act, v, k);
+              act_all<4>(act, v);
               if constexpr (GATED) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], g[i]);
