@@ -621,24 +621,27 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
       if (GATED && bias1) sts32(wbias + 128 + lane * 4, __float_as_uint(nb1));
       if (residual) copy_in(box, p.residual.p, p.residual.ld, p.vec_res, row, M, col, N);
     };
-    auto add16 = [&](bool add, uint32_t bias, const uint32_t (&r)[16], uint64_t (&v)[8]) {
+    constexpr int H = CG == 2 ? 2 : 1;  // 16-column halves of a chunk in registers at a time
+    auto add16 = [&](bool add, uint32_t bias, const uint32_t (&r)[H][16], uint64_t (&v)[8 * H]) {
       if (!add) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = f2pack(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+        for (int i = 0; i < 8 * H; ++i)
+          v[i] = f2pack(__uint_as_float(r[i / 8][2 * (i % 8)]), __uint_as_float(r[i / 8][2 * (i % 8) + 1]));
         return;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 4 * H; ++i) {
         const uint4 b = lds128(bias + i * 16);
-        v[2 * i] = add2(f2pack(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1])),
+        const uint32_t* x = &r[i / 4][4 * (i % 4)];
+        v[2 * i] = add2(f2pack(__uint_as_float(x[0]), __uint_as_float(x[1])),
                         f2pack(__uint_as_float(b.x), __uint_as_float(b.y)));
-        v[2 * i + 1] = add2(f2pack(__uint_as_float(r[4 * i + 2]), __uint_as_float(r[4 * i + 3])),
+        v[2 * i + 1] = add2(f2pack(__uint_as_float(x[2]), __uint_as_float(x[3])),
                             f2pack(__uint_as_float(b.z), __uint_as_float(b.w)));
       }
     };
-    auto put16 = [&](uint32_t at, int j, const uint64_t (&v)[8]) {  // two units of this thread's row
+    auto put16 = [&](uint32_t at, int j, const uint64_t (&v)[8 * H]) {  // units of this thread's row
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2 * H; ++i)
         sts128(at + ((static_cast<uint32_t>(2 * j + i) ^ sw) << 4),
                make_uint4(pack2<T>(v[4 * i]), pack2<T>(v[4 * i + 1]), pack2<T>(v[4 * i + 2]), pack2<T>(v[4 * i + 3])));
     };
@@ -705,26 +708,29 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
         const bool more = c + 32 * PER < OUTW && col + 32 * PER < N;
         if (more) load(col + 32 * PER);
 #pragma unroll 1
-        for (int j = 0; j < 2; ++j) {
-          uint32_t r0[16], r1[16];
-          tmem_ld16(tb + c + 16 * j, r0);
-          if constexpr (GATED) tmem_ld16(tb + BN / 2 + c + 16 * j, r1);
+        for (int j = 0; j < 2; j += H) {
+          uint32_t r0[H][16], r1[H][16];
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            tmem_ld16(tb + c + 16 * (j + h), r0[h]);
+            if constexpr (GATED) tmem_ld16(tb + BN / 2 + c + 16 * (j + h), r1[h]);
+          }
           tmem_ld_wait();
-          if (j == 1 && c + 32 * PER >= OUTW) release();
+          if (j + H == 2 && c + 32 * PER >= OUTW) release();
           if (!in) continue;
-          uint64_t v[8];
+          uint64_t v[8 * H];
           add16(bias0, wbias + j * 64, r0, v);
           if (save) put16(own + SLOT, j, v);
-          act_all<8>(act, v);
+          act_all<8 * H>(act, v);
           if constexpr (GATED) {
-            uint64_t g[8];
+            uint64_t g[8 * H];
             add16(bias1, wbias + 128 + j * 64, r1, g);
             if (save) put16(own + 2 * SLOT, j, g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], g[i]);
+            for (int i = 0; i < 8 * H; ++i) v[i] = mul2(v[i], g[i]);
           } else if (residual) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 2 * H; ++i) {
               const uint4 w = lds128(own + ((static_cast<uint32_t>(2 * j + i) ^ sw) << 4));
               const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
