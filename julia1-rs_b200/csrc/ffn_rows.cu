@@ -77,11 +77,38 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
   const long long r1 = min(r0 + slab_rows, static_cast<long long>(g.M));
   uint64_t s0[4] = {}, s1[4] = {};
   grid_dep_wait();
-  // The next RI rows' loads are in flight while these are worked on: without them the memory waited
-  // for the arithmetic (65536 x 1152 gated GELU 227 us, 3.3 TB/s).
-  constexpr int RI = GATED ? 1 : 2;
+  // VEC: the next DEPTH rows' pieces are on their way to shared memory while a row is worked on, each
+  // thread reading back what it asked for itself. Otherwise the next RI rows' are in registers.
+  constexpr int OPS = GATED ? 3 : ACT != J1_ACT_NONE ? 2 : 1, DEPTH = GATED ? 3 : ACT != J1_ACT_NONE ? 4 : 8;
+  constexpr int RI = GATED || VEC ? 1 : 2;
+  __shared__ uint4 ring[VEC ? DEPTH * OPS * GC : 1];
+  const uint32_t own = smem_u32(ring) + threadIdx.x * 16;
+  uint32_t slot = 0;
+  auto ask = [&](long long r) {
+    const int c = c0 + lane * 8;
+    const uint32_t bytes = r < r1 && c < g.N ? 16u : 0u;
+    const long long row = bytes ? r : 0, col = bytes ? c : 0;  // nothing is read for 0 bytes
+    auto one = [&](int op, const FfnMat& m) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(own + (slot * OPS + op) * (GC * 16)),
+                   "l"(static_cast<const uint16_t*>(m.p) + row * m.ld + col), "r"(bytes)
+                   : "memory");
+    };
+    one(0, g.dout);
+    if constexpr (OPS > 1) one(1, g.p0);
+    if constexpr (OPS > 2) one(2, g.p1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    slot = slot + 1 == DEPTH ? 0u : slot + 1;
+  };
   uint4 d[RI], p[RI], q[RI];
   auto fetch = [&](long long r) {
+    if constexpr (VEC) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+      const uint4* at = ring + slot * OPS * GC + threadIdx.x;
+      d[0] = at[0];
+      if constexpr (OPS > 1) p[0] = at[GC];
+      if constexpr (OPS > 2) q[0] = at[2 * GC];
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < RI; ++j) {
       const long long row = r + j * GR;
@@ -91,12 +118,17 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
       if constexpr (GATED) q[j] = load8<VEC>(g.p1, row, c0, lane, n);
     }
   };
-  fetch(r0 + ty);
+  if constexpr (VEC) {
+    for (int i = 0; i < DEPTH; ++i) ask(r0 + ty + i * GR);
+  } else {
+    fetch(r0 + ty);
+  }
   for (long long r = r0 + ty; r < r1; r += GR * RI) {
+    if constexpr (VEC) fetch(r);
     uint4 d0[RI], p0[RI], q0[RI];
 #pragma unroll
     for (int j = 0; j < RI; ++j) d0[j] = d[j], p0[j] = p[j], q0[j] = q[j];
-    fetch(r + GR * RI);
+    if constexpr (!VEC) fetch(r + GR * RI);
 #pragma unroll
     for (int j = 0; j < RI; ++j) {
       const long long row = r + j * GR;
@@ -124,7 +156,9 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
         if (g.d1.p) store8<T, VEC>(g.d1, row, c0, lane, n, z);
       }
     }
+    if constexpr (VEC) ask(r + DEPTH * GR);
   }
+  if constexpr (VEC) asm volatile("cp.async.wait_all;" ::: "memory");
   if (!g.partials) return;
 #pragma unroll
   for (int h = 0; h < (GATED ? 2 : 1); ++h) {

@@ -877,20 +877,29 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Ffn
   int mt, nt;
   tile_at(tile, p.group, p.m_tiles, p.n_tiles, mt, nt);
   const int row = mt * CG * BM + rq * 32, col = nt * BN + chunk * 32;
-  grid_dep_wait();
-  if (row >= p.M || col >= p.N) return;
-  // the workers of the tile's group whose shares meet its blocks [b0, b1)
+  // the workers [w, end) of the tile's group whose shares meet its blocks [b0, b1)
   const int b0 = tile * p.kb, b1 = b0 + p.kb;
   int w = tile / p.sk_r * p.sk_q;
   while (Units::share_begin(p, w + 1) <= b0) ++w;
+  int end = w + 1;
+  while (end < p.workers && Units::share_begin(p, end) < b1) ++end;
+  const float4* at = reinterpret_cast<const float4*>(p.partials) +
+                     (((static_cast<size_t>(w) + tile) * CG + rq / 4) * 4 + rq % 4) * (BN / 4) * 32 + (chunk * 8 + cg) * 32 + lane;
+  constexpr size_t PIECE = CG * 4 * (BN / 4) * 32;
+  grid_dep_wait();
+  if (row >= p.M || col >= p.N) return;
   float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (; w < p.workers && Units::share_begin(p, w) < b1; ++w) {
-    const float4 x = reinterpret_cast<const float4*>(
-        p.partials)[(((static_cast<size_t>(w) + tile) * CG + rq / 4) * 4 + rq % 4) * (BN / 4) * 32 + (chunk * 8 + cg) * 32 + lane];
-    t.x += x.x;
-    t.y += x.y;
-    t.z += x.z;
-    t.w += x.w;
+  for (; w < end; w += 4, at += 4 * PIECE) {  // four pieces in flight
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = w + i < end ? at[i * PIECE] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      t.x += x[i].x;
+      t.y += x[i].y;
+      t.z += x[i].z;
+      t.w += x[i].w;
+    }
   }
   box[lane][cg * 4] = t.x;
   box[lane][cg * 4 + 1] = t.y;
