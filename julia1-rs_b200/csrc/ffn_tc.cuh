@@ -331,34 +331,49 @@ static __device__ __noinline__ void copy_out(uint32_t box, void* p, long long ld
       }
     }
   } else {
-    // Two rows at a time, 16 lanes each: words where the row's columns start on one, else the words
-    // between them (elements 2 h + 1, 2 h + 2) and the first and last element by themselves. A lane reads
-    // the word behind its own as well: a shuffle in this function cost the kernel a third more code.
-    const int h = lane & 15, n = min(32, rows - row), left = min(32, N - col);  // columns of the matrix in the box
+    // Two rows at a time, 16 lanes each. A lane's rows all start on a word or all between two: there it
+    // stores the words between its own and the next (elements 2 h + 1, 2 h + 2), and the first and last
+    // lane the row's first and last element. A lane reads the word behind its own as well: a shuffle in
+    // this function cost the kernel a third more code.
+    const int h = lane & 15, n = rows - row, left = N - col;
     const int h1 = (h + 1) & 15;
-    uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row + (lane >> 4)) * ld + col;
+    int r = lane >> 4;
+    uint16_t* at = static_cast<uint16_t*>(p) + static_cast<long long>(row + r) * ld + col;
+    const bool odd = (reinterpret_cast<uintptr_t>(at) & 2u) != 0;
+    const uint32_t from = box + r * 64 + (h & 3) * 4, from1 = box + r * 64 + (h1 & 3) * 4;
+    const bool word = !odd || h < 15, end = odd && (h == 0 || h == 15);
+    uint16_t* at_word = at + 2 * h + (odd ? 1 : 0);
+    uint16_t* at_end = at + (h ? 31 : 0);
+    if (left >= 32) {
 #pragma unroll 1
-    for (int r0 = lane >> 4; r0 < 32; r0 += 8) {
-      uint32_t w[4], next[4];
+      for (int i0 = 0; i0 < 16; i0 += 8) {
+        uint32_t w[8], next[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 2 * i;
-        const uint32_t at_r = box + r * 64, s = (r >> 1) & 3;
-        w[i] = lds32(at_r + (((h >> 2) ^ s) << 4) + (h & 3) * 4);
-        next[i] = lds32(at_r + (((h1 >> 2) ^ s) << 4) + (h1 & 3) * 4);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (r0 + 2 * i < n) {
-          const bool odd = (reinterpret_cast<uintptr_t>(at) & 2u) != 0;
-          const int e = odd ? 2 * h + 1 : 2 * h;  // first element of this lane's word
-          const uint32_t v = odd ? __funnelshift_r(w[i], next[i], 16) : w[i];
-          if (e + 1 < left && e < 31)
-            *reinterpret_cast<uint32_t*>(at + e) = v;
-          else if (e < left)
-            at[e] = static_cast<uint16_t>(v);
-          if (odd && h == 0) at[0] = static_cast<uint16_t>(w[i]);
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t o = (i0 + i) * 128;
+          w[i] = lds32(from + o + (((h >> 2) ^ (i & 3)) << 4));
+          next[i] = lds32(from1 + o + (((h1 >> 2) ^ (i & 3)) << 4));
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (r < n) {
+            if (word) *reinterpret_cast<uint32_t*>(at_word) = __funnelshift_r(w[i], next[i], odd ? 16 : 0);
+            if (end) *at_end = static_cast<uint16_t>(h ? w[i] >> 16 : w[i]);
+          }
+          r += 2;
+          at_word += 2 * ld;
+          at_end += 2 * ld;
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w = lds32(from + i * 128 + (((h >> 2) ^ (i & 3)) << 4));
+        if (r < n) {
+          if (2 * h < left) at[2 * h] = static_cast<uint16_t>(w);
+          if (2 * h + 1 < left) at[2 * h + 1] = static_cast<uint16_t>(w >> 16);
+        }
+        r += 2;
         at += 2 * ld;
       }
     }
