@@ -952,7 +952,11 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(CG == 2 ? 2 * p.workers : p.workers * p.split));
   cfg.blockDim = dim3(32 * (2 + EW));
-  cfg.dynamicSmemBytes = fixed + p.ring;
+  // A CTA never waits for TMEM: two grids whose pairs or clusters held it on one SM and wanted it on
+  // another would wait for each other. Whoever takes 128 of the 512 columns takes 46 KB at least, so
+  // what fits an SM's 228 KB has at most four such parts (the other kernels here take more for theirs).
+  constexpr uint32_t SHARE = tmem_cols(BN) / 128 * (46u << 10);
+  cfg.dynamicSmemBytes = std::max(fixed + p.ring, SHARE);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -564,3 +564,24 @@ def test_refused_pointers(torch_cuda):
     assert e.value.status == j1.CUDA
     j1.op_linear(x.cuda(), w, out)
     assert bool((out == 0).all())
+
+
+def test_many_shapes_at_once(torch_cuda):
+    """Products of CTA pairs, of clusters that share a tile and of single CTAs, started together on a stream each,
+    give what they give alone: none holds accumulators another waits for."""
+    blocks = [_block(9500, 704, 512, BF, 41), _block(1, 768, 768, BF, 42), _block(40, 1152, 768, HF, 43),
+              _block(300, 128, 640, BF, 44), _block(2048, 768, 192, HF, 45), _block(129, 64, 2048, BF, 46)]
+    refs = []
+    for b in blocks:
+        _step(b, sync=True)
+        refs.append({k: b[k].clone() for k in RESULTS})
+    streams = [torch.cuda.Stream() for _ in blocks]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for j in range(len(blocks)):
+            k = (i + j) % len(blocks)
+            _step(blocks[k], stream=streams[k].cuda_stream)
+    torch.cuda.synchronize()
+    for b, ref in zip(blocks, refs):
+        for k in RESULTS:
+            assert torch.equal(b[k], ref[k]), k
