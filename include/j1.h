@@ -447,16 +447,16 @@ J1_API j1_status j1_op_attention_noalloc(const void* qkv, int64_t t, int32_t hid
 /* ---- the feed-forward block for training and serving (no reference counterpart)
  * Row-major matrices of 16-bit elements on device memory, one token per row; `ld*` are row
  * strides in elements (>= the row's width, any alignment of a whole element). Any M >= 0,
- * N >= 1, K >= 1. Weights are used as a checkpoint stores them, [N, K]. Products accumulate in
- * FP32, every epilogue works on the unrounded FP32 values, each result is rounded once. Biases
- * and their gradients are FP32.
+ * N >= 1, K >= 1 up to 2^30 (a gated block's N up to 2^29). Weights are used as a checkpoint
+ * stores them, [N, K]. Products accumulate in FP32, every epilogue works on the unrounded FP32
+ * values, each result is rounded once. Biases and their gradients are FP32.
  *
- * All pointers of a call must be memory of the calling thread's current device, and `stream`
- * a stream of it (NULL: its default stream); other pointers give J1_ERR_INVALID_ARG. Results
- * must not overlap each other or any input, except that j1_op_linear's out may be its residual
- * (same pointer and row stride). Elements between a row's width and its stride are neither
- * read nor written. Equal inputs give equal bits: no result depends on the order in which
- * blocks finish.
+ * All pointers of a call must be device memory (not managed memory) of the calling thread's
+ * current device, and `stream` a stream of it (NULL: its default stream); other pointers give
+ * J1_ERR_INVALID_ARG. Results must not overlap each other or any input, except that
+ * j1_op_linear's out may be its residual (same pointer and row stride). Elements between a row's
+ * width and its stride are not written, and what they hold does not matter. Equal inputs give
+ * equal bits: no result depends on the order in which blocks finish.
  *
  * With sync = 0 the calls only enqueue work and may be captured into a CUDA graph; the first
  * call of each kind on a device loads its kernels and should come before any capture.

@@ -2,6 +2,7 @@
 // the launches. Everything here runs on the host. Device memory is only taken for operands whose
 // rows do not start on 16-byte boundaries: the products read such an operand from a copy, in
 // stream-ordered memory of the library's own pool (product() below).
+#include <atomic>
 #include <climits>
 #include <cstdint>
 #include <mutex>
@@ -12,23 +13,28 @@
 
 using namespace j1rt;
 
+#define FFN_TRY(expr)          \
+  do {                         \
+    const j1_status s_ = (expr); \
+    if (s_) return s_;         \
+  } while (0)
+
 namespace {
 
 constexpr int kMaxDevices = 64;
-constexpr int kMaxDim = 1 << 30;
+constexpr int kMaxDim = 1 << 30;       // M, N, K
+constexpr int kMaxGated = 1 << 29;     // N of a gated block: its two projections are rows of one product
 
 // The operators' error word (0: no timed-out wait), one per device: a file-scope array, so that
 // no call allocates (a call may be captured, or a pool may own all of the device's memory).
 struct FfnDevice {
-  std::once_flag once;
-  cudaError_t rc = cudaSuccess;
+  std::atomic<bool> ready{false};
   int* err = nullptr;
   int num_sms = 0;
-  std::once_flag pool_once;
-  cudaError_t pool_rc = cudaSuccess;
-  cudaMemPool_t pool = nullptr;
+  std::atomic<cudaMemPool_t> pool{nullptr};
 };
 FfnDevice g_dev[kMaxDevices];
+std::mutex g_dev_mutex;  // first use of a device and of its pool; a failure leaves them for the next call
 
 j1_status device_state(FfnDevice** out, int* ordinal) {
   int dev = 0;
@@ -36,11 +42,16 @@ j1_status device_state(FfnDevice** out, int* ordinal) {
   if (e != cudaSuccess) return cuda_error(e, "cudaGetDevice");
   if (dev < 0 || dev >= kMaxDevices) return set_error(J1_ERR_UNSUPPORTED, "device ordinal above 63");
   FfnDevice& s = g_dev[dev];
-  std::call_once(s.once, [&s, dev] {
-    s.rc = ffn_error_word(&s.err);
-    if (s.rc == cudaSuccess) s.rc = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
-  });
-  if (s.rc != cudaSuccess) return cuda_error(s.rc, "error word");
+  if (!s.ready.load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> lock(g_dev_mutex);
+    cudaError_t rc = ffn_error_word(&s.err);
+    if (rc == cudaSuccess) rc = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
+    if (rc != cudaSuccess) {
+      cudaGetLastError();
+      return cuda_error(rc, "error word");
+    }
+    s.ready.store(true, std::memory_order_release);
+  }
   *out = &s;
   *ordinal = dev;
   return J1_OK;
@@ -71,17 +82,26 @@ bool overlap(const Arg& a, const Arg& b) {
   return d < static_cast<uint64_t>(a.cols) * a.elem || d + static_cast<uint64_t>(b.cols) * b.elem > row;
 }
 
-// Host checks of a call's sizes and matrices: strides, alignment, overlaps. `same`: index of an
-// input that the output `same_out` may coincide with.
-j1_status check_args(int dtype, int act, int M, int N, int K, const Arg* a, int n, int same = -1, int same_out = -1) {
-  if (dtype != J1_DTYPE_BF16 && dtype != J1_DTYPE_FP16) return bad("unknown dtype");
-  if (act < J1_ACT_NONE || act > J1_ACT_SILU) return bad("unknown activation");
+j1_status check_sizes(int M, int N, int K, int max_n) {
   if (M < 0 || N <= 0 || K <= 0) return bad("M must be >= 0, N and K positive");
   if (M > kMaxDim || N > kMaxDim || K > kMaxDim) return set_error(J1_ERR_UNSUPPORTED, "sizes above 2^30");
+  if (N > max_n) return set_error(J1_ERR_UNSUPPORTED, "N above 2^29");
+  return J1_OK;
+}
+
+// Host checks of a call's sizes and matrices: strides, alignment, overlaps. `same`: index of an
+// input that the output `same_out` may coincide with.
+j1_status check_args(int dtype, int act, int M, int N, int K, int max_n, const Arg* a, int n, int same = -1,
+                     int same_out = -1) {
+  if (dtype != J1_DTYPE_BF16 && dtype != J1_DTYPE_FP16) return bad("unknown dtype");
+  if (act < J1_ACT_NONE || act > J1_ACT_SILU) return bad("unknown activation");
+  FFN_TRY(check_sizes(M, N, K, max_n));
   for (int i = 0; i < n; ++i) {
     if (!a[i].p) continue;
     if (a[i].ld < a[i].cols) return bad(std::string(a[i].name) + ": row stride below the row's width");
     if (a[i].ld > (int64_t(1) << 38)) return set_error(J1_ERR_UNSUPPORTED, std::string(a[i].name) + ": row stride above 2^38");
+    if (a[i].rows > 1 && a[i].ld > (int64_t(1) << 46) / (a[i].rows - 1))
+      return set_error(J1_ERR_UNSUPPORTED, std::string(a[i].name) + ": more than 2^46 elements");
     if (a[i].lo() % a[i].elem) return bad(std::string(a[i].name) + ": not aligned to its element type");
   }
   for (int i = 0; i < n; ++i) {
@@ -106,9 +126,8 @@ j1_status check_device(const Arg* a, int n, int device) {
       cudaGetLastError();
       return cuda_error(e, a[i].name);
     }
-    if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
-      return bad(std::string(a[i].name) + " is not device memory");
-    if (at.type == cudaMemoryTypeDevice && at.device != device)
+    if (at.type != cudaMemoryTypeDevice) return bad(std::string(a[i].name) + " is not device memory");
+    if (at.device != device)
       return bad(std::string(a[i].name) + " is on device " + std::to_string(at.device) + ", the current device is " +
                  std::to_string(device));
   }
@@ -147,17 +166,29 @@ FfnGemm gemm_for(int dtype, int layout, int M, int N, int K, const FfnDevice* d)
 }
 
 // The device's pool, which keeps what it has taken (as a model's workspace does).
-cudaError_t device_pool(FfnDevice* d, int dev) {
-  std::call_once(d->pool_once, [d, dev] {
-    cudaMemPoolProps props = {};
-    props.allocType = cudaMemAllocationTypePinned;
-    props.location.type = cudaMemLocationTypeDevice;
-    props.location.id = dev;
-    d->pool_rc = cudaMemPoolCreate(&d->pool, &props);
-    uint64_t keep = UINT64_MAX;
-    if (d->pool_rc == cudaSuccess) d->pool_rc = cudaMemPoolSetAttribute(d->pool, cudaMemPoolAttrReleaseThreshold, &keep);
-  });
-  return d->pool_rc;
+cudaError_t device_pool(FfnDevice* d, int dev, cudaMemPool_t* out) {
+  cudaMemPool_t pool = d->pool.load(std::memory_order_acquire);
+  if (!pool) {
+    std::lock_guard<std::mutex> lock(g_dev_mutex);
+    pool = d->pool.load(std::memory_order_relaxed);
+    if (!pool) {
+      cudaMemPoolProps props = {};
+      props.allocType = cudaMemAllocationTypePinned;
+      props.location.type = cudaMemLocationTypeDevice;
+      props.location.id = dev;
+      cudaError_t e = cudaMemPoolCreate(&pool, &props);
+      if (e != cudaSuccess) return e;
+      uint64_t keep = UINT64_MAX;
+      e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
+      if (e != cudaSuccess) {
+        cudaMemPoolDestroy(pool);
+        return e;
+      }
+      d->pool.store(pool, std::memory_order_release);
+    }
+  }
+  *out = pool;
+  return cudaSuccess;
 }
 
 // One product. TMA reads rows on 16-byte boundaries only; other operands are copied first. (Reading
@@ -187,8 +218,9 @@ j1_status product(FfnGemm& g, FfnDevice* d, int dev, cudaStream_t st, const char
   void* mem = nullptr;
   if (c.n) {
     if (take_fault(J1_FAULT_ALLOC)) return set_error(J1_ERR_OOM, std::string(what) + ": device allocation failed (injected)");
-    cudaError_t e = device_pool(d, dev);
-    if (e == cudaSuccess) e = cudaMallocFromPoolAsync(&mem, bytes, d->pool, st);
+    cudaMemPool_t pool;
+    cudaError_t e = device_pool(d, dev, &pool);
+    if (e == cudaSuccess) e = cudaMallocFromPoolAsync(&mem, bytes, pool, st);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return cuda_error(e, what);
@@ -229,8 +261,7 @@ Workspace workspace_for(int M, int N, int K, int projections) {
 
 j1_status workspace_query(int M, int N, int K, int projections, size_t* bytes) {
   if (!bytes) return bad("NULL argument");
-  if (M < 0 || N <= 0 || K <= 0) return bad("M must be >= 0, N and K positive");
-  if (M > kMaxDim || N > kMaxDim || K > kMaxDim) return set_error(J1_ERR_UNSUPPORTED, "sizes above 2^30");
+  FFN_TRY(check_sizes(M, N, K, projections == 2 ? kMaxGated : kMaxDim));
   *bytes = workspace_for(M, N, K, projections).bytes;
   return J1_OK;
 }
@@ -247,12 +278,6 @@ j1_status check_workspace(const void* p, size_t bytes, size_t need) {
     if (take_fault(J1_FAULT_LAUNCH)) return cuda_error(cudaErrorLaunchFailure, what " (injected)"); \
     const int rc_ = (expr);                                                \
     if (rc_) return cuda_error(static_cast<cudaError_t>(rc_), what);       \
-  } while (0)
-
-#define FFN_TRY(expr)          \
-  do {                         \
-    const j1_status s_ = (expr); \
-    if (s_) return s_;         \
   } while (0)
 
 j1_status zero_rows(void* p, int64_t ld, int rows, int cols, size_t elem, cudaStream_t st) {
@@ -274,7 +299,7 @@ j1_status j1_op_linear(const j1_linear_args* a, void* stream, int sync) {
                         {"residual", a->residual, a->M, a->N, a->ldr, 2, false},
                         {"out", a->out, a->M, a->N, a->ldo, 2, true},
                         {"pre", a->pre, a->M, a->N, a->ldp, 2, true}};
-    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 6, 3, 4));
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, kMaxDim, args, 6, 3, 4));
     FfnDevice* d;
     int dev;
     FFN_TRY(device_state(&d, &dev));
@@ -307,7 +332,7 @@ j1_status j1_op_gated(const j1_gated_args* a, void* stream, int sync) {
                         {"out", a->out, a->M, a->N, a->ldo, 2, true},
                         {"pre_a", a->pre_a, a->M, a->N, a->ldpa, 2, true},
                         {"pre_g", a->pre_g, a->M, a->N, a->ldpg, 2, true}};
-    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 8));
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, kMaxGated, args, 8));
     FfnDevice* d;
     int dev;
     FFN_TRY(device_state(&d, &dev));
@@ -355,7 +380,7 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
                         {"dbias", a->dbias, 1, a->N, a->N, 4, true},
                         {"workspace", a->workspace, 1, static_cast<int64_t>(a->workspace_bytes),
                          static_cast<int64_t>(a->workspace_bytes), 1, true}};
-    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 8));
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, kMaxDim, args, 8));
     const Workspace ws = workspace_for(a->M, a->N, a->K, 1);
     FFN_TRY(check_workspace(a->workspace, a->workspace_bytes, ws.bytes));
     FfnDevice* d;
@@ -424,7 +449,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
                         {"dbg", a->dbg, 1, a->N, a->N, 4, true},
                         {"workspace", a->workspace, 1, static_cast<int64_t>(a->workspace_bytes),
                          static_cast<int64_t>(a->workspace_bytes), 1, true}};
-    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, args, 12));
+    FFN_TRY(check_args(a->dtype, a->act, a->M, a->N, a->K, kMaxGated, args, 12));
     const Workspace ws = workspace_for(a->M, a->N, a->K, 2);
     FFN_TRY(check_workspace(a->workspace, a->workspace_bytes, ws.bytes));
     FfnDevice* d;

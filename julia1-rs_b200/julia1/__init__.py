@@ -1205,7 +1205,11 @@ def _ffn_sizes(x, w):
 
 
 def _ffn_workspace(t):
-    return (0, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+    if t is None:
+        return 0, 0
+    if not t.is_contiguous():
+        _ffn_bad("workspace", t, "a contiguous tensor")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 _ffn_ops = {}

@@ -194,3 +194,28 @@ def test_host_failure_becomes_a_status():
     finally:
         j1.inject_fault(j1.FAULT_HOST, 0)
     assert e.value.status == j1.OOM and "j1_op_linear" in str(e.value)
+
+
+def test_limits_of_sizes_and_strides():
+    """A gated block's two projections are the rows of one product, so its N has half the range; a matrix whose
+    last element's offset would not fit an address is refused."""
+    L = j1.lib()
+    p = torch.zeros(64, dtype=BF).data_ptr()
+    with pytest.raises(j1.J1Error) as e:
+        j1.op_gated_backward_workspace(1, 2 ** 29 + 1, 1)
+    assert e.value.status == j1.UNSUPPORTED
+    assert j1.op_gated_backward_workspace(1, 2 ** 29, 1) > 2 ** 31 and j1.op_linear_backward_workspace(1, 2 ** 30, 1) > 2 ** 31
+    n = 2 ** 29 + 1
+    a = j1.J1GatedArgs(0, 0, 1, n, 1, p, 1, p, 1, p, 1, None, None, p, n, None, 0, None, 0)
+    assert L.j1_op_gated(a, None, 1) == j1.UNSUPPORTED and "2^29" in j1.last_error()
+    a = j1.J1GatedGradArgs(0, 0, 1, n, 1, p, n, p, 1, p, 1, p, 1, p, n, p, n, p, 1, None, 0, None, 0, None, None, p, 1 << 40)
+    assert L.j1_op_gated_backward(a, None, 1) == j1.UNSUPPORTED and "2^29" in j1.last_error()
+    for ld, status in ((1 << 38, j1.UNSUPPORTED), ((1 << 38) + 1, j1.UNSUPPORTED)):
+        a = j1.J1LinearArgs(0, 0, 1 << 20, 8, 8, p, ld, p, 8, None, None, 0, p, 8, None, 0)
+        assert L.j1_op_linear(a, None, 1) == status and "x: " in j1.last_error()
+
+
+def test_workspace_is_contiguous():
+    """An expanded tensor counts far more elements than it has memory."""
+    for op in ("linear_backward", "gated_backward"):
+        _refused(op, "contiguous", workspace=torch.zeros(1, dtype=torch.uint8).expand(1 << 30))

@@ -566,6 +566,19 @@ def test_refused_pointers(torch_cuda):
     assert bool((out == 0).all())
 
 
+def test_managed_memory_is_refused(torch_cuda):
+    import ctypes as C
+    torch.zeros(1, device="cuda")
+    rt, p = C.CDLL("libcudart.so.12"), C.c_void_p()
+    assert rt.cudaMallocManaged(C.byref(p), C.c_size_t(4096), C.c_uint(1)) == 0
+    try:
+        w, out = torch.zeros((8, 16), device="cuda", dtype=BF), torch.zeros((4, 8), device="cuda", dtype=BF)
+        a = j1.J1LinearArgs(0, 0, 4, 8, 16, p, 16, w.data_ptr(), 16, None, None, 0, out.data_ptr(), 8, None, 0)
+        assert j1.lib().j1_op_linear(a, None, 1) == j1.INVALID_ARG and "x is not device memory" in j1.last_error()
+    finally:
+        rt.cudaFree(p)
+
+
 def test_many_shapes_at_once(torch_cuda):
     """Products of CTA pairs, of clusters that share a tile and of single CTAs, started together on a stream each,
     give what they give alone: none holds accumulators another waits for."""
