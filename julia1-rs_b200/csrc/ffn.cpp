@@ -193,7 +193,7 @@ cudaError_t device_pool(FfnDevice* d, int dev, cudaMemPool_t* out) {
 
 // One product. TMA reads rows on 16-byte boundaries only; other operands are copied first. (Reading
 // them in the product instead, loader warps shifting aligned 16-byte pieces into place, kept the
-// tensor cores waiting: 65536 x 771 x 1155 took 527-606 us. A copy costs its bytes twice.) The memory
+// tensor cores waiting: 65536 x 771 x 1155 took 527-606 us, with the copies 198. A copy costs its bytes twice.) The memory
 // is taken and given back in stream order: calls on several streams, and captured graphs, have
 // their own.
 j1_status product(FfnGemm& g, FfnDevice* d, int dev, cudaStream_t st, const char* what) {
