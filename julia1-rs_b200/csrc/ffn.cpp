@@ -231,6 +231,7 @@ j1_status product(FfnGemm& g, FfnDevice* d, int dev, cudaStream_t st, const char
     }
   }
   int rc = take_fault(J1_FAULT_LAUNCH) ? static_cast<int>(cudaErrorLaunchFailure) : 0;
+  if (c.n) g.early = 0;  // the copies wait
   if (!rc && c.n) rc = launch_ffn_copies(c, st);
   if (!rc) rc = launch_ffn_gemm(g, st);
   if (mem) {
@@ -397,8 +398,8 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
     FfnMat dp = {a->dout, a->lddo};
     const bool products = a->dx || a->dw;
     const bool copy = products && (slope || !ffn_rows16(dp));  // both products read it
+    FfnGrad k = {};
     if (copy || a->dbias) {
-      FfnGrad k = {};
       k.fp16 = a->dtype == J1_DTYPE_FP16;
       k.act = a->act;
       k.M = a->M, k.N = a->N;
@@ -409,15 +410,20 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       k.partials = reinterpret_cast<float*>(base + ws.sums);
       FFN_LAUNCH(launch_ffn_grad(k, st), "linear gradient launch");
     }
+    const bool sums = ffn_grad_sums(k);
+    const int apart = a->dx && (sums || a->dw);  // the sums and dw run beside dx
     if (a->dx) {
       FfnGemm g = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d);
       g.a[0] = dp;
       g.b[0] = {a->w, a->ldw};
       g.out[0] = {a->dx, a->lddx};
+      g.late = apart;
       FFN_TRY(product(g, d, dev, st, "dx launch"));
     }
+    if (sums) FFN_LAUNCH(launch_ffn_grad_sums(k, apart, st), "bias gradient launch");
     if (a->dw) {
       FfnGemm g = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
+      g.early = apart;
       g.a[0] = dp;
       g.b[0] = {a->x, a->ldx};
       g.out[0] = {a->dw, a->lddw};
@@ -482,6 +488,8 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
     k.sum1 = a->dbg;
     k.partials = reinterpret_cast<float*>(base + ws.sums);
     FFN_LAUNCH(launch_ffn_grad(k, st), "gated gradient launch");
+    const bool sums = ffn_grad_sums(k);
+    const int apart = a->dx && (sums || a->dwa);  // the sums and the weights' gradients run beside dx
     if (a->dx) {
       FfnGemm g = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d);
       g.segs = 2;
@@ -490,10 +498,13 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
       g.b[0] = {a->wa, a->ldwa};
       g.b[1] = {a->wg, a->ldwg};
       g.out[0] = {a->dx, a->lddx};
+      g.late = apart;
       FFN_TRY(product(g, d, dev, st, "dx launch"));
     }
+    if (sums) FFN_LAUNCH(launch_ffn_grad_sums(k, apart, st), "bias gradient launch");
     if (a->dwa) {  // both weights' gradients as one product: rows [0, np) of da | dg are dwa's
       FfnGemm g = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
+      g.early = apart;
       g.rows0 = a->N;
       g.row1 = np;
       g.a[0] = k.d0;

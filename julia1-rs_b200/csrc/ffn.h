@@ -40,6 +40,11 @@ struct FfnGemm {
   FfnMat pre[2];    // written; p NULL: not wanted
   float* partials;  // workspace of split contractions, NULL: never split
   size_t partial_bytes;
+  // Kernels of one call that do not need each other run at once: a `late` kernel lets the next one start
+  // only when everything before itself is complete, so an `early` one launched behind it (or behind an
+  // early one) finds its inputs ready without waiting; it waits at its end instead, so that what follows
+  // it still follows both.
+  int early, late;
   int* err;         // device error word
   int num_sms;
 };
@@ -76,5 +81,8 @@ struct FfnGrad {
 };
 int ffn_grad_slabs(int M, int N);
 int launch_ffn_grad(const FfnGrad& g, cudaStream_t stream);
+// Adds the slabs' sums where there are several and a sum is wanted (ffn_grad_sums); early: see FfnGemm.
+bool ffn_grad_sums(const FfnGrad& g);
+int launch_ffn_grad_sums(const FfnGrad& g, int early, cudaStream_t stream);
 
 }  // namespace j1rt

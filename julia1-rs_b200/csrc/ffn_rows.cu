@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
 // sum[c] = partials[0][c] + partials[1][c] + ... : 32 columns per block, 32 slab strides at once with
 // four loads in flight each (one stride of eight and a load at a time took 10 us for 395 slabs),
 // joined in a fixed order.
-__global__ void __launch_bounds__(1024) slab_sum_kernel(const float* partials, int slabs, int N, float* sum0, float* sum1) {
+__global__ void __launch_bounds__(1024) slab_sum_kernel(const float* partials, int slabs, int N, float* sum0, float* sum1, int early) {
   __shared__ float red[32][33];
   grid_dep_launch();
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -196,12 +196,12 @@ __global__ void __launch_bounds__(1024) slab_sum_kernel(const float* partials, i
   float* sum = blockIdx.y ? sum1 : sum0;
   const float* p = partials + static_cast<size_t>(blockIdx.y) * slabs * N;
   float t = 0.f;
-  grid_dep_wait();
+  if (!early) grid_dep_wait();
   if (c < N)
     for (int s = ty; s < slabs; s += 128) {
       float v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = s + 32 * i < slabs ? p[static_cast<size_t>(s + 32 * i) * N + c] : 0.f;
+      for (int i = 0; i < 4; ++i) v[i] = s + 32 * i < slabs ? __ldcg(p + static_cast<size_t>(s + 32 * i) * N + c) : 0.f;
       t += (v[0] + v[1]) + (v[2] + v[3]);
     }
   red[ty][lane] = t;
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(1024) slab_sum_kernel(const float* partials, i
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
   if (lane == 0 && blockIdx.x * 32 + ty < N && sum) sum[blockIdx.x * 32 + ty] = t;
+  if (early) grid_dep_wait();
 }
 
 bool vec_ok(const FfnMat& m) { return !m.p || ffn_rows16(m); }
@@ -325,9 +326,15 @@ int launch_ffn_grad(const FfnGrad& g, cudaStream_t st) {
   else
     e = g.gated ? launch_grad<__nv_bfloat16, true>(k, vec, grid, slab_rows, st)
                 : launch_grad<__nv_bfloat16, false>(k, vec, grid, slab_rows, st);
-  if (e != cudaSuccess || !k.partials || slabs == 1) return static_cast<int>(e);
+  return static_cast<int>(e);
+}
+
+bool ffn_grad_sums(const FfnGrad& g) { return (g.sum0 || g.sum1) && ffn_grad_slabs(g.M, g.N) > 1; }
+
+int launch_ffn_grad_sums(const FfnGrad& g, int early, cudaStream_t st) {
   return static_cast<int>(launch_kernel(slab_sum_kernel, dim3((g.N + 31) / 32, g.gated ? 2 : 1), dim3(1024), 0, st,
-                                        static_cast<const float*>(k.partials), slabs, g.N, g.sum0, g.sum1));
+                                        static_cast<const float*>(g.partials), ffn_grad_slabs(g.M, g.N), g.N, g.sum0,
+                                        g.sum1, early));
 }
 
 }  // namespace j1rt

@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
   const uint32_t full = sbias + EW * BIAS_BYTES, empty = full + 64, tfull = empty + 64, tempty = tfull + 16, drain = tempty + 16;
   const uint32_t tmem_slot = drain + 8, abort_word = tmem_slot + 4;
 
-  grid_dep_launch();
+  if (!p.late) grid_dep_launch();
   const int warp = __shfl_sync(0xffffffffu, warp_id(), 0), lane = lane_id();
   const int split = p.split;
   const int crank = CG == 2 || split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -499,7 +499,8 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
     asm volatile("bar.sync 1, %0;" ::"n"(32 * (2 + EW)) : "memory");
   }
   tc_fence_after();
-  grid_dep_wait();
+  if (!p.early) grid_dep_wait();
+  if (p.late) grid_dep_launch();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -893,6 +894,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
     else
       tmem_dealloc(tmem_base, tmem_cols(BN));
   }
+  if (p.early) grid_dep_wait();
 }
 
 // Adds the pieces of every tile of a stream-K product in order and writes the rounded result.

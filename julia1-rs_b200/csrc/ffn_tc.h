@@ -25,6 +25,7 @@ struct FfnTc {
   uint32_t ring;            // shared memory of the stages
   int vec_out, vec_pre, vec_res;  // rows of whole 16-byte units: 16-byte accesses
   int a_rows;               // rows of one A box (K-major A): fewer than 128 when M is smaller
+  int early, late;          // see FfnGemm
   int* err;
 };
 
