@@ -1,7 +1,7 @@
 // j1_op_linear, j1_op_gated and their backward passes: argument checks, workspace layout and
 // the launches. Everything here runs on the host. Device memory is only taken for operands whose
 // rows do not start on 16-byte boundaries: the products read such an operand from a copy, in
-// stream-ordered memory of the library's own pool (product() below).
+// stream-ordered memory of the library's own pool (Copies below).
 #include <atomic>
 #include <climits>
 #include <cstdint>
@@ -12,6 +12,13 @@
 #include "model.h"
 
 using namespace j1rt;
+
+#define FFN_LAUNCH(expr, what)                                             \
+  do {                                                                     \
+    if (take_fault(J1_FAULT_LAUNCH)) return cuda_error(cudaErrorLaunchFailure, what " (injected)"); \
+    const int rc_ = (expr);                                                \
+    if (rc_) return cuda_error(static_cast<cudaError_t>(rc_), what);       \
+  } while (0)
 
 #define FFN_TRY(expr)          \
   do {                         \
@@ -191,55 +198,73 @@ cudaError_t device_pool(FfnDevice* d, int dev, cudaMemPool_t* out) {
   return cudaSuccess;
 }
 
-// One product. TMA reads rows on 16-byte boundaries only; other operands are copied first. (Reading
-// them in the product instead, loader warps shifting aligned 16-byte pieces into place, kept the
-// tensor cores waiting: 65536 x 771 x 1155 took 527-606 us, with the copies 198. A copy costs its bytes twice.) The memory
-// is taken and given back in stream order: calls on several streams, and captured graphs, have
-// their own.
-j1_status product(FfnGemm& g, FfnDevice* d, int dev, cudaStream_t st, const char* what) {
-  FfnMat* operands[4];
-  FfnCopies c = {};
-  size_t bytes = 0, at[4];
-  const int na = g.segs, nb = g.gated ? 2 : g.segs;
-  for (int i = 0; i < na + nb; ++i) {
-    const bool a = i < na;
-    FfnMat& m = a ? g.a[i] : g.b[i - na];
-    FfnCopy& o = c.m[c.n];
-    o.rows = a ? (g.layout == FFN_TN ? g.K : g.M) : (g.layout == FFN_NT ? g.N : g.K);
-    o.cols = a ? (g.layout == FFN_TN ? g.M : g.K) : (g.layout == FFN_NT ? g.K : g.N);
-    if (o.rows == 1) m.ld = (static_cast<long long>(o.cols) + 7) / 8 * 8;  // one row: the stride is never used
-    if (ffn_rows16(m)) continue;
-    o.src = m;
-    o.dst.ld = (static_cast<long long>(o.cols) + 7) / 8 * 8;
-    operands[c.n] = &m;
-    at[c.n++] = bytes;
-    bytes += up256(static_cast<size_t>(o.rows) * o.dst.ld * 2);
+// Copies of a call's operands. TMA reads rows on 16-byte boundaries only; the products' other operands
+// are copied first, all in one launch. (Reading them in the product instead, loader warps shifting
+// aligned 16-byte pieces into place, kept the tensor cores waiting: 65536 x 771 x 1155 took 527-606 us,
+// with the copies 198. A copy costs its bytes twice.) The memory is taken and given back in stream
+// order: calls on several streams, and captured graphs, have their own.
+class Copies {
+ public:
+  explicit Copies(cudaStream_t st) : st_(st) {}
+  ~Copies() {
+    if (mem_) cudaFreeAsync(mem_, st_);
   }
-  void* mem = nullptr;
-  if (c.n) {
-    if (take_fault(J1_FAULT_ALLOC)) return set_error(J1_ERR_OOM, std::string(what) + ": device allocation failed (injected)");
+  Copies(const Copies&) = delete;
+  Copies& operator=(const Copies&) = delete;
+
+  // Notes the operands of a product that need it.
+  void add(FfnGemm& g) {
+    const int na = g.segs, nb = g.gated ? 2 : g.segs;
+    for (int i = 0; i < na + nb; ++i) {
+      const bool a = i < na;
+      FfnMat& m = a ? g.a[i] : g.b[i - na];
+      FfnCopy o = {};
+      o.rows = a ? (g.layout == FFN_TN ? g.K : g.M) : (g.layout == FFN_NT ? g.N : g.K);
+      o.cols = a ? (g.layout == FFN_TN ? g.M : g.K) : (g.layout == FFN_NT ? g.K : g.N);
+      const long long ld = (static_cast<long long>(o.cols) + 7) / 8 * 8;
+      if (o.rows == 1) m.ld = ld;  // one row: the stride is never used
+      if (ffn_rows16(m)) continue;
+      o.src = m;
+      o.dst.ld = ld;
+      operands_[c_.n] = &m;
+      at_[c_.n] = bytes_;
+      c_.m[c_.n++] = o;
+      bytes_ += up256(static_cast<size_t>(o.rows) * ld * 2);
+    }
+  }
+  // Makes the copies and puts them in their operands' places.
+  j1_status make(FfnDevice* d, int dev) {
+    if (!c_.n) return J1_OK;
+    if (take_fault(J1_FAULT_ALLOC)) return set_error(J1_ERR_OOM, "operand copies: device allocation failed (injected)");
     cudaMemPool_t pool;
     cudaError_t e = device_pool(d, dev, &pool);
-    if (e == cudaSuccess) e = cudaMallocFromPoolAsync(&mem, bytes, pool, st);
+    if (e == cudaSuccess) e = cudaMallocFromPoolAsync(&mem_, bytes_, pool, st_);
     if (e != cudaSuccess) {
       cudaGetLastError();
-      return cuda_error(e, what);
+      mem_ = nullptr;
+      return cuda_error(e, "operand copies");
     }
-    for (int i = 0; i < c.n; ++i) {
-      c.m[i].dst.p = static_cast<uint8_t*>(mem) + at[i];
-      *operands[i] = c.m[i].dst;
+    for (int i = 0; i < c_.n; ++i) {
+      c_.m[i].dst.p = static_cast<uint8_t*>(mem_) + at_[i];
+      *operands_[i] = c_.m[i].dst;
     }
+    FFN_LAUNCH(launch_ffn_copies(c_, st_), "operand copies");
+    return J1_OK;
   }
-  int rc = take_fault(J1_FAULT_LAUNCH) ? static_cast<int>(cudaErrorLaunchFailure) : 0;
-  if (c.n) g.early = 0;  // the copies wait
-  if (!rc && c.n) rc = launch_ffn_copies(c, st);
-  if (!rc) rc = launch_ffn_gemm(g, st);
-  if (mem) {
-    const cudaError_t e = cudaFreeAsync(mem, st);
-    if (!rc) rc = e;
+  j1_status release() {
+    void* mem = mem_;
+    mem_ = nullptr;
+    const cudaError_t e = mem ? cudaFreeAsync(mem, st_) : cudaSuccess;
+    return e == cudaSuccess ? J1_OK : cuda_error(e, "operand copies");
   }
-  return rc ? cuda_error(static_cast<cudaError_t>(rc), what) : J1_OK;
-}
+
+ private:
+  cudaStream_t st_;
+  FfnMat* operands_[4] = {};
+  FfnCopies c_ = {};
+  size_t bytes_ = 0, at_[4] = {};
+  void* mem_ = nullptr;
+};
 
 // ---- backward workspace: gradients at the pre-activations (rows padded to 32 elements; the
 // gated pair side by side), slab sums of the bias gradients, partial products of dw.
@@ -274,12 +299,22 @@ j1_status check_workspace(const void* p, size_t bytes, size_t need) {
   return J1_OK;
 }
 
-#define FFN_LAUNCH(expr, what)                                             \
-  do {                                                                     \
-    if (take_fault(J1_FAULT_LAUNCH)) return cuda_error(cudaErrorLaunchFailure, what " (injected)"); \
-    const int rc_ = (expr);                                                \
-    if (rc_) return cuda_error(static_cast<cudaError_t>(rc_), what);       \
-  } while (0)
+// The rest of a backward pass behind its row kernel: dx, and beside it the bias gradients' sums and the
+// weights' gradients.
+j1_status backward_products(const FfnGrad& k, FfnGemm* dx, FfnGemm* dw, cudaStream_t st) {
+  const bool sums = ffn_grad_sums(k);
+  const int apart = dx && (sums || dw);
+  if (dx) {
+    dx->late = apart;
+    FFN_LAUNCH(launch_ffn_gemm(*dx, st), "dx launch");
+  }
+  if (sums) FFN_LAUNCH(launch_ffn_grad_sums(k, apart, st), "bias gradient launch");
+  if (dw) {
+    dw->early = apart;
+    FFN_LAUNCH(launch_ffn_gemm(*dw, st), "dw launch");
+  }
+  return J1_OK;
+}
 
 j1_status zero_rows(void* p, int64_t ld, int rows, int cols, size_t elem, cudaStream_t st) {
   if (!p) return J1_OK;
@@ -315,7 +350,11 @@ j1_status j1_op_linear(const j1_linear_args* a, void* stream, int sync) {
       g.residual = {a->residual, a->ldr};
       g.out[0] = {a->out, a->ldo};
       g.pre[0] = {a->pre, a->ldp};
-      FFN_TRY(product(g, d, dev, st, "linear launch"));
+      Copies copies(st);
+      copies.add(g);
+      FFN_TRY(copies.make(d, dev));
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "linear launch");
+      FFN_TRY(copies.release());
     }
     return finish(d, st, sync);
   });
@@ -351,7 +390,11 @@ j1_status j1_op_gated(const j1_gated_args* a, void* stream, int sync) {
       g.out[0] = {a->out, a->ldo};
       g.pre[0] = {a->pre_a, a->ldpa};
       g.pre[1] = {a->pre_g, a->ldpg};
-      FFN_TRY(product(g, d, dev, st, "gated launch"));
+      Copies copies(st);
+      copies.add(g);
+      FFN_TRY(copies.make(d, dev));
+      FFN_LAUNCH(launch_ffn_gemm(g, st), "gated launch");
+      FFN_TRY(copies.release());
     }
     return finish(d, st, sync);
   });
@@ -398,6 +441,24 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
     FfnMat dp = {a->dout, a->lddo};
     const bool products = a->dx || a->dw;
     const bool copy = products && (slope || !ffn_rows16(dp));  // both products read it
+    if (copy) dp = {base + ws.grads, ws.ld};
+    FfnGemm gx = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d), gw = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
+    Copies copies(st);
+    if (a->dx) {
+      gx.a[0] = dp;
+      gx.b[0] = {a->w, a->ldw};
+      gx.out[0] = {a->dx, a->lddx};
+      copies.add(gx);
+    }
+    if (a->dw) {
+      gw.a[0] = dp;
+      gw.b[0] = {a->x, a->ldx};
+      gw.out[0] = {a->dw, a->lddw};
+      gw.partials = reinterpret_cast<float*>(base + ws.partials);
+      gw.partial_bytes = ws.partial_bytes;
+      copies.add(gw);
+    }
+    FFN_TRY(copies.make(d, dev));
     FfnGrad k = {};
     if (copy || a->dbias) {
       k.fp16 = a->dtype == J1_DTYPE_FP16;
@@ -405,32 +466,13 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       k.M = a->M, k.N = a->N;
       k.dout = {a->dout, a->lddo};
       k.p0 = {slope ? a->pre : nullptr, a->ldp};
-      if (copy) k.d0 = dp = {base + ws.grads, ws.ld};
+      if (copy) k.d0 = dp;
       k.sum0 = a->dbias;
       k.partials = reinterpret_cast<float*>(base + ws.sums);
       FFN_LAUNCH(launch_ffn_grad(k, st), "linear gradient launch");
     }
-    const bool sums = ffn_grad_sums(k);
-    const int apart = a->dx && (sums || a->dw);  // the sums and dw run beside dx
-    if (a->dx) {
-      FfnGemm g = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d);
-      g.a[0] = dp;
-      g.b[0] = {a->w, a->ldw};
-      g.out[0] = {a->dx, a->lddx};
-      g.late = apart;
-      FFN_TRY(product(g, d, dev, st, "dx launch"));
-    }
-    if (sums) FFN_LAUNCH(launch_ffn_grad_sums(k, apart, st), "bias gradient launch");
-    if (a->dw) {
-      FfnGemm g = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
-      g.early = apart;
-      g.a[0] = dp;
-      g.b[0] = {a->x, a->ldx};
-      g.out[0] = {a->dw, a->lddw};
-      g.partials = reinterpret_cast<float*>(base + ws.partials);
-      g.partial_bytes = ws.partial_bytes;
-      FFN_TRY(product(g, d, dev, st, "dw launch"));
-    }
+    FFN_TRY(backward_products(k, a->dx ? &gx : nullptr, a->dw ? &gw : nullptr, st));
+    FFN_TRY(copies.release());
     return finish(d, st, sync);
   });
 }
@@ -487,34 +529,33 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
     k.sum0 = a->dba;
     k.sum1 = a->dbg;
     k.partials = reinterpret_cast<float*>(base + ws.sums);
-    FFN_LAUNCH(launch_ffn_grad(k, st), "gated gradient launch");
-    const bool sums = ffn_grad_sums(k);
-    const int apart = a->dx && (sums || a->dwa);  // the sums and the weights' gradients run beside dx
+    // both weights' gradients are one product: rows [0, np) of da | dg are dwa's
+    FfnGemm gx = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d), gw = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
+    Copies copies(st);
     if (a->dx) {
-      FfnGemm g = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d);
-      g.segs = 2;
-      g.a[0] = k.d0;
-      g.a[1] = k.d1;
-      g.b[0] = {a->wa, a->ldwa};
-      g.b[1] = {a->wg, a->ldwg};
-      g.out[0] = {a->dx, a->lddx};
-      g.late = apart;
-      FFN_TRY(product(g, d, dev, st, "dx launch"));
+      gx.segs = 2;
+      gx.a[0] = k.d0;
+      gx.a[1] = k.d1;
+      gx.b[0] = {a->wa, a->ldwa};
+      gx.b[1] = {a->wg, a->ldwg};
+      gx.out[0] = {a->dx, a->lddx};
+      copies.add(gx);
     }
-    if (sums) FFN_LAUNCH(launch_ffn_grad_sums(k, apart, st), "bias gradient launch");
-    if (a->dwa) {  // both weights' gradients as one product: rows [0, np) of da | dg are dwa's
-      FfnGemm g = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
-      g.early = apart;
-      g.rows0 = a->N;
-      g.row1 = np;
-      g.a[0] = k.d0;
-      g.b[0] = {a->x, a->ldx};
-      g.out[0] = {a->dwa, a->lddwa};
-      g.out[1] = {a->dwg, a->lddwg};
-      g.partials = reinterpret_cast<float*>(base + ws.partials);
-      g.partial_bytes = ws.partial_bytes;
-      FFN_TRY(product(g, d, dev, st, "dw launch"));
+    if (a->dwa) {
+      gw.rows0 = a->N;
+      gw.row1 = np;
+      gw.a[0] = k.d0;
+      gw.b[0] = {a->x, a->ldx};
+      gw.out[0] = {a->dwa, a->lddwa};
+      gw.out[1] = {a->dwg, a->lddwg};
+      gw.partials = reinterpret_cast<float*>(base + ws.partials);
+      gw.partial_bytes = ws.partial_bytes;
+      copies.add(gw);
     }
+    FFN_TRY(copies.make(d, dev));
+    FFN_LAUNCH(launch_ffn_grad(k, st), "gated gradient launch");
+    FFN_TRY(backward_products(k, a->dx ? &gx : nullptr, a->dwa ? &gw : nullptr, st));
+    FFN_TRY(copies.release());
     return finish(d, st, sync);
   });
 }
