@@ -301,12 +301,13 @@ int launch_ffn_copies(const FfnCopies& c, cudaStream_t st) {
   return static_cast<int>(launch_kernel(copies_kernel, grid, dim3(256), 0, st, c));
 }
 
-// About eight blocks per SM over both dimensions, at least 32 rows each, at most 512 slabs; up to 64
-// rows in one slab, which saves the second kernel (2 us) for two more turns of the first (1 us).
+// About eight blocks per SM over both dimensions, at least 16 rows each (2048 x 768 x 1152 linear backward
+// 17.9 us, with 32 rows 18.9, with 8 18.6: more sums to add), at most 512 slabs; up to 64 rows in one
+// slab, which saves the second kernel (2 us) for two more turns of the first (1 us).
 int ffn_grad_slabs(int M, int N) {
   const long long cols = (static_cast<long long>(N) + GC - 1) / GC;
   long long slabs = (1184 + cols - 1) / cols;
-  const long long most = M <= 64 ? 1 : (static_cast<long long>(M) + 31) / 32;
+  const long long most = M <= 64 ? 1 : (static_cast<long long>(M) + 15) / 16;
   if (slabs > most) slabs = most;
   if (slabs > 512) slabs = 512;
   return slabs < 1 ? 1 : static_cast<int>(slabs);
