@@ -25,12 +25,20 @@ struct Plan {
   int sk_q, sk_r, group;  // stream-K groups; order of the tiles (tile_at)
 };
 
-// The tile shape and split with the least time by a model of both sides' measurements: microseconds
-// per 64-block of a tile with all SMs busy (single CTAs are bound by what they load through L2, 32 KB
-// per 128 x 128 block against 64 KB per 256 x 256 for a pair, so their blocks cost three quarters of a
-// pair's for a quarter of the work), fewer when few are, plus what a launch does not overlap.
-// Measured: 8192 x 8192 x 8192 CG 2 x 256 0.67-0.75 ms, x 192 0.80, CG 1 x 128 1.04; 512 x 768 x 768 11.8, 11,
-// 7.3 us and CG 1 x 64 5.6 us; 16 x 8192 x 8192 CG 1 x 128 30 us, in clusters of two 26 us.
+// The tile shape and split with the least time by a model: microseconds per 64-block of a tile when few
+// SMs work (lone: latency) and when all do (busy: single CTAs are bound by what they load through L2,
+// 32 KB per 128 x 128 block against 64 KB per 256 x 256 for a pair), a launch with its epilogue (base),
+// and what a cluster's exchange costs: its accumulators' rows shared out (more CTAs, fewer for each) and
+// its traffic (more pieces to read). The constants are fitted to the times of 124 products (all operand
+// orders and gated; 1 to 131072 rows, contractions of 64 to 131072, weights from HBM for few rows) under
+// every plan: the plan chosen costs 0.9% more than the best one on average, 21% at most; an earlier model
+// whose exchange cost the same for all rows 10%. Some of them (us), best plan first:
+//   768 x 768 x 1024 TN    CG 1 x 64 5.3, x 128 6.7, x 64 in clusters of two 7.1, CG 2 x 256 9.9
+//   1 x 2048 x 8192        CG 1 x 128 in fours 10.6, x 64 in fours 11.7, in twos 14, in eights 16, one CTA 21-23
+//   16 x 8192 x 8192       CG 1 x 128 in twos 25.0, one CTA 28.7
+//   8192 x 768 x 1152      CG 2 x 192 13.3, CG 1 x 128 15.4, CG 2 x 256 15.8
+//   8192 x 8192 x 2048     CG 2 x 256 186, x 192 186, CG 1 x 128 257
+//   768 x 768 x 32768 TN   stream-K 47, CG 1 x 128 in twos 57
 Plan choose(const FfnGemm& g, int kb) {
   const int sms = g.num_sms, pairs = std::max(1, std::min(kPairs, sms / 2));
   Plan best = {};
@@ -38,26 +46,33 @@ Plan choose(const FfnGemm& g, int kb) {
   const auto take = [&](const Plan& p) {
     if (p.us < best.us) best = p;
   };
-  // busy: microseconds per block when every SM works, lone: when few do
-  const auto single = [&](int cfg, int bn, double busy, double lone) {
-    const long long tiles = ceil_div(g.M, 128) * ceil_div(g.N, g.gated ? bn / 2 : bn);
-    const double rows = std::min<double>(g.M, 128.0) / 128.0;  // small A boxes load less
+  struct Single {
+    int cfg, bn;
+    double lone, busy, few, base, split, ctas, rows, traffic;  // few: more per block when A has few rows
+  };
+  const auto single = [&](const Single& c) {
+    const long long tiles = ceil_div(g.M, 128) * ceil_div(g.N, g.gated ? c.bn / 2 : c.bn);
+    const double rows = g.layout == FFN_TN ? 1.0 : std::min<double>(g.M, 128.0) / 128.0;  // small A boxes load less
+    const double quarters = g.M > 64 ? 4 : g.M > 32 ? 2 : 1;
     for (int s = 1; s <= 8 && s <= kb; s *= 2) {
       const long long ctas = tiles * s;
-      if (s > 1 && ctas > sms) break;
+      // clusters of four and eight do not fill every part of the GPU
+      if (s > 1 && ctas > (s == 2 ? sms : s == 4 ? sms * 7 / 8 : sms * 5 / 7)) break;
       const double load = std::min(1.0, static_cast<double>(ctas) / sms);
-      const double step = lone + (busy * (bn + 128 * rows) / (bn + 128) - lone) * load;
-      const double per = static_cast<double>(ceil_div(kb, s)) * std::max(step, lone);
-      take({cfg, 1, bn, s, false, static_cast<double>(ceil_div(ctas, sms)) * per + 2.8 + (s > 1 ? 1.0 + 0.05 * s : 0.0), 1, 1, 8});
+      const double full = c.busy * (c.bn + 128 * rows) / (c.bn + 128);
+      const double step = c.lone + std::max(0.0, full - c.lone) * load + c.few * (1.0 - rows);
+      double us = static_cast<double>(ceil_div(ctas, sms) * ceil_div(kb, s)) * step + c.base + (g.gated ? 0.7 : 0.0);
+      if (s > 1) us += c.split + c.ctas * s + c.rows * quarters / s + c.traffic * load * s;
+      take({c.cfg, 1, c.bn, s, false, us, 1, 1, 8});
     }
   };
-  single(FFN_CG1_128, 128, 0.30, 0.15);
-  if (!g.gated) single(FFN_CG1_64, 64, 0.17, 0.13);
-  const auto pair = [&](int cfg, int bn, double busy, double lone) {
+  single({FFN_CG1_128, 128, 0.18, 0.25, 0.02, 3.4, -1.0, 0.0, 1.9, 1.0});
+  if (!g.gated) single({FFN_CG1_64, 64, 0.13, 0.16, 0.055, 2.85, -0.9, 0.08, 1.5, 0.36});
+  const auto pair = [&](int cfg, int bn, double lone, double busy, double base) {
     const long long tiles = ceil_div(g.M, 256) * ceil_div(g.N, g.gated ? bn / 2 : bn);
     const double load = std::min(1.0, static_cast<double>(tiles) / pairs);
     const double step = lone + (busy - lone) * load;
-    take({cfg, 2, bn, 1, false, static_cast<double>(ceil_div(tiles, pairs)) * kb * step + 5.0, 1, 1, 8});
+    take({cfg, 2, bn, 1, false, static_cast<double>(ceil_div(tiles, pairs)) * kb * step + base + (g.gated ? 0.75 : 0.0), 1, 1, 8});
     if (g.layout == FFN_TN && bn == 256 && g.partials && tiles * kb < INT_MAX && tiles * kb >= pairs &&
         (tiles + pairs) * kPieceBytes <= g.partial_bytes) {
       // q workers for every r tiles, then a pass over the pieces. Tiles of the same place in their group
@@ -69,15 +84,15 @@ Plan choose(const FfnGemm& g, int kb) {
         for (int r = 1; r <= 8; ++r) {
           const long long side = order ? nt : mt, other = order ? mt : nt, q = pairs * static_cast<long long>(r) / tiles;
           if (side % r || q < 1 || q * r * kb >= (1ll << 32)) continue;
-          const double compute = static_cast<double>(tiles) * kb * busy / static_cast<double>(q * (tiles / r));
+          const double compute = static_cast<double>(tiles) * kb * 0.445 / static_cast<double>(q * (tiles / r));
           const double memory = static_cast<double>(side + r * other) * kb * (64 * 256 * 2) / 6.0e6;
-          take({cfg, 2, bn, 1, true, std::max(compute, memory) + 9.0 + 0.03 * static_cast<double>(tiles + pairs),
+          take({cfg, 2, bn, 1, true, std::max(compute, memory) + 2.1 + 0.115 * static_cast<double>(tiles + pairs),
                 static_cast<int>(q), r, static_cast<int>(order ? 1 : mt)});
         }
     }
   };
-  pair(FFN_CG2_256, 256, 0.40, 0.28);
-  if (g.layout == FFN_NT && !g.gated) pair(FFN_CG2_192, 192, 0.335, 0.22);
+  pair(FFN_CG2_256, 256, 0.28, 0.41, 4.85);
+  if (g.layout == FFN_NT && !g.gated) pair(FFN_CG2_192, 192, 0.22, 0.315, 4.1);
   return best;
 }
 

@@ -42,8 +42,8 @@
 // 183-188 us (1.26 PFLOP/s; 0.75 of the measured burst rate), with GELU 203, with GELU and saved pre-
 // activations 240-254 (0.8 GB at 3.2 TB/s); 8192 x 768 x 1152 with residual 16.2 us; gated 8192 x
 // 1152 x 768 22.4 us (1.29 PFLOP/s), gated 4096 x 8192 x 4096 saved 365-388 us (1.42-1.5 PFLOP/s);
-// 8192 x 8192 x 8192 0.755 ms (1.46 PFLOP/s); 16 x 8192 x 8192 26.8 us (5.0 TB/s, 0.77 of measured);
-// 1 x 768 x 768 4.5 us. Large products are bound by what their tiles read through L2 and by the power
+// 8192 x 8192 x 8192 0.755 ms (1.46 PFLOP/s); 16 x 8192 x 8192 24.8-26.8 us (5.0-5.4 TB/s, 0.77-0.83 of
+// measured); 1 x 768 x 768 4.0 us. Large products are bound by what their tiles read through L2 and by the power
 // cap (tensor pipe busy 79% without activation at 32768 rows, 69% with GELU), an epilogue of
 // exponentials by the latency of its chains (issue slots 45% busy), few rows by the weights' bytes, the
 // smallest by launch, set-up and first loads.
@@ -821,7 +821,8 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
               float4 x[FLY][2], y[FLY][2];
 #pragma unroll
               for (int s = 0; s < FLY; ++s) {
-                const uint32_t base = mapa_shared(at, s0 + s < split ? s0 + s : s0);
+                if (s0 + s >= split) continue;
+                const uint32_t base = mapa_shared(at, s0 + s);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                   x[s][i] = ld_cluster(base + i * 512);
