@@ -43,9 +43,25 @@ struct FfnDevice {
 FfnDevice g_dev[kMaxDevices];
 std::mutex g_dev_mutex;  // first use of a device and of its pool; a failure leaves them for the next call
 
+// The first CUDA call of a host thread may be one of these operators, and tensor maps can only be made with
+// a context that is current: the runtime binds the device's when it is asked to.
+cudaError_t bind_context(int dev) {
+  using GetCurrent = CUresult (*)(CUcontext*);
+  static const GetCurrent current = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuCtxGetCurrent", &fn, cudaEnableDefault, &found);
+    return e == cudaSuccess && found == cudaDriverEntryPointSuccess ? reinterpret_cast<GetCurrent>(fn) : nullptr;
+  }();
+  CUcontext ctx = nullptr;
+  if (current && current(&ctx) == CUDA_SUCCESS && ctx) return cudaSuccess;
+  return cudaSetDevice(dev);
+}
+
 j1_status device_state(FfnDevice** out, int* ordinal) {
   int dev = 0;
-  const cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = bind_context(dev);
   if (e != cudaSuccess) return cuda_error(e, "cudaGetDevice");
   if (dev < 0 || dev >= kMaxDevices) return set_error(J1_ERR_UNSUPPORTED, "device ordinal above 63");
   FfnDevice& s = g_dev[dev];

@@ -598,3 +598,39 @@ def test_many_shapes_at_once(torch_cuda):
     for b, ref in zip(blocks, refs):
         for k in RESULTS:
             assert torch.equal(b[k], ref[k]), k
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_two_threads(torch_cuda, shared):
+    """Steps from two host threads, on one stream (their kernels interleave) or one each: kernels of a backward pass
+    that start before the one ahead has ended still follow what they read, whatever is queued between them."""
+    import threading
+    blocks = [_block(300, 768, 384, BF, 51), _block(200, 333, 129, HF, 52)]
+    refs = []
+    for b in blocks:
+        _step(b, sync=True)
+        refs.append({k: b[k].clone() for k in RESULTS})
+        for k in RESULTS:
+            b[k].fill_(float("nan"))
+    one = torch.cuda.Stream()
+    streams = [one, one if shared else torch.cuda.Stream()]
+    errors = []
+    torch.cuda.synchronize()
+
+    def work(b, s):
+        try:
+            for _ in range(30):
+                _step(b, stream=s.cuda_stream)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(blocks, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for b, ref in zip(blocks, refs):
+        for k in RESULTS:
+            assert torch.equal(b[k], ref[k]), k
