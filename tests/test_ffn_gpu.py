@@ -634,3 +634,36 @@ def test_two_threads(torch_cuda, shared):
     for b, ref in zip(blocks, refs):
         for k in RESULTS:
             assert torch.equal(b[k], ref[k]), k
+
+
+# Sizes whose products take every tile shape, cluster size and stream-K plan on a GPU of 148 SMs.
+PLANS = [("linear", (1, 32, 816)), ("linear", (100, 32, 816)), ("linear", (1, 880, 7464)), ("linear", (90, 880, 7464)),
+         ("linear", (1, 2080, 2546)), ("linear", (33, 2080, 2546)), ("linear", (50, 32, 200)), ("linear", (300, 40, 72)),
+         ("linear", (296, 3192, 336)), ("linear", (664, 3392, 392)), ("linear", (1479, 2472, 824)), ("linear", (5051, 69, 7661)),
+         ("gated", (1, 32, 200)), ("gated", (70, 32, 200)), ("gated", (1, 32, 488)), ("gated", (120, 65, 488)),
+         ("gated", (283, 3344, 728)), ("gated", (500, 700, 130)),
+         ("linear_backward", (1, 65, 36)), ("linear_backward", (1, 198, 33)), ("linear_backward", (1, 824, 32)),
+         ("linear_backward", (1, 2489, 2153)), ("linear_backward", (40, 1397, 4828)), ("linear_backward", (206, 33, 32)),
+         ("linear_backward", (478, 34, 32)), ("linear_backward", (71, 32, 32)), ("linear_backward", (155, 326, 4840)),
+         ("linear_backward", (1073, 402, 5106)), ("linear_backward", (1541, 986, 1431)), ("linear_backward", (2949, 32, 4868)),
+         ("linear_backward", (6012, 32, 2272)), ("linear_backward", (7356, 160, 2552)),
+         ("gated_backward", (1, 33, 38)), ("gated_backward", (1, 391, 32)), ("gated_backward", (1, 1128, 2120)),
+         ("gated_backward", (2, 3807, 835)), ("gated_backward", (1, 1168, 7560)), ("gated_backward", (226, 32, 32)),
+         ("gated_backward", (1035, 529, 2089)), ("gated_backward", (1309, 32, 2320)), ("gated_backward", (3338, 1070, 65)),
+         ("gated_backward", (4729, 32, 5184)), ("gated_backward", (7109, 96, 2560))]
+
+
+@pytest.mark.parametrize("i,op,size", [(i, op, s) for i, (op, s) in enumerate(PLANS)],
+                         ids=["%s-%s" % (op, _id(s)) for op, s in PLANS])
+def test_every_plan(torch_cuda, i, op, size):
+    dtype, act = TYPES[i % len(TYPES)]
+    if op == "linear":
+        check_linear(*size, dtype, act, bias=True, residual=True, save=True, seed=i)
+        check_linear(*size, dtype, act, bias=False, residual=False, save=False, seed=i)
+    elif op == "gated":
+        check_gated(*size, dtype, act, bias=True, save=True, seed=i)
+        check_gated(*size, dtype, act, bias=False, save=False, seed=i)
+    elif op == "linear_backward":
+        check_linear_backward(*size, dtype, act, seed=i)
+    else:
+        check_gated_backward(*size, dtype, act, seed=i)
