@@ -158,6 +158,14 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   for (int i = 0; i < nb; ++i)
     ok = ok && (g.layout == FFN_NT ? make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.N, g.K, g.b[i].ld, 64, b_rows, &why)
                                    : make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.K, g.N, g.b[i].ld, 64, b_rows, &why));
+  // the warps' own stores where rows are not whole 16-byte units (TMA would write the unit's rest), for one
+  // CTA's tiles (code that a launch of a few microseconds would fetch) and for results in two parts
+  p.tma_out = plan.cg == 2 && g.layout == FFN_NT && p.vec_out && p.vec_pre;
+  if (p.tma_out) {
+    ok = ok && make_tmap_16bit(&p.mo, g.fp16, g.out[0].p, g.M, g.N, g.out[0].ld, 32, 32, &why);
+    for (int i = 0; i < 2; ++i)
+      if (g.pre[i].p) ok = ok && make_tmap_16bit(&p.mp[i], g.fp16, g.pre[i].p, g.M, g.N, g.pre[i].ld, 32, 32, &why);
+  }
   if (!ok) return static_cast<int>(cudaErrorInvalidValue);
   return g.fp16 ? launch_ffn_tc_fp16(plan.cfg, g.layout, g.gated, p, stream)
                 : launch_ffn_tc_bf16(plan.cfg, g.layout, g.gated, p, stream);

@@ -28,8 +28,10 @@
 // The accumulator is double buffered in TMEM, so a tile's epilogue runs under the next tile's
 // products. The epilogue works on 32-column chunks, one thread per row: FP32 accumulators from
 // TMEM, bias, activation, residual, one rounding, then through a swizzled 32 x 32 box in shared
-// memory to coalesced 16-byte stores (words where rows are not 16-byte aligned: 8192 x 1153 x 768
-// with saved pre-activations 34 us, 47 with a settled alignment per row instead of per lane).
+// memory to the result. Pairs' forward boxes are stored by TMA where rows are whole 16-byte units
+// (131072 x 1152 x 768 with GELU and saved pre-activations 231 us, 249 with 16-byte stores by the warps);
+// other boxes by the warps, 16 bytes a lane, or words where rows are not 16-byte aligned (8192 x 1153 x
+// 768 with saved pre-activations 34 us; 47 with the alignment looked at per row instead of per lane).
 //
 // Code size counts: a launch of a few microseconds fetches its instructions cold, and a role's
 // loop that does not fit the innermost instruction cache costs about 180 cycles per turn. So single
@@ -39,9 +41,9 @@
 // GELU 212 us by halves, 203 whole).
 //
 // Measured on one B200 (CUDA graph, inputs larger than L2): 131072 x 1152 x 768 without activation
-// 183-188 us (1.26 PFLOP/s; 0.75 of the measured burst rate), with GELU 203, with GELU and saved pre-
-// activations 240-254 (0.8 GB at 3.2 TB/s); 8192 x 768 x 1152 with residual 16.2 us; gated 8192 x
-// 1152 x 768 22.4 us (1.29 PFLOP/s), gated 4096 x 8192 x 4096 saved 365-388 us (1.42-1.5 PFLOP/s);
+// 183-188 us (1.26 PFLOP/s; 0.75 of the measured burst rate), with GELU 200, with GELU and saved pre-
+// activations 217-231 (0.8 GB at 3.5 TB/s); 8192 x 768 x 1152 with residual 15.8 us; gated 8192 x
+// 1152 x 768 21.9 us (1.32 PFLOP/s), gated 4096 x 8192 x 4096 saved 365-388 us (1.42-1.5 PFLOP/s);
 // 8192 x 8192 x 8192 0.755 ms (1.46 PFLOP/s); 16 x 8192 x 8192 24.8-26.8 us (5.0-5.4 TB/s, 0.77-0.83 of
 // measured); 1 x 768 x 768 4.0 us. Large products are bound by what their tiles read through L2 and by the power
 // cap (tensor pipe busy 79% without activation at 32768 rows, 69% with GELU), an epilogue of
@@ -325,6 +327,13 @@ __device__ __forceinline__ void store_row8(const FfnMat& m, bool vec, long long 
     for (int i = 0; i < 8; ++i)
       if (col + i < N) at[i] = static_cast<uint16_t>(w[i >> 1] >> ((i & 1) * 16));
   }
+}
+
+// A box to columns from col, rows from row of a map's matrix; what is behind its edges (whole 16-byte
+// units) is left out.
+__device__ __forceinline__ void store_box(const CUtensorMap* map, uint32_t box, int col, int row) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(box), "r"(col), "r"(row)
+               : "memory");
 }
 
 // Copies a warp's box (32 rows x 32 columns, 64 bytes a row, unit u of row r at u ^ (r >> 1 & 3)) to rows
@@ -647,7 +656,13 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
       if (bias0) nb0 = in ? p.bias[0][col + lane] : 0.f;
       if (GATED && bias1) nb1 = in ? p.bias[1][col + lane] : 0.f;
     };
+    const bool tma = CG == 2 && LAYOUT == FFN_NT && p.tma_out;
+    auto boxes_free = [&]() {  // what was stored from them has been read
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+    };
     auto place = [&](int row, int col) {
+      if (tma && residual) boxes_free();
       if (bias0) sts32(wbias + lane * 4, __float_as_uint(nb0));
       if (GATED && bias1) sts32(wbias + 128 + lane * 4, __float_as_uint(nb1));
       if (residual) copy_in(box, p.residual.p, p.residual.ld, p.vec_res, row, M, col, N);
@@ -749,6 +764,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           tmem_ld_wait();
           if (j + H == 2 && c + 32 * PER >= OUTW) release();
           if (!in) continue;
+          if (tma) boxes_free();
           uint64_t v[8 * H];
           add16(bias0, wbias + j * 64, r0, v);
           if (save) put16(own + SLOT, j, v);
@@ -774,6 +790,20 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           put16(own, j, v);
         }
         if (!in) continue;
+        if (tma) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (save) {
+              store_box(&p.mp[0], box + SLOT, col, row);
+              if constexpr (GATED) store_box(&p.mp[1], box + 2 * SLOT, col, row);
+            }
+            store_box(&p.mo, box, col, row);
+            bulk_commit();
+          }
+          if (more) place(row, col + 32 * PER);
+          continue;
+        }
         if (save) {
           copy_out(box + SLOT, const_cast<void*>(p.pre[0].p), p.pre[0].ld, p.vec_pre, row, M, col, N);
           if (GATED) copy_out(box + 2 * SLOT, const_cast<void*>(p.pre[1].p), p.pre[1].ld, p.vec_pre, row, M, col, N);
@@ -784,6 +814,7 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
         if (more) place(row, col + 32 * PER);
       }
     }
+    if (tma && lane == 0) bulk_wait_all();
     if constexpr (CG == 1) {
       if (split > 1) {
         // All accumulators of the cluster are in shared memory. Units of 32 rows x 8 columns are

@@ -7,6 +7,7 @@ namespace j1rt {
 
 struct FfnTc {
   CUtensorMap ma[2], mb[2];
+  CUtensorMap mo, mp[2];    // out and pre in boxes of 32 x 32, where tma_out
   FfnMat a[2], b[2], out[2], pre[2], residual;
   const float* bias[2];
   int M, N, K;              // output rows, columns, contraction per segment
@@ -23,6 +24,7 @@ struct FfnTc {
   int stages;
   int boxes;                // 32 x 32 boxes per epilogue warp
   uint32_t ring;            // shared memory of the stages
+  int tma_out;              // pairs, forward: boxes are stored by TMA
   int vec_out, vec_pre, vec_res;  // rows of whole 16-byte units: 16-byte accesses
   int a_rows;               // rows of one A box (K-major A): fewer than 128 when M is smaller
   int early, late;          // see FfnGemm

@@ -667,3 +667,20 @@ def test_every_plan(torch_cuda, i, op, size):
         check_linear_backward(*size, dtype, act, seed=i)
     else:
         check_gated_backward(*size, dtype, act, seed=i)
+
+
+@pytest.mark.parametrize("pad", [0, 1, 8])
+def test_pairs_store_nothing_behind_rows(torch_cuda, pad):
+    """Tiles of CTA pairs over ragged rows and columns, stored as boxes where rows are whole 16-byte units (no padding, 8)
+    and element-wise otherwise; the residual in place, the rows behind the last one left as they were."""
+    for i, (dtype, act) in enumerate(TYPES[:3]):
+        for M, N, K in ((1479, 2472, 824), (700, 3392, 392)):
+            check_linear(M, N, K, dtype, act, bias=True, residual=True, save=True, pad=pad, seed=i, inplace=True)
+        check_gated(283, 3344, 728, dtype, act, bias=True, save=True, pad=pad, seed=i)
+    M, N, K = 1479, 2472, 824
+    g = gen(9)
+    x, w = mat(M, K, BF, g), mat(N, K, BF, g, K ** -0.5)
+    out, pre = (torch.full((M + 33, N), float("nan"), device="cuda", dtype=BF) for _ in range(2))
+    j1.op_linear(x, w, out[:M], act=j1.ACT_GELU, pre=pre[:M])
+    assert bool(out[M:].isnan().all()) and bool(pre[M:].isnan().all())
+    assert not bool(out[:M].isnan().any()) and not bool(pre[:M].isnan().any())
