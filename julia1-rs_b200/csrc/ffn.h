@@ -34,6 +34,7 @@ struct FfnGemm {
                // [rows0, row1) nowhere; INT_MAX: all to out[0]
   int rows0;
   FfnMat a[2], b[2];
+  long long lo;     // not 0: A is in two parts, what it was rounded by lies lo elements behind it
   const float* bias[2];
   FfnMat residual;  // p NULL: none
   FfnMat out[2];    // written
@@ -77,6 +78,7 @@ struct FfnGrad {
   FfnMat d0, d1;        // written: dp / da, dg
   float* sum0;          // [N] or NULL
   float* sum1;
+  long long lo;         // not 0: what d0 and d1 were rounded by goes lo elements behind them
   float* partials;      // ffn_grad_slabs(M, N) * 2 * N floats when a sum is wanted
 };
 int ffn_grad_slabs(int M, int N);

@@ -118,10 +118,11 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   const int nb = g.gated ? 2 : g.segs;
   for (int i = 0; i < 2; ++i) p.out[i] = g.out[i], p.pre[i] = g.pre[i], p.bias[i] = g.bias[i];
   p.M = g.M, p.N = g.N, p.K = g.K;
-  p.segs = g.segs;
+  p.segs = g.lo ? 2 * g.segs : g.segs;
+  p.b_and = g.segs - 1;
   p.kb_seg = static_cast<int>(ceil_div(g.K, 64));
-  if (static_cast<long long>(p.kb_seg) * g.segs > INT_MAX) return static_cast<int>(cudaErrorInvalidValue);
-  p.kb = p.kb_seg * g.segs;
+  if (static_cast<long long>(p.kb_seg) * p.segs > INT_MAX) return static_cast<int>(cudaErrorInvalidValue);
+  p.kb = p.kb_seg * p.segs;
   const Plan plan = choose(g, p.kb);
   p.act = g.act;
   p.row1 = g.row1, p.rows0 = g.rows0;
@@ -151,9 +152,12 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   }
   const char* why = nullptr;
   bool ok = true;
-  for (int i = 0; i < g.segs; ++i)
-    ok = ok && (g.layout == FFN_TN ? make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.K, g.M, g.a[i].ld, 64, 64, &why)
-                                   : make_tmap_16bit(&p.ma[i], g.fp16, g.a[i].p, g.M, g.K, g.a[i].ld, 64, p.a_rows, &why));
+  for (int i = 0; i < p.segs; ++i) {
+    FfnMat a = g.a[i & p.b_and];
+    if (i >= g.segs) a.p = static_cast<const uint16_t*>(a.p) + g.lo;
+    ok = ok && (g.layout == FFN_TN ? make_tmap_16bit(&p.ma[i], g.fp16, a.p, g.K, g.M, a.ld, 64, 64, &why)
+                                   : make_tmap_16bit(&p.ma[i], g.fp16, a.p, g.M, g.K, a.ld, 64, p.a_rows, &why));
+  }
   const uint32_t b_rows = g.layout != FFN_NT ? 64 : g.gated ? plan.bn / 2 : plan.bn / plan.cg;
   for (int i = 0; i < nb; ++i)
     ok = ok && (g.layout == FFN_NT ? make_tmap_16bit(&p.mb[i], g.fp16, g.b[i].p, g.N, g.K, g.b[i].ld, 64, b_rows, &why)

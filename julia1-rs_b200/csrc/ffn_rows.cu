@@ -68,6 +68,19 @@ __device__ __forceinline__ void store8(const FfnMat& m, long long row, int c0, i
   }
 }
 
+// What the values were rounded by when they were stored as T; 0 beyond T's range.
+template <typename T>
+__device__ __forceinline__ void rest(uint64_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    f2unpack(v[i], lo, hi);
+    const float2 f = Elem<T>::unpack(Elem<T>::pack(lo, hi));
+    lo -= f.x, hi -= f.y;
+    v[i] = f2pack(fabsf(lo) <= 3e38f ? lo : 0.f, fabsf(hi) <= 3e38f ? hi : 0.f);
+  }
+}
+
 template <typename T, bool GATED, int ACT, bool VEC>
 __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_rows) {
   __shared__ float red[GR][GC];
@@ -156,6 +169,14 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
       if (g.d0.p) store8<T, VEC>(g.d0, row, c0, lane, n, x);
       if constexpr (GATED) {
         if (g.d1.p) store8<T, VEC>(g.d1, row, c0, lane, n, z);
+      }
+      if (g.lo) {
+        rest<T>(x);
+        store8<T, VEC>({static_cast<const uint16_t*>(g.d0.p) + g.lo, g.d0.ld}, row, c0, lane, n, x);
+        if constexpr (GATED) {
+          rest<T>(z);
+          store8<T, VEC>({static_cast<const uint16_t*>(g.d1.p) + g.lo, g.d1.ld}, row, c0, lane, n, z);
+        }
       }
     }
     if constexpr (VEC) ask(r + DEPTH * GR);

@@ -527,14 +527,14 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           ok = false;
           break;
         }
-        const int seg = kb >= kb_seg ? 1 : 0;
-        const int k = (kb - (seg ? kb_seg : 0)) * BK;
+        const int seg = (kb >= kb_seg ? 1 : 0) + (kb >= 2 * kb_seg ? 1 : 0) + (kb >= 3 * kb_seg ? 1 : 0);
+        const int k = (kb - seg * kb_seg) * BK;
         const uint32_t da = sA + stage * a_bytes, db = sB + stage * B_BYTES;
         if (elect_one()) {
           if (leader) bar_expect(fb, CG * (a_bytes + B_BYTES));
           const uint32_t fc = CG == 2 ? mapa_shared(fb, 0) : fb;
           const CUtensorMap* ma = &p.ma[0] + seg;
-          const CUtensorMap* mb = &p.mb[0] + (GATED ? static_cast<int>(rank) : seg);
+          const CUtensorMap* mb = &p.mb[0] + (GATED ? static_cast<int>(rank) : seg & p.b_and);
           if constexpr (A_MN) {
             tma_box<CG>(ma, fc, da, m0, k);
             tma_box<CG>(ma, fc, da + A_BYTES / 2, m0 + 64, k);

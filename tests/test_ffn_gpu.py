@@ -684,3 +684,37 @@ def test_pairs_store_nothing_behind_rows(torch_cuda, pad):
     j1.op_linear(x, w, out[:M], act=j1.ACT_GELU, pre=pre[:M])
     assert bool(out[M:].isnan().all()) and bool(pre[M:].isnan().all())
     assert not bool(out[:M].isnan().any()) and not bool(pre[:M].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M,N,K", [(1, 5, 2000), (1, 300, 257), (16, 250, 129), (64, 64, 64), (170, 23, 40), (1, 4096, 72)])
+def test_few_gradients_in_two_parts(torch_cuda, dtype, M, N, K):
+    """Up to 2^12 gradients at the pre-activations reach the products in two parts: what the second part is rounded by
+    is a unit of a unit of the value (and a subnormal's half step), far below the result's own rounding."""
+    g = gen(M + N)
+    u, t = unit(dtype), tiny(dtype)
+    x, dout = mat(M, K, dtype, g), mat(M, N, dtype, g, 0.5)
+    ws = [mat(N, K, dtype, g, K ** -0.5) for _ in range(2)]
+    pre = [mat(M, N, dtype, g, 1.5) for _ in range(2)]
+    scr = scratch(j1.op_gated_backward_workspace(M, N, K))
+    d, p, q = dout.double(), pre[0].double(), pre[1].double()
+
+    def check(ds, es, weights, dx, dws):
+        off = [u * u * (v.abs() + e) + e + t for v, e in zip(ds, es)]
+        ref = sum(v @ w.double() for v, w in zip(ds, weights))
+        mag = sum((v.abs() + o) @ w.double().abs() for v, o, w in zip(ds, off, weights))
+        e = sum(o @ w.double().abs() for o, w in zip(off, weights)) + acc_err(2 * len(ds) * N) * mag
+        close("dx", dx, ref, u * (ref.abs() + e) + e + t + 1e-30)
+        for v, o, dw in zip(ds, off, dws):
+            ref = v.t() @ x.double()
+            e = o.t() @ x.double().abs() + acc_err(2 * M) * ((v.abs() + o).t() @ x.double().abs())
+            close("dw", dw, ref, u * (ref.abs() + e) + e + t + 1e-30)
+
+    dx, dw = mat(M, K, dtype), [mat(N, K, dtype) for _ in range(2)]
+    j1.op_linear_backward(dout, x, ws[0], pre=pre[0], act=j1.ACT_GELU, dx=dx, dw=dw[0], workspace=scr)
+    dp = d * slope64(p, "gelu")
+    check([dp], [d.abs() * SLOPE_ERR + 2.0 ** -23 * dp.abs()], ws[:1], dx, dw[:1])
+    j1.op_gated_backward(dout, x, ws[0], ws[1], pre[0], pre[1], act=j1.ACT_SILU, dx=dx, dwa=dw[0], dwg=dw[1], workspace=scr)
+    da, dg = d * q * slope64(p, "silu"), d * act64(p, "silu")
+    check([da, dg], [(d * q).abs() * SLOPE_ERR + 2.0 ** -22 * da.abs(), d.abs() * p.abs() * ACT_ERR + 2.0 ** -23 * dg.abs()],
+          ws, dx, dw)
