@@ -46,8 +46,8 @@
 // 1152 x 768 21.9 us (1.32 PFLOP/s), gated 4096 x 8192 x 4096 saved 365-388 us (1.42-1.5 PFLOP/s);
 // 8192 x 8192 x 8192 0.755 ms (1.46 PFLOP/s); 16 x 8192 x 8192 24.8-26.8 us (5.0-5.4 TB/s, 0.77-0.83 of
 // measured); 1 x 768 x 768 4.0 us. Large products are bound by what their tiles read through L2 and by the power
-// cap (tensor pipe busy 79% without activation at 32768 rows, 69% with GELU), an epilogue of
-// exponentials by the latency of its chains (issue slots 45% busy), few rows by the weights' bytes, the
+// cap (tensor pipe busy 77% without activation at 32768 rows, 67% with GELU), an epilogue of
+// exponentials by the latency of its chains (issue slots 44% busy), few rows by the weights' bytes, the
 // smallest by launch, set-up and first loads.
 #pragma once
 #include <cuda_runtime.h>
