@@ -496,8 +496,9 @@ J1_API j1_status j1_op_linear(const j1_linear_args* args, void* stream, int sync
 /* Gradients of j1_op_linear: dp = dout * act'(pre); dx = dp w; dw = dp^T x; dbias = sum of dp
  * over rows. dx, dw and dbias are written, not added to; each may be NULL (not wanted), not
  * all three. x is read for dw only, w for dx only, pre unless act is J1_ACT_NONE (where dp =
- * dout); what is not read may be NULL. dp is rounded to the dtype before the two products
- * (M N <= 2^12: kept in two parts of the dtype), dbias sums the unrounded values. The residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
+ * dout); what is not read may be NULL. For the two products dp is kept in two
+ * parts of the dtype, the second what the first was rounded by; dbias sums the unrounded values. The
+ * residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
  * workspace: at least j1_op_linear_backward_workspace bytes, 256-byte aligned; its contents
  * need not survive between calls, and calls that may overlap on the GPU need one each. */
 typedef struct j1_linear_grad_args {

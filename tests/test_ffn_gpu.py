@@ -718,3 +718,58 @@ def test_few_gradients_in_two_parts(torch_cuda, dtype, M, N, K):
     da, dg = d * q * slope64(p, "silu"), d * act64(p, "silu")
     check([da, dg], [(d * q).abs() * SLOPE_ERR + 2.0 ** -22 * da.abs(), d.abs() * p.abs() * ACT_ERR + 2.0 ** -23 * dg.abs()],
           ws, dx, dw)
+
+
+def check_in_parts(dtype, x, ds, es, weights, dx, dws, floor=0.0):
+    """dx and dw where the gradients at the pre-activations (ds, computed within es) reach the products in two parts:
+    the first cut to the type's bits, the second rounded to them, so within a unit of a unit of the value, and `floor`
+    for what lies below the second part's range."""
+    u, t, x = unit(dtype), tiny(dtype), x.double()
+    off = [u * u * (v.abs() + e) + e + floor for v, e in zip(ds, es)]
+    if dx is not None:
+        ref = sum(v @ w.double() for v, w in zip(ds, weights))
+        mag = sum((v.abs() + o) @ w.double().abs() for v, o, w in zip(ds, off, weights))
+        e = sum(o @ w.double().abs() for o, w in zip(off, weights)) + acc_err(2 * len(ds) * ds[0].shape[1]) * mag
+        close("dx", dx, ref, u * (ref.abs() + e) + e + t + 1e-30)
+    for v, o, dw in zip(ds, off, dws):
+        ref = v.t() @ x
+        e = o.t() @ x.abs() + acc_err(2 * x.shape[0]) * ((v.abs() + o).t() @ x.abs())
+        close("dw", dw, ref, u * (ref.abs() + e) + e + t + 1e-30)
+
+
+def rounded_once(name, got, ref):
+    """The errors of one rounding are uniform over a spacing s: squares of mean s^2 / 12 and variance s^4 / 180. All of
+    them together stay within five standard deviations of their mean and 10% for what else is in 32 bits (a dozen
+    roundings of 2^-24 per slope and sum: 1/200 of an FP16 unit); a second rounding of the terms doubles the mean."""
+    s2 = (torch.finfo(got.dtype).eps * torch.exp2(ref.abs().clamp_min(float(torch.finfo(got.dtype).tiny)).log2().floor())) ** 2
+    most = float(s2.sum() / 12 + 5 * (s2 * s2).sum().sqrt() / math.sqrt(180))
+    off = float((got.double() - ref).norm())
+    assert off <= 1.1 * math.sqrt(most), (name, off, math.sqrt(float(s2.sum()) / 12))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("M,N,K", [(1, 4104, 72), (64, 65, 300), (2, 8192, 64), (513, 130, 200), (2048, 768, 200), (4096, 64, 64),
+                                   (777, 333, 129), (30000, 136, 72)])
+def test_gradients_are_rounded_once_at_every_size(torch_cuda, dtype, M, N, K):
+    """However many gradients at the pre-activations there are, their rounding stays far below the results' own."""
+    g = gen(M + N)
+    x, dout = mat(M, K, dtype, g), mat(M, N, dtype, g, 0.5)
+    ws = [mat(N, K, dtype, g, K ** -0.5) for _ in range(2)]
+    pre = [mat(M, N, dtype, g, 1.5) for _ in range(2)]
+    scr = scratch(j1.op_gated_backward_workspace(M, N, K))
+    d, p, q = dout.double(), pre[0].double(), pre[1].double()
+    dx, dw = mat(M, K, dtype), [mat(N, K, dtype) for _ in range(2)]
+    for act in ("gelu", "relu"):
+        j1.op_linear_backward(dout, x, ws[0], pre=pre[0], act=ACTS[act], dx=dx, dw=dw[0], workspace=scr)
+        dp = d * slope64(p, act)
+        e = d.abs() * SLOPE_ERR + 2.0 ** -23 * dp.abs() if act == "gelu" else torch.zeros_like(d)
+        check_in_parts(dtype, x, [dp], [e], ws[:1], dx, dw[:1], tiny(dtype) * 4)
+        rounded_once("dx", dx, dp @ ws[0].double())
+        rounded_once("dw", dw[0], dp.t() @ x.double())
+    j1.op_gated_backward(dout, x, *ws, *pre, act=j1.ACT_SILU, dx=dx, dwa=dw[0], dwg=dw[1], workspace=scr)
+    da, dg = d * q * slope64(p, "silu"), d * act64(p, "silu")
+    check_in_parts(dtype, x, [da, dg], [(d * q).abs() * SLOPE_ERR + 2.0 ** -22 * da.abs(),
+                                        d.abs() * p.abs() * ACT_ERR + 2.0 ** -23 * dg.abs()], ws, dx, dw, tiny(dtype) * 4)
+    rounded_once("gated dx", dx, da @ ws[0].double() + dg @ ws[1].double())
+    rounded_once("dwa", dw[0], da.t() @ x.double())
+    rounded_once("dwg", dw[1], dg.t() @ x.double())
