@@ -283,7 +283,7 @@ class Copies {
 };
 
 // ---- backward workspace: gradients at the pre-activations (rows padded to 32 elements; the
-// gated pair side by side), slab sums of the bias gradients, partial products of dw.
+// gated pair side by side), FP16's scale, slab sums of the bias gradients, partial products of dw.
 int pad32(int n) { return (n + 31) / 32 * 32; }
 // They are kept in two parts (the rounded value and what it was rounded by: 16 significant bits of BF16, 22 of
 // FP16), whose products are summed in one accumulator, so that the results are rounded once as the formulas have
@@ -291,7 +291,7 @@ int pad32(int n) { return (n + 31) / 32 * 32; }
 // gradients and at 65536 x 1152 alike (errors and sums both grow with the root of the number of terms), for half
 // the products' time. Without an activation or with ReLU (linear) they are dout or 0: one part holds them.
 struct Workspace {
-  size_t grads, sums, partials, bytes;  // offsets of the three parts, total
+  size_t grads, scale, sums, partials, bytes;  // offsets of the four parts, total
   size_t partial_bytes;
   long long ld, lo;  // of the gradients: row stride, distance of the second part
 };
@@ -300,7 +300,8 @@ Workspace workspace_for(int M, int N, int K, int projections) {
   w.lo = static_cast<long long>(projections) * pad32(N);
   w.ld = 2 * w.lo;
   w.grads = 0;
-  w.sums = up256(static_cast<size_t>(M) * w.ld * 2);
+  w.scale = up256(static_cast<size_t>(M) * w.ld * 2);
+  w.sums = w.scale + up256(kFfnScaleFloats * sizeof(float));
   w.partials = w.sums + up256(static_cast<size_t>(ffn_grad_slabs(M, N)) * projections * N * 4);
   w.partial_bytes = ffn_partial_bytes(projections * pad32(N), K, M);
   w.bytes = w.partials + up256(w.partial_bytes);
@@ -468,8 +469,13 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
     const bool copy = products && (slope || !ffn_rows16(dp));  // both products read it
     if (copy) dp = {base + ws.grads, ws.ld};
     FfnGemm gx = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d), gw = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
+    FfnGrad k = {};
     Copies copies(st);
-    if (copy && slope && a->act != J1_ACT_RELU) gx.lo = gw.lo = ws.lo;
+    const bool dout_or_0 = !slope || a->act == J1_ACT_RELU;
+    if (copy && !dout_or_0) {
+      gx.lo = gw.lo = ws.lo;
+      if (a->dtype == J1_DTYPE_FP16) gx.scale = gw.scale = k.scale = reinterpret_cast<float*>(base + ws.scale);
+    }
     if (a->dx) {
       gx.a[0] = dp;
       gx.b[0] = {a->w, a->ldw};
@@ -485,7 +491,6 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       copies.add(gw);
     }
     FFN_TRY(copies.make(d, dev));
-    FfnGrad k = {};
     if (copy || a->dbias) {
       k.fp16 = a->dtype == J1_DTYPE_FP16;
       k.act = a->act;
@@ -553,6 +558,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
       k.d0 = {base + ws.grads, ws.ld};
       k.d1 = {base + ws.grads + static_cast<size_t>(np) * 2, ws.ld};
       k.lo = ws.lo;
+      if (k.fp16) k.scale = reinterpret_cast<float*>(base + ws.scale);
     }
     k.sum0 = a->dba;
     k.sum1 = a->dbg;
@@ -560,6 +566,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
     // both weights' gradients are one product: rows [0, np) of da | dg are dwa's
     FfnGemm gx = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d), gw = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
     gx.lo = gw.lo = k.lo;
+    gx.scale = gw.scale = k.scale;
     Copies copies(st);
     if (a->dx) {
       gx.segs = 2;

@@ -35,6 +35,7 @@ struct FfnGemm {
   int rows0;
   FfnMat a[2], b[2];
   long long lo;     // not 0: A is in two parts, what it was rounded by lies lo elements behind it
+  const float* scale;  // FP16: what a sum is multiplied by before it is rounded (device memory), NULL: 1
   const float* bias[2];
   FfnMat residual;  // p NULL: none
   FfnMat out[2];    // written
@@ -80,7 +81,12 @@ struct FfnGrad {
   float* sum1;
   long long lo;         // not 0: what d0 and d1 were rounded by goes lo elements behind them
   float* partials;      // ffn_grad_slabs(M, N) * 2 * N floats when a sum is wanted
+  // FP16, NULL: as they are. d0 and d1 are multiplied by a power of two of the call that brings the
+  // largest of their finite magnitudes to [2^14, 2^15); scale[0] receives its inverse, the rest is scratch.
+  float* scale;         // kFfnScaleFloats
 };
+constexpr int kFfnMaxBlocks = 888;
+constexpr int kFfnScaleFloats = 1 + kFfnMaxBlocks;
 int ffn_grad_slabs(int M, int N);
 int launch_ffn_grad(const FfnGrad& g, cudaStream_t stream);
 // Adds the slabs' sums where there are several and a sum is wanted (ffn_grad_sums); early: see FfnGemm.

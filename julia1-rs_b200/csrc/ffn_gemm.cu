@@ -141,6 +141,7 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   p.group = plan.stream_k ? plan.group : 8;
   p.a_rows = plan.cg == 1 && g.layout != FFN_TN && g.M < 128 ? (g.M + 7) / 8 * 8 : 128;
   p.early = g.early, p.late = g.late;
+  p.scale = g.scale;
   p.err = g.err;
   p.residual = g.residual;
   p.vec_res = g.residual.p && ffn_rows16(g.residual) && g.N % 8 == 0;

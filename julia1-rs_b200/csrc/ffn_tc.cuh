@@ -692,6 +692,14 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
                make_uint4(pack2<T>(v[4 * i]), pack2<T>(v[4 * i + 1]), pack2<T>(v[4 * i + 2]), pack2<T>(v[4 * i + 3])));
     };
 
+    // products of FP16 gradients: the power of two their operand was multiplied by is taken out here
+    constexpr bool SCALED = LAYOUT != FFN_NT && std::is_same<T, __half>::value;
+    uint64_t scale = 0ull;
+    if constexpr (SCALED) {
+      const float f = p.scale ? __ldcg(p.scale) : 1.f;
+      scale = f2pack(f, f);
+    }
+
     int acc = 0;
     bool ok = true;
     for (; ok && u.ok(); u.next(), u.at(mt, nt), ++acc) {
@@ -767,6 +775,10 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
           if (tma) boxes_free();
           uint64_t v[8 * H];
           add16(bias0, wbias + j * 64, r0, v);
+          if constexpr (SCALED) {
+#pragma unroll
+            for (int i = 0; i < 8 * H; ++i) v[i] = mul2(v[i], scale);
+          }
           if (save) put16(own + SLOT, j, v);
           act_all<8 * H>(act, v);
           if constexpr (GATED) {
@@ -877,6 +889,10 @@ __global__ void __launch_bounds__(32 * (2 + epi_warps(CG, BN, LAYOUT, GATED)), 1
               cluster_arrive();
               left = true;
             }
+            if constexpr (SCALED) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], scale);
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               v[i] = add2(v[i], f2pack(__shfl_sync(0xffffffffu, b0, 2 * i), __shfl_sync(0xffffffffu, b0, 2 * i + 1)));
@@ -965,6 +981,10 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Ffn
       t.z += x[i].z;
       t.w += x[i].w;
     }
+  }
+  if constexpr (std::is_same<T, __half>::value) {
+    const float f = p.scale ? __ldcg(p.scale) : 1.f;
+    t.x *= f, t.y *= f, t.z *= f, t.w *= f;
   }
   box[lane][cg * 4] = t.x;
   box[lane][cg * 4 + 1] = t.y;

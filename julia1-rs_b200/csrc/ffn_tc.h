@@ -22,6 +22,7 @@ struct FfnTc {
   int stream_k;             // each worker takes an equal share of all tiles' blocks; FP32 pieces to partials
   int sk_q, sk_r;           // stream-K: workers per group of tiles, tiles per group
   float* partials;
+  const float* scale;       // see FfnGemm
   int stages;
   int boxes;                // 32 x 32 boxes per epilogue warp
   uint32_t ring;            // shared memory of the stages

@@ -773,3 +773,60 @@ def test_gradients_are_rounded_once_at_every_size(torch_cuda, dtype, M, N, K):
     rounded_once("gated dx", dx, da @ ws[0].double() + dg @ ws[1].double())
     rounded_once("dwa", dw[0], da.t() @ x.double())
     rounded_once("dwg", dw[1], dg.t() @ x.double())
+
+
+@pytest.mark.parametrize("M,N,K", [(4096, 40, 24), (3, 100, 65), (300, 264, 72)])
+@pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -22, 2.0 ** 13])
+def test_fp16_gradients_keep_their_range(torch_cuda, M, N, K, size):
+    """FP16 gradients at the pre-activations far below and above the type's range, whose results are in it: both parts
+    are scaled by a power of two of the call, so only what is 2^-38 of the largest is lost."""
+    g = gen(M + K)
+    big = size > 1
+    x = mat(M, K, HF, g, M ** -0.5 * 2.0 ** -12 if big else 8.0)
+    ws = [mat(N, K, HF, g, N ** -0.5 * 2.0 ** -12 if big else 8.0) for _ in range(2)]
+    dout = mat(M, N, HF, g, size)
+    a = mat(M, N, HF, g, 1.5)
+    if not big:
+        a.sub_(4.0)  # slopes and values of the far side
+    q = mat(M, N, HF, g, 16.0 if big else 0.01)
+    scr = scratch(j1.op_gated_backward_workspace(M, N, K))
+    dx, dw = mat(M, K, HF), [mat(N, K, HF) for _ in range(2)]
+    db = [torch.empty(N, device="cuda") for _ in range(2)]
+    d, p, r = dout.double(), a.double(), q.double()
+    rel = 2.0 ** -18  # of a slope or value on the far side: its exponential's argument is rounded twice, |p| < 12
+
+    def check(ds, es, weights, dws):
+        floor = 2.0 ** -38 * max(float(v.abs().max()) for v in ds)
+        check_in_parts(HF, x, ds, es, weights, dx, dws, floor)
+        for v, e, b in zip(ds, es, db):
+            close("db", b, v.sum(0), e.sum(0) + acc_err(M) * (v.abs() + e).sum(0))
+
+    s = slope64(p, "silu")
+    dp = d * s
+    j1.op_linear_backward(dout, x, ws[0], pre=a, act=j1.ACT_SILU, dx=dx, dw=dw[0], dbias=db[0], workspace=scr)
+    slope_err = rel * (s.abs() + torch.sigmoid(p))
+    check([dp], [d.abs() * slope_err], ws[:1], dw[:1])
+    assert bool((dw[0] != 0).any()) and not bool(dx.isinf().any())
+    da, dg = d * r * s, d * act64(p, "silu")
+    j1.op_gated_backward(dout, x, *ws, a, q, act=j1.ACT_SILU, dx=dx, dwa=dw[0], dwg=dw[1], dba=db[0], dbg=db[1], workspace=scr)
+    check([da, dg], [(d * r).abs() * slope_err, rel * dg.abs()], ws, dw)
+
+
+def test_fp16_gradients_of_zeros_and_infinities(torch_cuda):
+    """The scale of a call whose gradients are all 0, or that holds infinities and NaN beside small ones."""
+    M, N, K = 40, 24, 16
+    g = gen(2)
+    x, w, pre = mat(M, K, HF, g), mat(N, K, HF, g), mat(M, N, HF, g)
+    dout, dx, dw = torch.zeros((M, N), device="cuda", dtype=HF), mat(M, K, HF), mat(N, K, HF)
+    scr = scratch(j1.op_linear_backward_workspace(M, N, K))
+    call = lambda: j1.op_linear_backward(dout, x, w, pre=pre, act=j1.ACT_GELU, dx=dx, dw=dw, workspace=scr)  # noqa: E731
+    call()
+    assert bool((dx == 0).all()) and bool((dw == 0).all())
+    dout.copy_(torch.randn((M, N), generator=g, device="cuda") * 2.0 ** -12)
+    call()
+    ref = dx.clone()
+    dout[7, 3], dout[9, 5], dout[11, 7] = float("inf"), float("nan"), -float("inf")
+    call()
+    assert bool(dx[9].isnan().all()) and bool(dx[[7, 11]].isinf().all())
+    rest = [i for i in range(M) if i not in (7, 9, 11)]
+    assert torch.equal(dx[rest], ref[rest])
