@@ -497,8 +497,8 @@ J1_API j1_status j1_op_linear(const j1_linear_args* args, void* stream, int sync
  * over rows. dx, dw and dbias are written, not added to; each may be NULL (not wanted), not
  * all three. x is read for dw only, w for dx only, pre unless act is J1_ACT_NONE (where dp =
  * dout); what is not read may be NULL. For the two products dp is kept in two
- * parts of the dtype, the second what the first was rounded by; in FP16 both are scaled by a power of
- * two of the call, taken out of the products' sums, so that only what is below 2^-38 of the largest finite dp
+ * parts of the dtype, both of its sign (an infinite x or w gives the infinity that dp itself would), the
+ * second what the first leaves; in FP16 both are scaled by a power of two of the call, taken out of the products' sums, so that only what is below 2^-38 of the largest finite dp
  * is lost. dbias sums the unrounded values. The residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
  * workspace: at least j1_op_linear_backward_workspace bytes, 256-byte aligned; its contents
  * need not survive between calls, and calls that may overlap on the GPU need one each. */

@@ -285,7 +285,7 @@ class Copies {
 // ---- backward workspace: gradients at the pre-activations (rows padded to 32 elements; the
 // gated pair side by side), FP16's scale, slab sums of the bias gradients, partial products of dw.
 int pad32(int n) { return (n + 31) / 32 * 32; }
-// They are kept in two parts (the rounded value and what it was rounded by: 16 significant bits of BF16, 22 of
+// They are kept in two parts (the value cut to the type and what is left of it: 16 significant bits of BF16, 22 of
 // FP16), whose products are summed in one accumulator, so that the results are rounded once as the formulas have
 // it. With one part the relative error of dx and dw against 64 bits is 0.00235 for BF16 and not 0.00166, at 1 x 64
 // gradients and at 65536 x 1152 alike (errors and sums both grow with the root of the number of terms), for half

@@ -34,7 +34,7 @@ struct FfnGemm {
                // [rows0, row1) nowhere; INT_MAX: all to out[0]
   int rows0;
   FfnMat a[2], b[2];
-  long long lo;     // not 0: A is in two parts, what it was rounded by lies lo elements behind it
+  long long lo;     // not 0: A is in two parts, the second lies lo elements behind the first
   const float* scale;  // FP16: what a sum is multiplied by before it is rounded (device memory), NULL: 1
   const float* bias[2];
   FfnMat residual;  // p NULL: none
@@ -79,7 +79,7 @@ struct FfnGrad {
   FfnMat d0, d1;        // written: dp / da, dg
   float* sum0;          // [N] or NULL
   float* sum1;
-  long long lo;         // not 0: what d0 and d1 were rounded by goes lo elements behind them
+  long long lo;         // not 0: d0 and d1 are kept in two parts, the second goes lo elements behind the first
   float* partials;      // ffn_grad_slabs(M, N) * 2 * N floats when a sum is wanted
   // FP16, NULL: as they are. d0 and d1 are multiplied by a power of two of the call that brings the
   // largest of their finite magnitudes to [2^14, 2^15); scale[0] receives its inverse, the rest is scratch.

@@ -26,6 +26,9 @@ struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
+  // Rounded towards zero (a NaN may become an infinity); the least magnitude that multiplies as itself.
+  static __device__ __forceinline__ float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+  static constexpr float kStep = 0x1p-126f;
 };
 template <>
 struct Elem<__half> {
@@ -42,6 +45,8 @@ struct Elem<__half> {
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
+  static __device__ __forceinline__ float cut(float v) { return __half2float(__float2half_rz(v)); }
+  static constexpr float kStep = 0x1p-24f;
 };
 
 // Minimum and maximum that keep a NaN (fminf / fmaxf drop it).

@@ -51,15 +51,8 @@ __device__ __forceinline__ void pairs(const uint4& u, uint64_t (&v)[4]) {
     v[i] = f2pack(f.x, f.y);
   }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(const FfnMat& m, long long row, int c0, int lane, int n, const uint64_t (&v)[4]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float lo, hi;
-    f2unpack(v[i], lo, hi);
-    w[i] = Elem<T>::pack(lo, hi);
-  }
+template <bool VEC>
+__device__ __forceinline__ void store8(const FfnMat& m, long long row, int c0, int lane, int n, const uint32_t (&w)[4]) {
   uint16_t* at = static_cast<uint16_t*>(const_cast<void*>(m.p)) + row * m.ld + c0;
   if constexpr (VEC) {
     if (c0 + lane * 8 < n) *reinterpret_cast<uint4*>(at + lane * 8) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -70,16 +63,33 @@ __device__ __forceinline__ void store8(const FfnMat& m, long long row, int c0, i
   }
 }
 
-// What the values were rounded by when they were stored as T; 0 beyond T's range.
+// The values rounded to T, or in two parts: cut to T's bits, and what is left, rounded. Both parts have the
+// value's sign and neither is 0 unless the value is (the second is 2^-24 of it at least, and T's smallest step):
+// an infinite factor then gives the infinity that the value itself would, not inf - inf or 0 inf.
 template <typename T>
-__device__ __forceinline__ void rest(uint64_t (&v)[4]) {
+__device__ __forceinline__ void rounded(const uint64_t (&v)[4], uint32_t (&w)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float lo, hi;
     f2unpack(v[i], lo, hi);
-    const float2 f = Elem<T>::unpack(Elem<T>::pack(lo, hi));
-    lo -= f.x, hi -= f.y;
-    v[i] = f2pack(fabsf(lo) <= 3e38f ? lo : 0.f, fabsf(hi) <= 3e38f ? hi : 0.f);
+    w[i] = Elem<T>::pack(lo, hi);
+  }
+}
+template <typename T>
+__device__ __forceinline__ float2 two_parts(float v) {
+  const float m = fabsf(v), first = Elem<T>::cut(m != 0.f ? max_nan(m, Elem<T>::kStep) : m);
+  const float left = max_nan(fmaxf(m - first, m * 0x1p-24f), Elem<T>::kStep);
+  return make_float2(copysignf(first, v), copysignf(m != 0.f ? left : 0.f, v));
+}
+template <typename T>
+__device__ __forceinline__ void two_parts(const uint64_t (&v)[4], uint32_t (&w)[4], uint32_t (&rest)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    f2unpack(v[i], lo, hi);
+    const float2 a = two_parts<T>(lo), b = two_parts<T>(hi);
+    w[i] = Elem<T>::pack(a.x, b.x);
+    rest[i] = Elem<T>::pack(a.y, b.y);
   }
 }
 
@@ -255,17 +265,19 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
           if constexpr (GATED) z[i] = mul2(z[i], scale);
         }
       }
-      if (g.d0.p) store8<T, VEC>(g.d0, row, c0, lane, n, x);
-      if constexpr (GATED) {
-        if (g.d1.p) store8<T, VEC>(g.d1, row, c0, lane, n, z);
-      }
-      if (g.lo) {
-        rest<T>(x);
-        store8<T, VEC>({static_cast<const uint16_t*>(g.d0.p) + g.lo, g.d0.ld}, row, c0, lane, n, x);
-        if constexpr (GATED) {
-          rest<T>(z);
-          store8<T, VEC>({static_cast<const uint16_t*>(g.d1.p) + g.lo, g.d1.ld}, row, c0, lane, n, z);
+      auto store = [&](const FfnMat& m, const uint64_t(&v)[4]) {
+        uint32_t w[4], left[4];
+        if (g.lo) {
+          two_parts<T>(v, w, left);
+          store8<VEC>({static_cast<const uint16_t*>(m.p) + g.lo, m.ld}, row, c0, lane, n, left);
+        } else {
+          rounded<T>(v, w);
         }
+        store8<VEC>(m, row, c0, lane, n, w);
+      };
+      if (g.d0.p) store(g.d0, x);
+      if constexpr (GATED) {
+        if (g.d1.p) store(g.d1, z);
       }
     }
     if constexpr (VEC) ask(r + DEPTH * GR);

@@ -830,3 +830,42 @@ def test_fp16_gradients_of_zeros_and_infinities(torch_cuda):
     assert bool(dx[9].isnan().all()) and bool(dx[[7, 11]].isinf().all())
     rest = [i for i in range(M) if i not in (7, 9, 11)]
     assert torch.equal(dx[rest], ref[rest])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("act,M,N,K", [("gelu", 4, 64, 40), ("silu", 30, 20, 33), ("relu", 1, 40, 264),
+                                       ("gelu_tanh", 130, 100, 72)])
+def test_infinite_operands_of_gradients(torch_cuda, dtype, act, M, N, K):
+    """An infinite weight, input or output gradient gives the infinities of the definition, in its own column or row,
+    and no NaN where that has none: both parts of a gradient at a pre-activation have its sign, and neither is 0."""
+    g = gen(M + N)
+    x, dout = mat(M, K, dtype, g), mat(M, N, dtype, g, 0.5)
+    ws = [mat(N, K, dtype, g, K ** -0.5) for _ in range(2)]
+    pre = [mat(M, N, dtype, g, 1.5) for _ in range(2)]
+    inf = float("inf")
+    ws[0][N // 2, 3], ws[1][N // 3, 5] = inf, -inf
+    x[M // 2, 7], x[M // 3, 9] = -inf, inf
+    d, p, q = dout.double(), pre[0].double(), pre[1].double()
+    dx, dw = mat(M, K, dtype), [mat(N, K, dtype) for _ in range(2)]
+    scr = scratch(j1.op_gated_backward_workspace(M, N, K))
+
+    def same(name, got, ref):
+        got = got.double()
+        for what in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(what(got), what(ref)), (name, what.__name__, int((what(got) != what(ref)).sum()))
+
+    for late in (False, True):
+        if late:  # a gradient that is infinite itself, in finite weights and inputs
+            for t in ws + [x]:
+                t[t.isinf()] = 1.0
+            dout[M - 1, 2], dout[M // 2, N - 1] = inf, -inf
+            d = dout.double()
+        dp = d * slope64(p, act)
+        j1.op_linear_backward(dout, x, ws[0], pre=pre[0], act=ACTS[act], dx=dx, dw=dw[0], workspace=scr)
+        same("linear dx", dx, (dp[:, :, None] * ws[0].double()).sum(1))
+        same("linear dw", dw[0], (dp[:, :, None] * x.double()[:, None]).sum(0))
+        da, dg = d * q * slope64(p, act), d * act64(p, act)
+        j1.op_gated_backward(dout, x, *ws, *pre, act=ACTS[act], dx=dx, dwa=dw[0], dwg=dw[1], workspace=scr)
+        same("gated dx", dx, (da[:, :, None] * ws[0].double() + dg[:, :, None] * ws[1].double()).sum(1))
+        same("gated dwa", dw[0], (da[:, :, None] * x.double()[:, None]).sum(0))
+        same("gated dwg", dw[1], (dg[:, :, None] * x.double()[:, None]).sum(0))
