@@ -26,9 +26,9 @@ struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ float2 unpack(uint32_t u) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
-  // Rounded towards zero (a NaN may become an infinity); the least magnitude that multiplies as itself.
+  // Rounded towards zero (a NaN may become an infinity); the smallest step.
   static __device__ __forceinline__ float cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
-  static constexpr float kStep = 0x1p-126f;
+  static constexpr float kStep = 0x1p-133f;
 };
 template <>
 struct Elem<__half> {

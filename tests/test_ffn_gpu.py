@@ -869,3 +869,15 @@ def test_infinite_operands_of_gradients(torch_cuda, dtype, act, M, N, K):
         same("gated dx", dx, (da[:, :, None] * ws[0].double() + dg[:, :, None] * ws[1].double()).sum(1))
         same("gated dwa", dw[0], (da[:, :, None] * x.double()[:, None]).sum(0))
         same("gated dwg", dw[1], (dg[:, :, None] * x.double()[:, None]).sum(0))
+
+
+def test_tiny_bf16_gradients(torch_cuda):
+    """Gradients at the pre-activations near the end of BF16's range keep both parts, down to its smallest step, 2^-133."""
+    M, N, K = 40, 64, 48
+    g = gen(6)
+    x, w, pre = mat(M, K, BF, g, 2.0 ** 100), mat(N, K, BF, g, 2.0 ** 100), mat(M, N, BF, g, 1.5)
+    dout, dx, dw = mat(M, N, BF, g, 2.0 ** -116), mat(M, K, BF), mat(N, K, BF)
+    j1.op_linear_backward(dout, x, w, pre=pre, act=j1.ACT_SILU, dx=dx, dw=dw,
+                          workspace=scratch(j1.op_linear_backward_workspace(M, N, K)))
+    d, s = dout.double(), slope64(pre.double(), "silu")
+    check_in_parts(BF, x, [d * s], [d.abs() * 2.0 ** -20], [w], dx, [dw], 2.0 ** -133)
