@@ -70,26 +70,46 @@ __device__ __forceinline__ float recip_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// Every activation here but ReLU is p times a logistic function of an odd polynomial of p, and all
-// are evaluated that way, with one exponential and one reciprocal per value (the exponential may
-// overflow on the far side: 1 / inf = 0):
-//   silu       p / (1 + 2^(-p log2 e))
-//   gelu_tanh  0.5 (1 + tanh z) = 1 / (1 + 2^(-2 z log2 e)),  z = sqrt(2/pi) (p + 0.044715 p^3)
-//   gelu       Phi(p) = 1 / (1 + 2^(-p R(p^2))): R(p^2) = log2(Phi / (1 - Phi)) / p is smooth and even; a
-//              polynomial of degree 6 in p^2, fitted here by reweighted least squares on |p| <= 6 to the
-//              smallest maximal error of Phi, is within 3e-8 of Phi (5e-8 in FP32 arithmetic), and its
-//              leading coefficient keeps it growing beyond.
+// Activations but ReLU are p times a factor s between 0 and 1, with one exponential and one reciprocal per value
+// (an exponential may overflow on the far side: 1 / inf = 0):
+//   silu       s = 1 / (1 + 2^(-p log2 e))
+//   gelu_tanh  s = 0.5 (1 + tanh z) = 1 / (1 + 2^(-2 z log2 e)),  z = sqrt(2/pi) (p + 0.044715 p^3)
+//   gelu       s = Phi(p) = 1 - Phi(-p);  Phi(-q) = e^(-q^2 / 2) u Q(u) for q >= 0, u = 1 / (1 + 0.3 q): the
+//              factor before u Q(u) has the tail's fall, and what is left is smooth in u on (0, 1]. Q, of degree 7, is
+//              fitted here to the smallest maximal error relative to Phi(-q), 1.7e-7 up to q = 14 (a linear
+//              program over 1500 points, coefficients rounded one after the other); 5e-7 in FP32 arithmetic up to
+//              q = 2, beyond it what the rounding of q^2 / 2 in the exponent makes, 8e-6 at q = 13.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTanhA = -2.302208198144325f;                // -2 sqrt(2 / pi) log2(e)
 constexpr float kTanhB = -2.302208198144325f * 0.044715f;
-__host__ __device__ constexpr float gelu_coef(int k) {  // minus the coefficient of p^(2 k) in R
-  return k == 0   ? -2.3022093772888184f
-         : k == 1 ? -0.10483512282371521f
-         : k == 2 ? 9.404900629306212e-05f
-         : k == 3 ? 1.5958001313265413e-04f
-         : k == 4 ? -1.1439842637628317e-05f
-         : k == 5 ? 3.8163187809914234e-07f
-                  : -5.06724973092787e-09f;
+__host__ __device__ constexpr float gelu_coef(int k) {  // of u^k in Q
+  return k == 0   ? 0.11962930113077164f
+         : k == 1 ? 0.12075395882129669f
+         : k == 2 ? 0.09991350769996643f
+         : k == 3 ? 0.1285615861415863f
+         : k == 4 ? -0.0536835677921772f
+         : k == 5 ? 0.20635342597961426f
+         : k == 6 ? -0.1572030633687973f
+                  : 0.03567477688193321f;
+}
+
+// Phi of a pair of values, and e^(-p^2 / 2).
+__device__ __forceinline__ uint64_t normal_cdf(uint64_t p, uint64_t& density) {
+  auto c2 = [](float c) { return f2pack(c, c); };
+  float a, b, d, e;
+  f2unpack(mul2(mul2(p, p), c2(-0.5f * kLog2e)), a, b);
+  density = f2pack(exp2_approx(a), exp2_approx(b));
+  f2unpack(fma2(p & 0x7fffffff7fffffffull, c2(0.3f), c2(1.f)), a, b);
+  const uint64_t u = f2pack(recip_approx(a), recip_approx(b));
+  uint64_t x = c2(gelu_coef(7));
+#pragma unroll
+  for (int k = 6; k >= 0; --k) x = fma2(x, u, c2(gelu_coef(k)));
+  x = mul2(mul2(x, u), density);
+  f2unpack(x, a, b);
+  f2unpack(fma2(x, c2(-1.f), c2(1.f)), d, e);
+  float p0, p1;
+  f2unpack(p, p0, p1);
+  return f2pack(p0 < 0.f ? a : d, p1 < 0.f ? b : e);
 }
 
 // act of a pair of values (packed FP32 arithmetic around the exponentials and reciprocals).
@@ -104,11 +124,7 @@ __device__ __forceinline__ uint64_t act_pair(uint64_t p) {
   auto c2 = [](float c) { return f2pack(c, c); };
   uint64_t x;
   if constexpr (ACT == J1_ACT_GELU) {
-    const uint64_t t = mul2(p, p);
-    x = c2(gelu_coef(6));
-#pragma unroll
-    for (int k = 5; k >= 0; --k) x = fma2(x, t, c2(gelu_coef(k)));
-    x = mul2(x, p);
+    return mul2(p, normal_cdf(p, x));
   } else if constexpr (ACT == J1_ACT_GELU_TANH) {
     x = mul2(p, fma2(mul2(p, p), c2(kTanhB), c2(kTanhA)));
   } else {
@@ -119,8 +135,8 @@ __device__ __forceinline__ uint64_t act_pair(uint64_t p) {
   return mul2(p, f2pack(recip_approx(a), recip_approx(b)));
 }
 
-// act'(p) and act(p) of a pair. With s the logistic function and x(p) its argument, act = p s and
-// act' = s + p s (1 - s) x'(p); for gelu p s (1 - s) x' is p phi(p), taken from the density itself.
+// act'(p) and act(p) of a pair. gelu: s + p phi(p). The others, with s the logistic function and x(p) its
+// argument: act = p s and act' = s + p s (1 - s) x'(p).
 // The tanh form's slope is constant to FP32 beyond |p| = 40; clamping there keeps 0 * inf out of it.
 template <int ACT>
 __device__ __forceinline__ void act_slope(uint64_t p, uint64_t& slope, uint64_t& value) {
@@ -133,6 +149,11 @@ __device__ __forceinline__ void act_slope(uint64_t p, uint64_t& slope, uint64_t&
     f2unpack(p, a, b);
     slope = f2pack(a > 0.f ? 1.f : 0.f, b > 0.f ? 1.f : 0.f);
     value = f2pack(a < 0.f ? 0.f : a, b < 0.f ? 0.f : b);
+  } else if constexpr (ACT == J1_ACT_GELU) {
+    uint64_t density;
+    const uint64_t s = normal_cdf(p, density);
+    value = mul2(p, s);
+    slope = fma2(mul2(p, c2(0.3989422804014327f)), density, s);
   } else {
     uint64_t h = p, x;
     if constexpr (ACT == J1_ACT_GELU_TANH) {
@@ -140,12 +161,7 @@ __device__ __forceinline__ void act_slope(uint64_t p, uint64_t& slope, uint64_t&
       h = f2pack(min_nan(max_nan(a, -40.f), 40.f), min_nan(max_nan(b, -40.f), 40.f));
     }
     const uint64_t t = mul2(h, h);
-    if constexpr (ACT == J1_ACT_GELU) {
-      x = c2(gelu_coef(6));
-#pragma unroll
-      for (int k = 5; k >= 0; --k) x = fma2(x, t, c2(gelu_coef(k)));
-      x = mul2(x, h);
-    } else if constexpr (ACT == J1_ACT_GELU_TANH) {
+    if constexpr (ACT == J1_ACT_GELU_TANH) {
       x = mul2(h, fma2(t, c2(kTanhB), c2(kTanhA)));
     } else {
       x = mul2(h, c2(-kLog2e));
@@ -154,16 +170,11 @@ __device__ __forceinline__ void act_slope(uint64_t p, uint64_t& slope, uint64_t&
     f2unpack(add2(f2pack(exp2_approx(a), exp2_approx(b)), c2(1.f)), a, b);
     const uint64_t s = f2pack(recip_approx(a), recip_approx(b));
     value = mul2(p, s);
-    if constexpr (ACT == J1_ACT_GELU) {
-      f2unpack(mul2(t, c2(-0.5f * kLog2e)), a, b);
-      slope = fma2(mul2(h, c2(0.3989422804014327f)), f2pack(exp2_approx(a), exp2_approx(b)), s);
-    } else {
-      const uint64_t rest = fma2(s, c2(-1.f), c2(1.f));  // 1 - s
-      if constexpr (ACT == J1_ACT_GELU_TANH)
-        slope = fma2(mul2(mul2(h, s), rest), fma2(t, c2(3.f * 0.044715f * 1.5957691216057308f), c2(1.5957691216057308f)), s);
-      else
-        slope = fma2(mul2(h, s), rest, s);
-    }
+    const uint64_t rest = fma2(s, c2(-1.f), c2(1.f));  // 1 - s
+    if constexpr (ACT == J1_ACT_GELU_TANH)
+      slope = fma2(mul2(mul2(h, s), rest), fma2(t, c2(3.f * 0.044715f * 1.5957691216057308f), c2(1.5957691216057308f)), s);
+    else
+      slope = fma2(mul2(h, s), rest, s);
   }
 }
 

@@ -881,3 +881,51 @@ def test_tiny_bf16_gradients(torch_cuda):
                           workspace=scratch(j1.op_linear_backward_workspace(M, N, K)))
     d, s = dout.double(), slope64(pre.double(), "silu")
     check_in_parts(BF, x, [d * s], [d.abs() * 2.0 ** -20], [w], dx, [dw], 2.0 ** -133)
+
+
+def _phi(p):
+    return torch.exp(torch.special.log_ndtr(p))
+
+
+# act(p) and act'(p) without the cancellation that 1 + erf or 1 + tanh has on the far side
+def _tail(p, act):
+    if act == "gelu":
+        s = _phi(p)
+        return p * s, s + p * torch.exp(-0.5 * p * p) / math.sqrt(2.0 * math.pi)
+    z = p if act == "silu" else 2.0 * math.sqrt(2.0 / math.pi) * (p + 0.044715 * p ** 3)
+    dz = torch.ones_like(p) if act == "silu" else 2.0 * math.sqrt(2.0 / math.pi) * (1.0 + 3 * 0.044715 * p * p)
+    s = torch.sigmoid(z)
+    return p * s, s + p * s * torch.sigmoid(-z) * dz
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_far_side_of_activations(torch_cuda, dtype, act):
+    """Negative pre-activations, where activation and slope are small: relative to the value itself, as long as it
+    is a normal number of the type. The exponential's argument (up to 126 binary orders) passes a few roundings of
+    2^-24 of itself, which the result has as a relative error; value and slope of one unit roundings besides. Factors
+    below 2^-126 may be 0 in 32 bits, and the slope has one of them times p and the argument's slope."""
+    p = torch.arange(-16.0, 0.0, 2.0 ** -6, device="cuda").to(dtype)
+    M, N, K = p.numel(), 8, 16
+    x, w = torch.zeros((M, K), device="cuda", dtype=dtype), torch.zeros((N, K), device="cuda", dtype=dtype)
+    x[:, 0], w[:, 0] = p, 1.0
+    out, dx = torch.empty((M, N), device="cuda", dtype=dtype), torch.empty((M, K), device="cuda", dtype=dtype)
+    j1.op_linear(x, w, out, act=ACTS[act])
+    value, slope = _tail(p.double(), act)
+    orders = (value / p.double()).log2().abs()  # of the logistic function or Phi
+    rel = 8 * 2.0 ** -24 * (orders + 8)
+    least = float(torch.finfo(dtype).tiny)
+    normal = value.abs() > 2 * least
+    assert int(normal.sum()) > (240 if dtype == HF else 600)
+    close("out", out[normal], value[normal, None].expand(-1, N), ((unit(dtype) + rel) * value.abs() + 2.0 ** -126 * p.double().abs())[normal, None])
+    # dx = N equal columns of act'(p), each with what its two terms of opposite sign were off by
+    w.zero_()
+    w[0, :] = 1.0
+    dout = torch.zeros((M, N), device="cuda", dtype=dtype)
+    dout[:, 0] = 1.0
+    pre = p[:, None].expand(M, N).contiguous()
+    j1.op_linear_backward(dout, x, w, pre=pre, act=ACTS[act], dx=dx, workspace=scratch(j1.op_linear_backward_workspace(M, N, K)))
+    terms = (value / p.double()).abs() + (slope - value / p.double()).abs()
+    steep = {"gelu": p.double().abs(), "silu": torch.ones_like(value), "gelu_tanh": 1.6 * (1 + 0.135 * p.double() ** 2)}[act]
+    normal = slope.abs() > 2 * least
+    close("dx", dx[normal], slope[normal, None].expand(-1, K), ((unit(dtype) + unit(dtype) ** 2) * slope.abs() + 2 * rel * terms + 2.0 ** -126 * (1 + p.double().abs() * steep))[normal, None])
