@@ -376,6 +376,12 @@ J1_API void j1_inject_fault(int32_t kind, int32_t count);
  * Returns J1_ERR_DEVICE_TIMEOUT (site 99) when the timeout was detected and reported, as a
  * forward's stuck wait would be; the context stays usable. */
 J1_API j1_status j1_selftest_device_timeout(int ordinal, int64_t limit_cycles);
+/* How a product of the feed-forward operators runs on a device of num_sms SMs (host only). product: 0
+ * j1_op_linear, 1 j1_op_gated, 2 dx and 3 dw of j1_op_linear_backward, 4 dx and 5 dw of
+ * j1_op_gated_backward. plan[6]: CTAs per tile, its accumulator columns, CTAs that share a tile's contraction, workers
+ * per group of tiles of a stream-K product (0: it is none), tiles per group, 1 where groups lie along columns. */
+J1_API j1_status j1_selftest_ffn_plan(int32_t product, int32_t act, int32_t M, int32_t N, int32_t K, int32_t num_sms,
+                                      int32_t* plan);
 
 /* ------------------------------------------------------------ kernel-level ops
  * On caller device memory (e.g. torch tensors); `stream` is a cudaStream_t or NULL.

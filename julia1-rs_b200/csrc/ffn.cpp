@@ -308,6 +308,28 @@ Workspace workspace_for(int M, int N, int K, int projections) {
   return w;
 }
 
+// The sizes of a backward pass's products, in `parts` parts of the gradients at the pre-activations: dx (a gated
+// block's projections are two segments) and dw (their weights' rows are one product, the second's from pad32(N)).
+FfnGemm dx_product(int dtype, int M, int N, int K, int projections, int parts, const Workspace& ws, const FfnDevice* d) {
+  FfnGemm g = gemm_for(dtype, FFN_NN, M, K, N, d);
+  g.segs = projections;
+  g.lo = parts == 2 ? ws.lo : 0;
+  return g;
+}
+FfnGemm dw_product(int dtype, int M, int N, int K, int projections, int parts, const Workspace& ws, void* workspace, const FfnDevice* d) {
+  FfnGemm g = gemm_for(dtype, FFN_TN, projections == 2 ? pad32(N) + N : N, K, M, d);
+  if (projections == 2) {
+    g.rows0 = N;
+    g.row1 = pad32(N);
+  }
+  g.lo = parts == 2 ? ws.lo : 0;
+  g.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.partials);
+  g.partial_bytes = ws.partial_bytes;
+  return g;
+}
+// Gradients of a linear layer without activation or with ReLU are dout or 0.
+int parts_for(int act, int projections) { return projections == 1 && (act == J1_ACT_NONE || act == J1_ACT_RELU) ? 1 : 2; }
+
 j1_status workspace_query(int M, int N, int K, int projections, size_t* bytes) {
   if (!bytes) return bad("NULL argument");
   FFN_TRY(check_sizes(M, N, K, projections == 2 ? kMaxGated : kMaxDim));
@@ -468,14 +490,13 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
     const bool products = a->dx || a->dw;
     const bool copy = products && (slope || !ffn_rows16(dp));  // both products read it
     if (copy) dp = {base + ws.grads, ws.ld};
-    FfnGemm gx = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d), gw = gemm_for(a->dtype, FFN_TN, a->N, a->K, a->M, d);
+    const int parts = parts_for(a->act, 1);
+    FfnGemm gx = dx_product(a->dtype, a->M, a->N, a->K, 1, parts, ws, d);
+    FfnGemm gw = dw_product(a->dtype, a->M, a->N, a->K, 1, parts, ws, base, d);
     FfnGrad k = {};
     Copies copies(st);
-    const bool dout_or_0 = !slope || a->act == J1_ACT_RELU;
-    if (copy && !dout_or_0) {
-      gx.lo = gw.lo = ws.lo;
-      if (a->dtype == J1_DTYPE_FP16) gx.scale = gw.scale = k.scale = reinterpret_cast<float*>(base + ws.scale);
-    }
+    if (products && parts == 2 && a->dtype == J1_DTYPE_FP16)
+      gx.scale = gw.scale = k.scale = reinterpret_cast<float*>(base + ws.scale);
     if (a->dx) {
       gx.a[0] = dp;
       gx.b[0] = {a->w, a->ldw};
@@ -486,8 +507,6 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       gw.a[0] = dp;
       gw.b[0] = {a->x, a->ldx};
       gw.out[0] = {a->dw, a->lddw};
-      gw.partials = reinterpret_cast<float*>(base + ws.partials);
-      gw.partial_bytes = ws.partial_bytes;
       copies.add(gw);
     }
     FFN_TRY(copies.make(d, dev));
@@ -498,7 +517,7 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       k.dout = {a->dout, a->lddo};
       k.p0 = {slope ? a->pre : nullptr, a->ldp};
       if (copy) k.d0 = dp;
-      k.lo = gx.lo;
+      if (copy) k.lo = gx.lo;
       k.sum0 = a->dbias;
       k.partials = reinterpret_cast<float*>(base + ws.sums);
       FFN_LAUNCH(launch_ffn_grad(k, st), "linear gradient launch");
@@ -563,13 +582,12 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
     k.sum0 = a->dba;
     k.sum1 = a->dbg;
     k.partials = reinterpret_cast<float*>(base + ws.sums);
-    // both weights' gradients are one product: rows [0, np) of da | dg are dwa's
-    FfnGemm gx = gemm_for(a->dtype, FFN_NN, a->M, a->K, a->N, d), gw = gemm_for(a->dtype, FFN_TN, np + a->N, a->K, a->M, d);
-    gx.lo = gw.lo = k.lo;
+    const int parts = parts_for(a->act, 2);
+    FfnGemm gx = dx_product(a->dtype, a->M, a->N, a->K, 2, parts, ws, d);
+    FfnGemm gw = dw_product(a->dtype, a->M, a->N, a->K, 2, parts, ws, base, d);
     gx.scale = gw.scale = k.scale;
     Copies copies(st);
     if (a->dx) {
-      gx.segs = 2;
       gx.a[0] = k.d0;
       gx.a[1] = k.d1;
       gx.b[0] = {a->wa, a->ldwa};
@@ -578,14 +596,10 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
       copies.add(gx);
     }
     if (a->dwa) {
-      gw.rows0 = a->N;
-      gw.row1 = np;
       gw.a[0] = k.d0;
       gw.b[0] = {a->x, a->ldx};
       gw.out[0] = {a->dwa, a->lddwa};
       gw.out[1] = {a->dwg, a->lddwg};
-      gw.partials = reinterpret_cast<float*>(base + ws.partials);
-      gw.partial_bytes = ws.partial_bytes;
       copies.add(gw);
     }
     FFN_TRY(copies.make(d, dev));
@@ -593,6 +607,32 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
     FFN_TRY(backward_products(k, a->dx ? &gx : nullptr, a->dwa ? &gw : nullptr, st));
     FFN_TRY(copies.release());
     return finish(d, st, sync);
+  });
+}
+
+j1_status j1_selftest_ffn_plan(int32_t product, int32_t act, int32_t M, int32_t N, int32_t K, int32_t num_sms, int32_t* plan) {
+  return guard("j1_selftest_ffn_plan", [&]() -> j1_status {
+    if (!plan || product < 0 || product > 5 || num_sms < 2) return bad("unknown product, fewer than two SMs, or NULL argument");
+    const int projections = product == 1 || product > 3 ? 2 : 1;
+    if (act < J1_ACT_NONE || act > J1_ACT_SILU) return bad("unknown activation");
+    FFN_TRY(check_sizes(M, N, K, projections == 2 ? kMaxGated : kMaxDim));
+    if (!M) return bad("no rows");
+    FfnDevice d;
+    d.num_sms = num_sms;
+    const Workspace ws = workspace_for(M, N, K, projections);
+    const int parts = parts_for(act, projections);
+    FfnGemm g;
+    if (product < 2) {
+      g = gemm_for(J1_DTYPE_BF16, FFN_NT, M, N, K, &d);
+      g.gated = product;
+    } else if (product == 2 || product == 4) {
+      g = dx_product(J1_DTYPE_BF16, M, N, K, projections, parts, ws, &d);
+    } else {
+      uint8_t any;  // not touched: a workspace is there
+      g = dw_product(J1_DTYPE_BF16, M, N, K, projections, parts, ws, &any, &d);
+    }
+    ffn_plan(g, plan);
+    return J1_OK;
   });
 }
 

@@ -53,6 +53,8 @@ struct FfnGemm {
 
 // The operands a and b must have rows on 16-byte boundaries (ffn_rows16).
 int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream);
+// How it would run (see j1_selftest_ffn_plan; host arithmetic only).
+void ffn_plan(const FfnGemm& g, int32_t* plan);
 // Workspace that a split contraction of these sizes may take (host arithmetic only).
 size_t ffn_partial_bytes(int M, int N, int K);
 // Device address of the operators' error word on the current device.

@@ -113,6 +113,13 @@ size_t ffn_partial_bytes(int M, int N, int K) {
   return static_cast<size_t>(tiles + kPairs) * kPieceBytes;
 }
 
+void ffn_plan(const FfnGemm& g, int32_t* plan) {
+  const int segs = g.lo ? 2 * g.segs : g.segs;
+  const Plan p = choose(g, static_cast<int>(ceil_div(g.K, 64)) * segs);
+  const int32_t v[6] = {p.cg, p.bn, p.split, p.stream_k ? p.sk_q : 0, p.sk_r, p.stream_k && p.group == 1};
+  std::copy(v, v + 6, plan);
+}
+
 int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   FfnTc p = {};
   const int nb = g.gated ? 2 : g.segs;

@@ -39,7 +39,7 @@ EXPORTS = [
     "j1_tokenizer_encode", "j1_tokenizer_encode_batch", "j1_text_encoder_load", "j1_text_encoder_destroy",
     "j1_text_encoder_clear_cache", "j1_text_encoder_options", "j1_text_encoder_tokenize", "j1_text_encoder_encode",
     "j1_text_encoder_request_tokens", "j1_text_encoder_encode_batch", "j1_engine_logits_text", "j1_json_dumps",
-    "j1_inject_fault", "j1_selftest_device_timeout",
+    "j1_inject_fault", "j1_selftest_device_timeout", "j1_selftest_ffn_plan",
     "j1_op_linear", "j1_op_linear_backward", "j1_op_linear_backward_workspace",
     "j1_op_gated", "j1_op_gated_backward", "j1_op_gated_backward_workspace",
 ]
@@ -274,6 +274,8 @@ def lib():
     L.j1_inject_fault.restype = None
     L.j1_selftest_device_timeout.argtypes = [C.c_int, C.c_int64]
     L.j1_selftest_device_timeout.restype = C.c_int
+    L.j1_selftest_ffn_plan.argtypes = [C.c_int32] * 6 + [C.POINTER(C.c_int32)]
+    L.j1_selftest_ffn_plan.restype = C.c_int
     for name, args in (("linear", J1LinearArgs), ("linear_backward", J1LinearGradArgs), ("gated", J1GatedArgs),
                        ("gated_backward", J1GatedGradArgs)):
         f = getattr(L, "j1_op_" + name)
@@ -903,6 +905,17 @@ def selftest_device_timeout(ordinal: int = 0, limit_cycles: int = 2_000_000) -> 
     """Bounded device wait on a barrier nothing arrives at; returns the status
     (DEVICE_TIMEOUT when the timeout was detected and reported)."""
     return int(lib().j1_selftest_device_timeout(int(ordinal), int(limit_cycles)))
+
+
+FFN_PRODUCTS = ("linear", "gated", "linear dx", "linear dw", "gated dx", "gated dw")
+
+
+def selftest_ffn_plan(product: str, M: int, N: int, K: int, act: int = 0, num_sms: int = 148):
+    """How a product (FFN_PRODUCTS) of the feed-forward operators runs: (CTAs per tile, accumulator columns, CTAs per
+    contraction, stream-K workers per group or 0, tiles per group, groups along columns). Host only."""
+    plan = (C.c_int32 * 6)()
+    check(lib().j1_selftest_ffn_plan(FFN_PRODUCTS.index(product), act, M, N, K, num_sms, plan))
+    return tuple(plan)
 
 
 def json_dumps(text: str) -> str:

@@ -219,3 +219,38 @@ def test_workspace_is_contiguous():
     """An expanded tensor counts far more elements than it has memory."""
     for op in ("linear_backward", "gated_backward"):
         _refused(op, "contiguous", workspace=torch.zeros(1, dtype=torch.uint8).expand(1 << 30))
+
+
+def _plan_kind(product, M, N, K, act):
+    ctas, columns, split, workers, group, across = j1.selftest_ffn_plan(product, M, N, K, act)
+    return product, ctas, columns, split, min(group, 3) if workers else 0, across
+
+
+def test_gpu_tests_take_every_kind_of_plan():
+    """Tile shape, cluster size, stream-K groups of one, two or more tiles and their direction: what products of sizes up
+    to 131072 x 8192 x 8192 run as on 148 SMs is also run by the GPU tests, so a change of the plans' model shows here."""
+    import random
+    import test_ffn_gpu as gpu
+    products = {"linear": ("linear",), "gated": ("gated",), "linear_backward": ("linear dx", "linear dw"),
+                "gated_backward": ("gated dx", "gated dw")}
+    run = [(op, size, act) for size in gpu.SIZES for op in products for _, act in gpu.TYPES]
+    run += [(op, size, gpu.TYPES[i % len(gpu.TYPES)][1]) for i, (op, size) in enumerate(gpu.PLANS)]
+    run += [(op, size, act) for op, size, _, act in gpu.MORE_PLANS]
+    tested = {_plan_kind(p, *size, gpu.ACTS[act]) for op, size, act in run for p in products[op]}
+    rng, found = random.Random(1), {}
+    for _ in range(60000):
+        size = tuple(int(2 ** rng.uniform(lo, hi)) for lo, hi in ((0, 17), (3, 13), (3, 13)))
+        p, act = rng.choice(j1.FFN_PRODUCTS), rng.choice((j1.ACT_NONE, j1.ACT_GELU))
+        found.setdefault(_plan_kind(p, *size, act), (size, act))
+    assert len(found) > 50
+    missing = {k: v for k, v in found.items() if k not in tested}
+    assert not missing, missing
+
+
+def test_plan_query_refusals():
+    L, plan = j1.lib(), (C.c_int32 * 6)()
+    for args in ((6, 0, 8, 8, 8, 148), (-1, 0, 8, 8, 8, 148), (0, 5, 8, 8, 8, 148), (0, 0, 0, 8, 8, 148), (0, 0, 8, 0, 8, 148),
+                 (0, 0, 8, 8, 8, 1)):
+        assert L.j1_selftest_ffn_plan(*args, plan) == j1.INVALID_ARG
+    assert L.j1_selftest_ffn_plan(0, 0, 8, 8, 8, 148, None) == j1.INVALID_ARG
+    assert L.j1_selftest_ffn_plan(1, 0, 1, 2 ** 29 + 1, 1, 148, plan) == j1.UNSUPPORTED

@@ -929,3 +929,24 @@ def test_far_side_of_activations(torch_cuda, dtype, act):
     steep = {"gelu": p.double().abs(), "silu": torch.ones_like(value), "gelu_tanh": 1.6 * (1 + 0.135 * p.double() ** 2)}[act]
     normal = slope.abs() > 2 * least
     close("dx", dx[normal], slope[normal, None].expand(-1, K), ((unit(dtype) + unit(dtype) ** 2) * slope.abs() + 2 * rel * terms + 2.0 ** -126 * (1 + p.double().abs() * steep))[normal, None])
+
+
+# ... and those that the list above does not reach: clusters of eight on wide tiles, and stream-K products whose groups are
+# single tiles, pairs or more of them, along the rows of tiles or along their columns.
+MORE_PLANS = [("gated_backward", (70, 8, 8), BF, "silu"), ("gated_backward", (10135, 8, 905), HF, "gelu"),
+              ("gated_backward", (14182, 206, 203), BF, "gelu"), ("gated_backward", (3511, 466, 1153), BF, "gelu"),
+              ("gated_backward", (9357, 1923, 157), HF, "silu"), ("gated_backward", (3796, 66, 4978), BF, "silu"),
+              ("gated_backward", (3375, 1234, 450), HF, "gelu"), ("gated_backward", (7425, 1223, 717), BF, "gelu"),
+              ("gated_backward", (3313, 196, 2555), BF, "gelu_tanh"), ("gated_backward", (13273, 615, 759), HF, "gelu"),
+              ("linear_backward", (9732, 9, 892), BF, "gelu"), ("linear_backward", (16058, 412, 202), HF, "silu"),
+              ("linear_backward", (7039, 401, 1953), BF, "gelu"), ("linear_backward", (3432, 230, 5080), BF, "gelu"),
+              ("linear_backward", (3986, 5250, 200), HF, "gelu"), ("linear_backward", (3740, 191, 5228), BF, "silu"),
+              ("linear_backward", (1, 631, 4838), BF, "gelu"), ("linear_backward", (1, 3723, 845), HF, "gelu"),
+              ("linear_backward", (28426, 469, 1793), BF, "none"), ("linear_backward", (47429, 1171, 764), BF, "none")]
+
+
+@pytest.mark.parametrize("i,op,size,dtype,act", [(i,) + p for i, p in enumerate(MORE_PLANS)],
+                         ids=["%s-%s" % (p[0], _id(p[1])) for p in MORE_PLANS])
+def test_more_plans(torch_cuda, i, op, size, dtype, act):
+    check = check_linear_backward if op == "linear_backward" else check_gated_backward
+    check(*size, dtype, act, seed=i)
