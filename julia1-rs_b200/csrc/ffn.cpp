@@ -67,13 +67,19 @@ j1_status device_state(FfnDevice** out, int* ordinal) {
   FfnDevice& s = g_dev[dev];
   if (!s.ready.load(std::memory_order_acquire)) {
     std::lock_guard<std::mutex> lock(g_dev_mutex);
-    cudaError_t rc = ffn_error_word(&s.err);
-    if (rc == cudaSuccess) rc = cudaDeviceGetAttribute(&s.num_sms, cudaDevAttrMultiProcessorCount, dev);
-    if (rc != cudaSuccess) {
-      cudaGetLastError();
-      return cuda_error(rc, "error word");
+    if (!s.ready.load(std::memory_order_relaxed)) {  // else another thread was first: its values are in use
+      int* err = nullptr;
+      int sms = 0;
+      cudaError_t rc = ffn_error_word(&err);
+      if (rc == cudaSuccess) rc = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+      if (rc != cudaSuccess) {
+        cudaGetLastError();
+        return cuda_error(rc, "error word");
+      }
+      s.err = err;
+      s.num_sms = sms;
+      s.ready.store(true, std::memory_order_release);
     }
-    s.ready.store(true, std::memory_order_release);
   }
   *out = &s;
   *ordinal = dev;

@@ -950,3 +950,39 @@ MORE_PLANS = [("gated_backward", (70, 8, 8), BF, "silu"), ("gated_backward", (10
 def test_more_plans(torch_cuda, i, op, size, dtype, act):
     check = check_linear_backward if op == "linear_backward" else check_gated_backward
     check(*size, dtype, act, seed=i)
+
+
+FIRST_CALLS = """
+import sys, threading
+sys.path.insert(0, %r)
+import torch
+import julia1 as j1
+x, w = (torch.ones(n, 64, device="cuda", dtype=torch.bfloat16) for n in (40, 24))
+outs = [torch.zeros(40, 24, device="cuda", dtype=torch.bfloat16) for _ in range(12)]
+torch.cuda.synchronize()
+gate, errors = threading.Barrier(len(outs)), []
+
+def call(out):
+    try:
+        gate.wait()
+        j1.op_linear(x, w, out)
+    except Exception as e:
+        errors.append(e)
+
+threads = [threading.Thread(target=call, args=(o,)) for o in outs]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert not errors, errors
+assert all(bool((o == 64).all()) for o in outs)
+"""
+
+
+def test_first_calls_of_many_threads(torch_cuda):
+    """The first calls of a process on a device, from several threads at once (its error word and size are looked up by one)."""
+    import os
+    import subprocess
+    import sys
+    path = os.path.dirname(os.path.dirname(os.path.abspath(j1.__file__)))
+    for _ in range(2):
+        r = subprocess.run([sys.executable, "-c", FIRST_CALLS % path], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0, r.stdout + r.stderr
