@@ -465,7 +465,7 @@ J1_API j1_status j1_op_attention_noalloc(const void* qkv, int64_t t, int32_t hid
  * equal bits: no result depends on the order in which blocks finish.
  *
  * With sync = 0 the calls only enqueue work and may be captured into a CUDA graph; the first
- * call of each kind on a device loads its kernels and should come before any capture.
+ * of them on a device, whichever it is (one with M = 0 too), loads every kernel and should come before any capture.
  * Device-side timeouts of sync = 0 calls are reported by the next of these calls made with
  * sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Operands whose rows all start on 16-byte
  * boundaries are read in place and nothing is allocated; other operands of a product are copied

@@ -38,10 +38,10 @@ struct FfnDevice {
   std::atomic<bool> ready{false};
   int* err = nullptr;
   int num_sms = 0;
-  std::atomic<cudaMemPool_t> pool{nullptr};
+  cudaMemPool_t pool = nullptr;  // for operand copies
 };
 FfnDevice g_dev[kMaxDevices];
-std::mutex g_dev_mutex;  // first use of a device and of its pool; a failure leaves them for the next call
+std::mutex g_dev_mutex;  // first use of a device; a failure leaves it for the next call
 
 // The first CUDA call of a host thread may be one of these operators, and tensor maps can only be made with
 // a context that is current: the runtime binds the device's when it is asked to.
@@ -58,6 +58,22 @@ cudaError_t bind_context(int dev) {
   return cudaSetDevice(dev);
 }
 
+// The device's pool, which keeps what it has taken (as a model's workspace does).
+cudaError_t make_pool(int dev, cudaMemPool_t* pool) {
+  cudaMemPoolProps props = {};
+  props.allocType = cudaMemAllocationTypePinned;
+  props.location.type = cudaMemLocationTypeDevice;
+  props.location.id = dev;
+  cudaError_t e = cudaMemPoolCreate(pool, &props);
+  if (e != cudaSuccess) return e;
+  uint64_t keep = UINT64_MAX;
+  e = cudaMemPoolSetAttribute(*pool, cudaMemPoolAttrReleaseThreshold, &keep);
+  if (e != cudaSuccess) cudaMemPoolDestroy(*pool);
+  return e;
+}
+
+// The first use of a device does all that a stream capture does not allow, or that would wait for the device:
+// kernels are loaded, whichever the calls will take, and the pool is made.
 j1_status device_state(FfnDevice** out, int* ordinal) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -72,10 +88,16 @@ j1_status device_state(FfnDevice** out, int* ordinal) {
       int sms = 0;
       cudaError_t rc = ffn_error_word(&err);
       if (rc == cudaSuccess) rc = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+      if (rc == cudaSuccess) rc = load_ffn_rows();
+      if (rc == cudaSuccess) rc = load_ffn_tc_bf16();
+      if (rc == cudaSuccess) rc = load_ffn_tc_fp16();
+      cudaMemPool_t pool = nullptr;
+      if (rc == cudaSuccess) rc = make_pool(dev, &pool);
       if (rc != cudaSuccess) {
         cudaGetLastError();
-        return cuda_error(rc, "error word");
+        return cuda_error(rc, "first use of the device");
       }
+      s.pool = pool;
       s.err = err;
       s.num_sms = sms;
       s.ready.store(true, std::memory_order_release);
@@ -194,32 +216,6 @@ FfnGemm gemm_for(int dtype, int layout, int M, int N, int K, const FfnDevice* d)
   return g;
 }
 
-// The device's pool, which keeps what it has taken (as a model's workspace does).
-cudaError_t device_pool(FfnDevice* d, int dev, cudaMemPool_t* out) {
-  cudaMemPool_t pool = d->pool.load(std::memory_order_acquire);
-  if (!pool) {
-    std::lock_guard<std::mutex> lock(g_dev_mutex);
-    pool = d->pool.load(std::memory_order_relaxed);
-    if (!pool) {
-      cudaMemPoolProps props = {};
-      props.allocType = cudaMemAllocationTypePinned;
-      props.location.type = cudaMemLocationTypeDevice;
-      props.location.id = dev;
-      cudaError_t e = cudaMemPoolCreate(&pool, &props);
-      if (e != cudaSuccess) return e;
-      uint64_t keep = UINT64_MAX;
-      e = cudaMemPoolSetAttribute(pool, cudaMemPoolAttrReleaseThreshold, &keep);
-      if (e != cudaSuccess) {
-        cudaMemPoolDestroy(pool);
-        return e;
-      }
-      d->pool.store(pool, std::memory_order_release);
-    }
-  }
-  *out = pool;
-  return cudaSuccess;
-}
-
 // Copies of a call's operands. TMA reads rows on 16-byte boundaries only; the products' other operands
 // are copied first, all in one launch. (Reading them in the product instead, loader warps shifting
 // aligned 16-byte pieces into place, kept the tensor cores waiting: 65536 x 771 x 1155 took 527-606 us,
@@ -255,12 +251,10 @@ class Copies {
     }
   }
   // Makes the copies and puts them in their operands' places.
-  j1_status make(FfnDevice* d, int dev) {
+  j1_status make(FfnDevice* d) {
     if (!c_.n) return J1_OK;
     if (take_fault(J1_FAULT_ALLOC)) return set_error(J1_ERR_OOM, "operand copies: device allocation failed (injected)");
-    cudaMemPool_t pool;
-    cudaError_t e = device_pool(d, dev, &pool);
-    if (e == cudaSuccess) e = cudaMallocFromPoolAsync(&mem_, bytes_, pool, st_);
+    const cudaError_t e = cudaMallocFromPoolAsync(&mem_, bytes_, d->pool, st_);
     if (e != cudaSuccess) {
       cudaGetLastError();
       mem_ = nullptr;
@@ -406,7 +400,7 @@ j1_status j1_op_linear(const j1_linear_args* a, void* stream, int sync) {
       g.pre[0] = {a->pre, a->ldp};
       Copies copies(st);
       copies.add(g);
-      FFN_TRY(copies.make(d, dev));
+      FFN_TRY(copies.make(d));
       FFN_LAUNCH(launch_ffn_gemm(g, st), "linear launch");
       FFN_TRY(copies.release());
     }
@@ -446,7 +440,7 @@ j1_status j1_op_gated(const j1_gated_args* a, void* stream, int sync) {
       g.pre[1] = {a->pre_g, a->ldpg};
       Copies copies(st);
       copies.add(g);
-      FFN_TRY(copies.make(d, dev));
+      FFN_TRY(copies.make(d));
       FFN_LAUNCH(launch_ffn_gemm(g, st), "gated launch");
       FFN_TRY(copies.release());
     }
@@ -515,7 +509,7 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
       gw.out[0] = {a->dw, a->lddw};
       copies.add(gw);
     }
-    FFN_TRY(copies.make(d, dev));
+    FFN_TRY(copies.make(d));
     if (copy || a->dbias) {
       k.fp16 = a->dtype == J1_DTYPE_FP16;
       k.act = a->act;
@@ -608,7 +602,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
       gw.out[1] = {a->dwg, a->lddwg};
       copies.add(gw);
     }
-    FFN_TRY(copies.make(d, dev));
+    FFN_TRY(copies.make(d));
     FFN_LAUNCH(launch_ffn_grad(k, st), "gated gradient launch");
     FFN_TRY(backward_products(k, a->dx ? &gx : nullptr, a->dwa ? &gw : nullptr, st));
     FFN_TRY(copies.release());

@@ -57,6 +57,10 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream);
 void ffn_plan(const FfnGemm& g, int32_t* plan);
 // Workspace that a split contraction of these sizes may take (host arithmetic only).
 size_t ffn_partial_bytes(int M, int N, int K);
+// Load the kernels on the current device (a lazily loaded one could not be launched first in a stream capture).
+cudaError_t load_ffn_rows();
+cudaError_t load_ffn_tc_bf16();
+cudaError_t load_ffn_tc_fp16();
 // Device address of the operators' error word on the current device.
 cudaError_t ffn_error_word(int** p);
 

@@ -165,6 +165,10 @@ __global__ void __launch_bounds__(GC, 4) max_kernel(const FfnGrad g, int col_blo
   }
 }
 
+// Gradients that are scaled before they are stored.
+template <typename T, bool GATED, int ACT>
+constexpr bool kScaled = std::is_same<T, __half>::value && (GATED || (ACT != J1_ACT_NONE && ACT != J1_ACT_RELU));
+
 template <typename T, bool GATED, int ACT, bool VEC>
 __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_rows, int maxima) {
   __shared__ float red[GR][GC];
@@ -180,7 +184,7 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
   // registers 141, with nothing asked for ahead 227). Otherwise the next RI rows' are in registers.
   constexpr int OPS = GATED ? 3 : ACT != J1_ACT_NONE ? 2 : 1, DEPTH = GATED ? 3 : ACT != J1_ACT_NONE ? 4 : 8;
   constexpr int RI = GATED || VEC ? 1 : 2;
-  constexpr bool SCALED = std::is_same<T, __half>::value && (GATED || (ACT != J1_ACT_NONE && ACT != J1_ACT_RELU));
+  constexpr bool SCALED = kScaled<T, GATED, ACT>;
   __shared__ uint4 ring[VEC ? DEPTH * OPS * GC : 1];
   const uint32_t own = smem_u32(ring) + threadIdx.x * 16;
   uint32_t slot = 0;
@@ -394,9 +398,30 @@ __global__ void __launch_bounds__(256) copies_kernel(const FfnCopies c) {
 }
 
 template <typename T, bool GATED, int ACT>
+cudaError_t load_act() {
+  cudaFuncAttributes a;
+  cudaError_t e = cudaFuncGetAttributes(&a, grad_kernel<T, GATED, ACT, true>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, grad_kernel<T, GATED, ACT, false>);
+  if constexpr (kScaled<T, GATED, ACT>) {
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, max_kernel<GATED, ACT, true>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, max_kernel<GATED, ACT, false>);
+  }
+  return e;
+}
+template <typename T, bool GATED>
+cudaError_t load_acts() {
+  cudaError_t e = load_act<T, GATED, J1_ACT_NONE>();
+  if (e == cudaSuccess) e = load_act<T, GATED, J1_ACT_RELU>();
+  if (e == cudaSuccess) e = load_act<T, GATED, J1_ACT_GELU>();
+  if (e == cudaSuccess) e = load_act<T, GATED, J1_ACT_GELU_TANH>();
+  if (e == cudaSuccess) e = load_act<T, GATED, J1_ACT_SILU>();
+  return e;
+}
+
+template <typename T, bool GATED, int ACT>
 cudaError_t launch_grad(const FfnGrad& g, bool vec, dim3 grid, int slab_rows, cudaStream_t st) {
   int maxima = 0;
-  if constexpr (std::is_same<T, __half>::value && (GATED || (ACT != J1_ACT_NONE && ACT != J1_ACT_RELU))) {
+  if constexpr (kScaled<T, GATED, ACT>) {
     if (g.scale) {
       const long long tiles = (static_cast<long long>(g.M) + 2 * GR - 1) / (2 * GR) * grid.x;
       maxima = static_cast<int>(tiles < kFfnMaxBlocks ? tiles : kFfnMaxBlocks);
@@ -420,6 +445,17 @@ cudaError_t launch_grad(const FfnGrad& g, bool vec, dim3 grid, int slab_rows, cu
 }
 
 }  // namespace
+
+cudaError_t load_ffn_rows() {
+  cudaFuncAttributes a;
+  cudaError_t e = cudaFuncGetAttributes(&a, copies_kernel);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&a, slab_sum_kernel);
+  if (e == cudaSuccess) e = load_acts<__half, false>();
+  if (e == cudaSuccess) e = load_acts<__half, true>();
+  if (e == cudaSuccess) e = load_acts<__nv_bfloat16, false>();
+  if (e == cudaSuccess) e = load_acts<__nv_bfloat16, true>();
+  return e;
+}
 
 int launch_ffn_copies(const FfnCopies& c, cudaStream_t st) {
   long long rows = 1, cols = 1;

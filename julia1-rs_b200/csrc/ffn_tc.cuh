@@ -1005,10 +1005,7 @@ __global__ void __launch_bounds__(256) pieces_kernel(const __grid_constant__ Ffn
 template <typename T, int CG, int BN, int LAYOUT, bool GATED>
 int launch_one(FfnTc& p, cudaStream_t stream) {
   constexpr int EW = epi_warps(CG, BN, LAYOUT, GATED);
-  static std::atomic<unsigned long long> configured{0};
   auto kern = tc_kernel<T, CG, BN, LAYOUT, GATED>;
-  cudaError_t e = set_smem_once(kern, SMEM_MAX, configured);
-  if (e != cudaSuccess) return static_cast<int>(e);
   // no more stages than blocks a CTA will see: a small CTA can share the SM with the kernel before.
   // A cluster's CTAs leave their accumulators (BM x BN floats) over the stages.
   p.boxes = 1 + (p.pre[0].p ? (GATED ? 2 : 1) : 0);
@@ -1036,7 +1033,7 @@ int launch_one(FfnTc& p, cudaStream_t stream) {
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = CG == 2 || p.split > 1 ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
   if (e != cudaSuccess || !p.stream_k) return static_cast<int>(e);
   return static_cast<int>(launch_kernel(pieces_kernel<T>, dim3(static_cast<unsigned>(p.tiles) * (256 / 32) * 8), dim3(256), 0,
                                         stream, p));
@@ -1055,6 +1052,32 @@ int launch_cfg(int cfg, FfnTc& p, cudaStream_t stream) {
       break;
   }
   return static_cast<int>(cudaErrorInvalidValue);
+}
+
+// Loads the kernels of a layout on the current device, with their shared memory.
+template <typename T, int CG, int BN, int LAYOUT, bool GATED>
+cudaError_t load_one() {
+  return cudaFuncSetAttribute(tc_kernel<T, CG, BN, LAYOUT, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
+}
+template <typename T, int LAYOUT, bool GATED>
+cudaError_t load_cfg() {
+  cudaError_t e = load_one<T, 2, 256, LAYOUT, GATED>();
+  if (e == cudaSuccess) e = load_one<T, 1, 128, LAYOUT, GATED>();
+  if constexpr (LAYOUT == FFN_NT && !GATED)
+    if (e == cudaSuccess) e = load_one<T, 2, 192, LAYOUT, GATED>();
+  if constexpr (!GATED)
+    if (e == cudaSuccess) e = load_one<T, 1, 64, LAYOUT, GATED>();
+  return e;
+}
+template <typename T>
+cudaError_t load_tc() {
+  cudaFuncAttributes a;
+  cudaError_t e = cudaFuncGetAttributes(&a, pieces_kernel<T>);
+  if (e == cudaSuccess) e = load_cfg<T, FFN_NT, true>();
+  if (e == cudaSuccess) e = load_cfg<T, FFN_NT, false>();
+  if (e == cudaSuccess) e = load_cfg<T, FFN_NN, false>();
+  if (e == cudaSuccess) e = load_cfg<T, FFN_TN, false>();
+  return e;
 }
 
 template <typename T>

@@ -986,3 +986,55 @@ def test_first_calls_of_many_threads(torch_cuda):
     for _ in range(2):
         r = subprocess.run([sys.executable, "-c", FIRST_CALLS % path], capture_output=True, text=True, timeout=300)
         assert r.returncode == 0, r.stdout + r.stderr
+
+
+CAPTURED_FIRST = """
+import sys
+sys.path.insert(0, %r)
+import torch
+import julia1 as j1
+none, wide = torch.empty(0, 8, device="cuda", dtype=torch.bfloat16), torch.empty(8, 8, device="cuda", dtype=torch.bfloat16)
+j1.op_linear(none, wide, none)  # the first call, without rows
+torch.manual_seed(1)
+steps = []
+for dtype in (torch.bfloat16, torch.float16):
+    for M, N, K in ((1, 64, 40), (300, 72, 136), (77, 65, 51), (2000, 1100, 712), (700, 3392, 392), (7356, 160, 512)):
+        e = lambda *s: torch.randn(s, device="cuda").to(dtype)
+        t = dict(x=e(M, K), wa=e(N, K), wg=e(N, K), pa=e(M, N), pg=e(M, N), out=e(M, N), y=e(M, N), dout=e(M, N), dx=e(M, K),
+                 dwa=e(N, K), dwg=e(N, K), dl=e(M, K), dwl=e(N, K), db=torch.empty(N, device="cuda"), dba=torch.empty(N, device="cuda"),
+                 ws=torch.empty(j1.op_gated_backward_workspace(M, N, K), device="cuda", dtype=torch.uint8))
+        for act in range(5):
+            steps.append((t, act, {k: torch.empty_like(t[k]) for k in ("out", "y", "dx", "dwa", "dwg", "dl", "dwl", "db", "dba")}))
+
+def step(t, act, stream):
+    o = dict(act=act, stream=stream, sync=False)
+    j1.op_gated(t["x"], t["wa"], t["wg"], t["out"], **o)
+    j1.op_linear(t["x"], t["wa"], t["y"], bias=t["db"].fill_(0.5), residual=t["dout"], **o)
+    j1.op_gated_backward(t["dout"], t["x"], t["wa"], t["wg"], t["pa"], t["pg"], dx=t["dx"], dwa=t["dwa"], dwg=t["dwg"], dba=t["dba"],
+                         workspace=t["ws"], **o)
+    j1.op_linear_backward(t["dout"], t["x"], t["wa"], pre=t["pa"], dx=t["dl"], dw=t["dwl"], dbias=t["db"], workspace=t["ws"], **o)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    for t, act, got in steps:
+        step(t, act, torch.cuda.current_stream().cuda_stream)
+        for k in got:
+            got[k].copy_(t[k])
+graph.replay()
+torch.cuda.synchronize()
+for t, act, got in steps:
+    step(t, act, None)
+    torch.cuda.synchronize()
+    for k in got:
+        assert torch.equal(got[k], t[k]), (k, act, t["x"].shape)
+"""
+
+
+def test_captured_after_one_call(torch_cuda):
+    """One call of any kind on a device, without rows even, and every kernel of the operators may be captured."""
+    import os
+    import subprocess
+    import sys
+    path = os.path.dirname(os.path.dirname(os.path.abspath(j1.__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST % path], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
