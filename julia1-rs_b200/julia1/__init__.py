@@ -1217,6 +1217,16 @@ def _ffn_sizes(x, w):
     return M, N, K
 
 
+def _ffn_workspace_size(query, *sizes):
+    if max(sizes) > 1 << 30:  # before they become C ints
+        raise J1Error(UNSUPPORTED, "sizes above 2^30")
+    if min(sizes) < 0:
+        raise J1Error(INVALID_ARG, "M must be >= 0, N and K positive")
+    n = C.c_size_t()
+    check(query(*sizes, C.byref(n)))
+    return n.value
+
+
 def _ffn_workspace(t):
     if t is None:
         return 0, 0
@@ -1251,9 +1261,7 @@ def op_linear(x, w, out, bias=None, act=ACT_NONE, residual=None, pre=None, strea
 
 def op_linear_backward_workspace(M, N, K):
     """Bytes of workspace op_linear_backward needs (any dtype, activation and set of gradients)."""
-    n = C.c_size_t()
-    check(lib().j1_op_linear_backward_workspace(M, N, K, C.byref(n)))
-    return n.value
+    return _ffn_workspace_size(lib().j1_op_linear_backward_workspace, M, N, K)
 
 
 def op_linear_backward(dout, x, w, pre=None, act=ACT_NONE, dx=None, dw=None, dbias=None, workspace=None, stream=None,
@@ -1285,9 +1293,7 @@ def op_gated(x, wa, wg, out, ba=None, bg=None, act=ACT_GELU, pre_a=None, pre_g=N
 
 def op_gated_backward_workspace(M, N, K):
     """Bytes of workspace op_gated_backward needs (any dtype, activation and set of gradients)."""
-    n = C.c_size_t()
-    check(lib().j1_op_gated_backward_workspace(M, N, K, C.byref(n)))
-    return n.value
+    return _ffn_workspace_size(lib().j1_op_gated_backward_workspace, M, N, K)
 
 
 def op_gated_backward(dout, x, wa, wg, pre_a, pre_g, act=ACT_GELU, dx=None, dwa=None, dwg=None, dba=None, dbg=None,

@@ -254,3 +254,15 @@ def test_plan_query_refusals():
         assert L.j1_selftest_ffn_plan(*args, plan) == j1.INVALID_ARG
     assert L.j1_selftest_ffn_plan(0, 0, 8, 8, 8, 148, None) == j1.INVALID_ARG
     assert L.j1_selftest_ffn_plan(1, 0, 1, 2 ** 29 + 1, 1, 148, plan) == j1.UNSUPPORTED
+
+
+@pytest.mark.parametrize("size", [j1.op_linear_backward_workspace, j1.op_gated_backward_workspace])
+def test_workspace_sizes_beyond_32_bits(size):
+    """Sizes that a C int does not hold are refused, not cut to its bits."""
+    for at in range(3):
+        for n, status in ((2 ** 32 + 64, j1.UNSUPPORTED), (2 ** 31, j1.UNSUPPORTED), (-2 ** 32 + 64, j1.INVALID_ARG)):
+            args = [64, 64, 64]
+            args[at] = n
+            with pytest.raises(j1.J1Error) as e:
+                size(*args)
+            assert e.value.status == status, args
