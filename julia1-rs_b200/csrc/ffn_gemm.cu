@@ -124,7 +124,7 @@ int launch_ffn_gemm(const FfnGemm& g, cudaStream_t stream) {
   FfnTc p = {};
   const int nb = g.gated ? 2 : g.segs;
   for (int i = 0; i < 2; ++i) p.out[i] = g.out[i], p.pre[i] = g.pre[i], p.bias[i] = g.bias[i];
-  p.M = g.M, p.N = g.N, p.K = g.K;
+  p.M = g.M, p.N = g.N;
   p.segs = g.lo ? 2 * g.segs : g.segs;
   p.b_and = g.segs - 1;
   p.kb_seg = static_cast<int>(ceil_div(g.K, 64));

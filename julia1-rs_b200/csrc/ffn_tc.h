@@ -8,9 +8,9 @@ namespace j1rt {
 struct FfnTc {
   CUtensorMap ma[4], mb[2];
   CUtensorMap mo, mp[2];    // out and pre in boxes of 32 x 32, where tma_out
-  FfnMat a[2], b[2], out[2], pre[2], residual;
+  FfnMat out[2], pre[2], residual;
   const float* bias[2];
-  int M, N, K;              // output rows, columns, contraction per segment
+  int M, N;                 // output rows, columns
   int segs, kb_seg, kb;     // segments, 64-blocks per segment, 64-blocks in all
   int b_and;                // segment s multiplies ma[s] with mb[s & b_and]
   int act;
