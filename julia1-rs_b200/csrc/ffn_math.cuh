@@ -74,41 +74,39 @@ __device__ __forceinline__ float recip_approx(float x) {
 // (an exponential may overflow on the far side: 1 / inf = 0):
 //   silu       s = 1 / (1 + 2^(-p log2 e))
 //   gelu_tanh  s = 0.5 (1 + tanh z) = 1 / (1 + 2^(-2 z log2 e)),  z = sqrt(2/pi) (p + 0.044715 p^3)
-//   gelu       s = Phi(p) = 1 - Phi(-p);  Phi(-q) = e^(-q^2 / 2) u Q(u) for q >= 0, u = 1 / (1 + 0.3 q): the
-//              factor before u Q(u) has the tail's fall, and what is left is smooth in u on (0, 1]. Q, of degree 7, is
-//              fitted here to the smallest maximal error relative to Phi(-q), 1.7e-7 up to q = 14 (a linear
+//   gelu       s = Phi(p) = 1 - Phi(-p);  Phi(-q) = e^(-q^2 / 2) u Q(u) for q >= 0, u = 1 / (3.3125 + q): the
+//              factor before u Q(u) has the tail's fall, and what is left is smooth in u. Q, of degree 7, is
+//              fitted here to the smallest maximal error relative to Phi(-q), 1.3e-7 up to q = 14 (a linear
 //              program over 1500 points, coefficients rounded one after the other); 5e-7 in FP32 arithmetic up to
 //              q = 2, beyond it what the rounding of q^2 / 2 in the exponent makes, 8e-6 at q = 13.
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kTanhA = -2.302208198144325f;                // -2 sqrt(2 / pi) log2(e)
 constexpr float kTanhB = -2.302208198144325f * 0.044715f;
 __host__ __device__ constexpr float gelu_coef(int k) {  // of u^k in Q
-  return k == 0   ? 0.11962930113077164f
-         : k == 1 ? 0.12075395882129669f
-         : k == 2 ? 0.09991350769996643f
-         : k == 3 ? 0.1285615861415863f
-         : k == 4 ? -0.0536835677921772f
-         : k == 5 ? 0.20635342597961426f
-         : k == 6 ? -0.1572030633687973f
-                  : 0.03567477688193321f;
+  return k == 0   ? 0.3987848460674286f
+         : k == 1 ? 1.3320972919464111f
+         : k == 2 ? 3.6793785095214844f
+         : k == 3 ? 15.142889976501465f
+         : k == 4 ? -19.1063175201416f
+         : k == 5 ? 262.7478332519531f
+         : k == 6 ? -682.2756958007812f
+                  : 523.8531494140625f;
 }
 
 // Phi of a pair of values, and e^(-p^2 / 2).
 __device__ __forceinline__ uint64_t normal_cdf(uint64_t p, uint64_t& density) {
   auto c2 = [](float c) { return f2pack(c, c); };
-  float a, b, d, e;
+  float p0, p1, a, b, d, e;
+  f2unpack(p, p0, p1);
   f2unpack(mul2(mul2(p, p), c2(-0.5f * kLog2e)), a, b);
   density = f2pack(exp2_approx(a), exp2_approx(b));
-  f2unpack(fma2(p & 0x7fffffff7fffffffull, c2(0.3f), c2(1.f)), a, b);
-  const uint64_t u = f2pack(recip_approx(a), recip_approx(b));
+  const uint64_t u = f2pack(recip_approx(fabsf(p0) + 3.3125f), recip_approx(fabsf(p1) + 3.3125f));
   uint64_t x = c2(gelu_coef(7));
 #pragma unroll
   for (int k = 6; k >= 0; --k) x = fma2(x, u, c2(gelu_coef(k)));
   x = mul2(mul2(x, u), density);
   f2unpack(x, a, b);
   f2unpack(fma2(x, c2(-1.f), c2(1.f)), d, e);
-  float p0, p1;
-  f2unpack(p, p0, p1);
   return f2pack(p0 < 0.f ? a : d, p1 < 0.f ? b : e);
 }
 
