@@ -464,9 +464,9 @@ J1_API j1_status j1_op_attention_noalloc(const void* qkv, int64_t t, int32_t hid
  * width and its stride are not written, and what they hold does not matter. Equal inputs give
  * equal bits: no result depends on the order in which blocks finish.
  *
- * With sync = 0 the calls only enqueue work and may be captured into a CUDA graph; the first
- * of them on a device, whichever it is (one with M = 0 too), loads every kernel and should come before any capture.
- * Device-side timeouts of sync = 0 calls are reported by the next of these calls made with
+ * With sync = 0 the calls only enqueue work and may be captured into a CUDA graph; the first of them
+ * on a device, whichever it is (one with M = 0 will do), loads every kernel and must come before any
+ * capture. Device-side timeouts of sync = 0 calls are reported by the next of these calls made with
  * sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Operands whose rows all start on 16-byte
  * boundaries are read in place and nothing is allocated; other operands of a product are copied
  * first, to stream-ordered memory of a pool of the library, which keeps the most it ever needed
@@ -502,10 +502,11 @@ J1_API j1_status j1_op_linear(const j1_linear_args* args, void* stream, int sync
 /* Gradients of j1_op_linear: dp = dout * act'(pre); dx = dp w; dw = dp^T x; dbias = sum of dp
  * over rows. dx, dw and dbias are written, not added to; each may be NULL (not wanted), not
  * all three. x is read for dw only, w for dx only, pre unless act is J1_ACT_NONE (where dp =
- * dout); what is not read may be NULL. For the two products dp is kept in two
- * parts of the dtype, both of its sign (an infinite x or w gives the infinity that dp itself would), the
- * second what the first leaves; in FP16 both are scaled by a power of two of the call, taken out of the products' sums, so that only what is below 2^-38 of the largest finite dp
- * is lost. dbias sums the unrounded values. The residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
+ * dout); what is not read may be NULL. For the two products dp is kept in two parts of the dtype
+ * (16 significant bits of BF16, 22 of FP16), both of its sign: an infinite x or w gives the infinity
+ * that dp itself would. In FP16 both parts are scaled by a power of two of the call, which the
+ * products' sums lose again before they are rounded; what is below 2^-38 of the largest finite dp is
+ * lost. dbias sums the unrounded values. The residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
  * workspace: at least j1_op_linear_backward_workspace bytes, 256-byte aligned; its contents
  * need not survive between calls, and calls that may overlap on the GPU need one each. */
 typedef struct j1_linear_grad_args {

@@ -31,8 +31,9 @@ struct Plan {
 // and what a cluster's exchange costs: its accumulators' rows shared out (more CTAs, fewer for each) and
 // its traffic (more pieces to read). The constants are fitted to the times of 124 products (all operand
 // orders and gated; 1 to 131072 rows, contractions of 64 to 131072, weights from HBM for few rows) under
-// every plan: the plan chosen costs 0.9% more than the best one on average, 21% at most; an earlier model
-// whose exchange cost the same for all rows 10%. Some of them (us), best plan first:
+// every plan: among them the plan chosen costs 0.9% more than the best one on average, 21% at most (an earlier model
+// whose exchange cost the same for all rows 10%); among 124 others, most of random sizes, 4.7% and 62%, the most where a
+// long M meets K below 64, whose epilogues it leaves out. Some of the first (us), best plan first:
 //   768 x 768 x 1024 TN    CG 1 x 64 5.3, x 128 6.7, x 64 in clusters of two 7.1, CG 2 x 256 9.9
 //   1 x 2048 x 8192        CG 1 x 128 in fours 10.6, x 64 in fours 11.7, in twos 14, in eights 16, one CTA 21-23
 //   16 x 8192 x 8192       CG 1 x 128 in twos 25.0, one CTA 28.7

@@ -3,11 +3,12 @@
 //
 //   linear: dp = dout act'(p)                        gated: da = dout g act'(a), dg = dout act(a)
 //
-// Bound by memory: 2 bytes per element and operand. A block owns 256 columns and a slab of
-// rows; 32 threads cover the columns, 8 rows are worked on at once, each thread keeps its
-// columns' sums in registers over the slab. 65536 x 1152 gated GELU: 116 us, 6.5 TB/s, the
-// measured copy rate. Slab sums go to the workspace in FP32 and a second
-// kernel adds them in slab order, so a sum's bits do not depend on which block ran first.
+// Bound by memory: 2 bytes per element of every operand and of both parts of every gradient. A block
+// owns 256 columns and a slab of rows; 32 threads cover the columns, 8 rows are worked on at once, each
+// thread keeps its columns' sums in registers over the slab. 65536 x 1152 gated GELU: 193 us, 5.5 TB/s (0.83
+// of the measured copy rate: the slopes and the cutting into parts take issue slots). Slab sums go to the
+// workspace in FP32 and a second kernel adds them in slab order, so a sum's bits do not depend on which
+// block ran first.
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -110,8 +111,8 @@ __device__ __forceinline__ void gradients(uint64_t& d, uint64_t p, uint64_t& q) 
 // The largest finite magnitude of the gradients at the pre-activations, per block. FP16 has 2^-24 to 2^16, where
 // dout, the activation's slope and the gate may each be small or large without the products' results being so: the
 // gradients are scaled by a power of two of the call before they are rounded. It takes a pass of its own over their
-// operands. Tiles of 16 rows x 256 columns, two rows per thread in flight: 65536 x 1152 gated GELU 100 us (4.5 TB/s,
-// the slopes' exponentials between the loads), 2048 x 768 linear 4.5 us; with tiles of 64 rows, four in flight, too few blocks
+// operands. Tiles of 16 rows x 256 columns, two rows per thread in flight: 65536 x 1152 gated GELU 107 us (4.2 TB/s,
+// the slopes' arithmetic between the loads), 2048 x 768 linear 4.5 us; with tiles of 64 rows, four in flight, too few blocks
 // had work at small sizes (the call on 2048 rows 12 us longer).
 template <bool GATED, int ACT, bool VEC>
 __global__ void __launch_bounds__(GC, 4) max_kernel(const FfnGrad g, int col_blocks) {
@@ -180,8 +181,8 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
   uint64_t s0[4] = {}, s1[4] = {};
   grid_dep_wait();
   // VEC: the next DEPTH rows' pieces are on their way to shared memory while a row is worked on, each
-  // thread reading back what it asked for itself (65536 x 1152 gated GELU 116 us; with the next row in
-  // registers 141, with nothing asked for ahead 227). Otherwise the next RI rows' are in registers.
+  // thread reading back what it asked for itself (65536 x 1152 gated GELU, gradients in one part: 116 us; with the
+  // next row in registers 141, with nothing asked for ahead 227). Otherwise the next RI rows' are in registers.
   constexpr int OPS = GATED ? 3 : ACT != J1_ACT_NONE ? 2 : 1, DEPTH = GATED ? 3 : ACT != J1_ACT_NONE ? 4 : 8;
   constexpr int RI = GATED || VEC ? 1 : 2;
   constexpr bool SCALED = kScaled<T, GATED, ACT>;
@@ -469,8 +470,8 @@ int launch_ffn_copies(const FfnCopies& c, cudaStream_t st) {
   return static_cast<int>(launch_kernel(copies_kernel, grid, dim3(256), 0, st, c));
 }
 
-// About eight blocks per SM over both dimensions, at least 16 rows each (2048 x 768 x 1152 linear backward
-// 17.9 us, with 32 rows 18.9, with 8 18.6: more sums to add), at most 512 slabs; up to 64 rows in one
+// About eight blocks per SM over both dimensions, at least 16 rows each (2048 x 768 x 1152 linear backward with
+// gradients in one part 17.9 us, with 32 rows 18.9, with 8 18.6: more sums to add), at most 512 slabs; up to 64 rows in one
 // slab, which saves the second kernel (2 us) for two more turns of the first (1 us).
 int ffn_grad_slabs(int M, int N) {
   const long long cols = (static_cast<long long>(N) + GC - 1) / GC;

@@ -1,6 +1,6 @@
 // Matrix products of the feed-forward operators on tcgen05, with their epilogues.
 //
-//   out[M, N] = act(A . B + bias) (+ residual), A . B over one or two operand pairs
+//   out[M, N] = act(A . B + bias) (+ residual), A . B over one to four operand pairs
 //   out[M, N] = act(A B0^T + bias0) * (A B1^T + bias1)                            (gated)
 //
 // One kernel for every operand order: an operand whose contraction index is contiguous in
@@ -29,7 +29,7 @@
 // products. The epilogue works on 32-column chunks, one thread per row: FP32 accumulators from
 // TMEM, bias, activation, residual, one rounding, then through a swizzled 32 x 32 box in shared
 // memory to the result. Pairs' forward boxes are stored by TMA where rows are whole 16-byte units
-// (131072 x 1152 x 768 with GELU and saved pre-activations 231 us, 249 with 16-byte stores by the warps);
+// (131072 x 1152 x 768 with GELU and saved pre-activations in 7% less time than with 16-byte stores by the warps);
 // other boxes by the warps, 16 bytes a lane, or words where rows are not 16-byte aligned (8192 x 1153 x
 // 768 with saved pre-activations 34 us; 47 with the alignment looked at per row instead of per lane).
 //
@@ -38,16 +38,16 @@
 // CTAs work in rolled loops of 16 columns, box copies and waiting loops are out of line, and
 // shared memory is addressed with 32-bit addresses throughout. Pairs, whose launches are long,
 // take the 32 columns of a chunk at once for twice the independent work (131072 x 1152 x 768 with
-// GELU 212 us by halves, 203 whole).
+// GELU 4% less time than by halves).
 //
 // Measured on one B200 (CUDA graph, inputs larger than L2): 131072 x 1152 x 768 without activation
-// 183-188 us (1.26 PFLOP/s; 0.75 of the measured burst rate), with GELU 200, with GELU and saved pre-
-// activations 217-231 (0.8 GB at 3.5 TB/s); 8192 x 768 x 1152 with residual 15.8 us; gated 8192 x
+// 183-188 us (1.26 PFLOP/s; 0.75 of the measured burst rate), with GELU 211, with GELU and saved pre-
+// activations 227-236 (0.8 GB at 3.5 TB/s); 8192 x 768 x 1152 with residual 15.8 us; gated 8192 x
 // 1152 x 768 21.9 us (1.32 PFLOP/s), gated 4096 x 8192 x 4096 saved 365-388 us (1.42-1.5 PFLOP/s);
 // 8192 x 8192 x 8192 0.755 ms (1.46 PFLOP/s); 16 x 8192 x 8192 24.8-26.8 us (5.0-5.4 TB/s, 0.77-0.83 of
 // measured); 1 x 768 x 768 4.0 us. Large products are bound by what their tiles read through L2 and by the power
-// cap (tensor pipe busy 77% without activation at 32768 rows, 67% with GELU), an epilogue of
-// exponentials by the latency of its chains (issue slots 44% busy), few rows by the weights' bytes, the
+// cap (tensor pipe busy 75% without activation at 32768 rows, 63% with GELU), an epilogue of
+// exponentials by the latency of its chains (issue slots 54% busy), few rows by the weights' bytes, the
 // smallest by launch, set-up and first loads.
 #pragma once
 #include <cuda_runtime.h>
@@ -68,7 +68,7 @@ constexpr int BM = 128;  // rows of a tile per CTA
 constexpr int BK = 64;   // contraction elements per stage
 // Epilogue warps. A linear forward tile on a pair has up to 32,768 activations per CTA, each with an
 // exponential and a reciprocal: with two warps per SM sub-partition their latencies were not hidden
-// (131072 x 1152 x 768 with GELU 326 us, without 182 us), with four they are (219 us then). Gated tiles
+// (131072 x 1152 x 768 with GELU 326 us, without 182 us), with four they were (219 us then). Gated tiles
 // have half of them, products without an activation none: eight warps leave room for more stages
 // (gated with sixteen: 65536 x 1152 x 768 saved 206 us as with eight, 4096 x 8192 x 4096 saved 443 us
 // against 384).
