@@ -505,7 +505,7 @@ J1_API j1_status j1_op_linear(const j1_linear_args* args, void* stream, int sync
  * dout); what is not read may be NULL. For the two products dp is kept in two parts of the dtype
  * (16 significant bits of BF16, 22 of FP16), both of its sign: an infinite x or w gives the infinity
  * that dp itself would. In FP16 both parts are scaled by a power of two of the call, which the
- * products' sums lose again before they are rounded; what is below 2^-38 of the largest finite dp is
+ * products' sums lose again before they are rounded; what is below 2^-37 of the largest finite dp is
  * lost. dbias sums the unrounded values. The residual's gradient is dout. M = 0 gives dw = 0, dbias = 0.
  * workspace: at least j1_op_linear_backward_workspace bytes, 256-byte aligned; its contents
  * need not survive between calls, and calls that may overlap on the GPU need one each. */

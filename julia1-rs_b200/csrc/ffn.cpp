@@ -309,27 +309,25 @@ Workspace workspace_for(int M, int N, int K, int projections) {
   return w;
 }
 
-// The sizes of a backward pass's products, in `parts` parts of the gradients at the pre-activations: dx (a gated
+// The sizes of a backward pass's products (parts: the gradients at the pre-activations are in two): dx (a gated
 // block's projections are two segments) and dw (their weights' rows are one product, the second's from pad32(N)).
-FfnGemm dx_product(int dtype, int M, int N, int K, int projections, int parts, const Workspace& ws, const FfnDevice* d) {
+FfnGemm dx_product(int dtype, int M, int N, int K, int projections, bool parts, const Workspace& ws, const FfnDevice* d) {
   FfnGemm g = gemm_for(dtype, FFN_NN, M, K, N, d);
   g.segs = projections;
-  g.lo = parts == 2 ? ws.lo : 0;
+  g.lo = parts ? ws.lo : 0;
   return g;
 }
-FfnGemm dw_product(int dtype, int M, int N, int K, int projections, int parts, const Workspace& ws, void* workspace, const FfnDevice* d) {
+FfnGemm dw_product(int dtype, int M, int N, int K, int projections, bool parts, const Workspace& ws, void* workspace, const FfnDevice* d) {
   FfnGemm g = gemm_for(dtype, FFN_TN, projections == 2 ? pad32(N) + N : N, K, M, d);
   if (projections == 2) {
     g.rows0 = N;
     g.row1 = pad32(N);
   }
-  g.lo = parts == 2 ? ws.lo : 0;
+  g.lo = parts ? ws.lo : 0;
   g.partials = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ws.partials);
   g.partial_bytes = ws.partial_bytes;
   return g;
 }
-// Gradients of a linear layer without activation or with ReLU are dout or 0.
-int parts_for(int act, int projections) { return projections == 1 && (act == J1_ACT_NONE || act == J1_ACT_RELU) ? 1 : 2; }
 
 j1_status workspace_query(int M, int N, int K, int projections, size_t* bytes) {
   if (!bytes) return bad("NULL argument");
@@ -491,12 +489,12 @@ j1_status j1_op_linear_backward(const j1_linear_grad_args* a, void* stream, int 
     const bool products = a->dx || a->dw;
     const bool copy = products && (slope || !ffn_rows16(dp));  // both products read it
     if (copy) dp = {base + ws.grads, ws.ld};
-    const int parts = parts_for(a->act, 1);
+    const bool parts = ffn_two_parts(false, a->act);
     FfnGemm gx = dx_product(a->dtype, a->M, a->N, a->K, 1, parts, ws, d);
     FfnGemm gw = dw_product(a->dtype, a->M, a->N, a->K, 1, parts, ws, base, d);
     FfnGrad k = {};
     Copies copies(st);
-    if (products && parts == 2 && a->dtype == J1_DTYPE_FP16)
+    if (products && parts && a->dtype == J1_DTYPE_FP16)
       gx.scale = gw.scale = k.scale = reinterpret_cast<float*>(base + ws.scale);
     if (a->dx) {
       gx.a[0] = dp;
@@ -583,7 +581,7 @@ j1_status j1_op_gated_backward(const j1_gated_grad_args* a, void* stream, int sy
     k.sum0 = a->dba;
     k.sum1 = a->dbg;
     k.partials = reinterpret_cast<float*>(base + ws.sums);
-    const int parts = parts_for(a->act, 2);
+    const bool parts = ffn_two_parts(true, a->act);
     FfnGemm gx = dx_product(a->dtype, a->M, a->N, a->K, 2, parts, ws, d);
     FfnGemm gw = dw_product(a->dtype, a->M, a->N, a->K, 2, parts, ws, base, d);
     gx.scale = gw.scale = k.scale;
@@ -621,7 +619,7 @@ j1_status j1_selftest_ffn_plan(int32_t product, int32_t act, int32_t M, int32_t 
     FfnDevice d;
     d.num_sms = num_sms;
     const Workspace ws = workspace_for(M, N, K, projections);
-    const int parts = parts_for(act, projections);
+    const bool parts = ffn_two_parts(projections == 2, act);
     FfnGemm g;
     if (product < 2) {
       g = gemm_for(J1_DTYPE_BF16, FFN_NT, M, N, K, &d);

@@ -6,6 +6,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "../../include/j1.h"
+
 namespace j1rt {
 
 // A row-major matrix of 16-bit elements: row r starts at p + r * ld elements.
@@ -75,6 +77,10 @@ struct FfnCopies {
 };
 int launch_ffn_copies(const FfnCopies& c, cudaStream_t stream);
 
+// Whether gradients at the pre-activations are kept in two parts. A linear layer's without activation or with ReLU
+// are dout or 0: one holds them.
+__host__ __device__ constexpr bool ffn_two_parts(bool gated, int act) { return gated || (act != J1_ACT_NONE && act != J1_ACT_RELU); }
+
 // dp = dout * act'(pre) (linear), or da = dout * g * act'(a), dg = dout * act(a) (gated): the
 // gradients at the pre-activations, rounded to the element type, with the column sums of the
 // unrounded values. d0 (and d1) may be NULL (sums only); sums may be NULL.
@@ -85,7 +91,7 @@ struct FfnGrad {
   FfnMat d0, d1;        // written: dp / da, dg
   float* sum0;          // [N] or NULL
   float* sum1;
-  long long lo;         // not 0: d0 and d1 are kept in two parts, the second goes lo elements behind the first
+  long long lo;         // in two parts: the second goes lo elements behind the first
   float* partials;      // ffn_grad_slabs(M, N) * 2 * N floats when a sum is wanted
   // FP16, NULL: as they are. d0 and d1 are multiplied by a power of two of the call that brings the
   // largest of their finite magnitudes to [2^14, 2^15); scale[0] receives its inverse, the rest is scratch.

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(GC, 4) max_kernel(const FfnGrad g, int col_blo
 
 // Gradients that are scaled before they are stored.
 template <typename T, bool GATED, int ACT>
-constexpr bool kScaled = std::is_same<T, __half>::value && (GATED || (ACT != J1_ACT_NONE && ACT != J1_ACT_RELU));
+constexpr bool kScaled = std::is_same<T, __half>::value && ffn_two_parts(GATED, ACT);
 
 template <typename T, bool GATED, int ACT, bool VEC>
 __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_rows, int maxima) {
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(GC, 3) grad_kernel(const FfnGrad g, int slab_r
       }
       auto store = [&](const FfnMat& m, const uint64_t(&v)[4]) {
         uint32_t w[4], left[4];
-        if (g.lo) {
+        if constexpr (ffn_two_parts(GATED, ACT)) {
           two_parts<T>(v, w, left);
           store8<VEC>({static_cast<const uint16_t*>(m.p) + g.lo, m.ld}, row, c0, lane, n, left);
         } else {
