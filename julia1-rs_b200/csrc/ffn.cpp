@@ -72,8 +72,24 @@ cudaError_t make_pool(int dev, cudaMemPool_t* pool) {
   return e;
 }
 
-// The first use of a device does all that a stream capture does not allow, or that would wait for the device:
-// kernels are loaded, whichever the calls will take, and the pool is made.
+// What the first use of a device prepares: kernels are loaded, whichever the calls will take, and the pool is made. A
+// capture under way (this thread's, or another's in the global mode) would forbid that, and end: it touches no stream, so the
+// thread takes the relaxed mode for it.
+cudaError_t first_use(int dev, int** err, int* sms, cudaMemPool_t* pool) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return e;
+  e = ffn_error_word(err);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = load_ffn_rows();
+  if (e == cudaSuccess) e = load_ffn_tc_bf16();
+  if (e == cudaSuccess) e = load_ffn_tc_fp16();
+  if (e == cudaSuccess) e = make_pool(dev, pool);
+  const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess && back != cudaSuccess) cudaMemPoolDestroy(*pool);
+  return e == cudaSuccess ? back : e;
+}
+
 j1_status device_state(FfnDevice** out, int* ordinal) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -86,13 +102,8 @@ j1_status device_state(FfnDevice** out, int* ordinal) {
     if (!s.ready.load(std::memory_order_relaxed)) {  // else another thread was first: its values are in use
       int* err = nullptr;
       int sms = 0;
-      cudaError_t rc = ffn_error_word(&err);
-      if (rc == cudaSuccess) rc = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-      if (rc == cudaSuccess) rc = load_ffn_rows();
-      if (rc == cudaSuccess) rc = load_ffn_tc_bf16();
-      if (rc == cudaSuccess) rc = load_ffn_tc_fp16();
       cudaMemPool_t pool = nullptr;
-      if (rc == cudaSuccess) rc = make_pool(dev, &pool);
+      const cudaError_t rc = first_use(dev, &err, &sms, &pool);
       if (rc != cudaSuccess) {
         cudaGetLastError();
         return cuda_error(rc, "first use of the device");

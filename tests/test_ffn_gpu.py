@@ -1038,3 +1038,15 @@ def test_captured_after_one_call(torch_cuda):
     path = os.path.dirname(os.path.dirname(os.path.abspath(j1.__file__)))
     r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST % path], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_first_call_in_a_capture(torch_cuda):
+    """The first call on a device may be in a capture itself: what it prepares is not part of the graph and does not end it."""
+    import os
+    import subprocess
+    import sys
+    path = os.path.dirname(os.path.dirname(os.path.abspath(j1.__file__)))
+    first = "j1.op_linear(none, wide, none)"
+    assert CAPTURED_FIRST.count(first) == 1
+    r = subprocess.run([sys.executable, "-c", CAPTURED_FIRST.replace(first, "pass") % path], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
