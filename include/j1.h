@@ -466,11 +466,11 @@ J1_API j1_status j1_op_attention_noalloc(const void* qkv, int64_t t, int32_t hid
  *
  * With sync = 0 the calls only enqueue work and may be captured into a CUDA graph. The first of them
  * on a device, whichever it is and in a capture too, loads every kernel: some milliseconds, which a
- * call with M = 0 takes ahead of time. Device-side timeouts of sync = 0 calls are reported by the next of these calls made with
- * sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Operands whose rows all start on 16-byte
- * boundaries are read in place and nothing is allocated; other operands of a product are copied
- * first, to stream-ordered memory of a pool of the library, which keeps the most it ever needed
- * at once. */
+ * call with M = 0 takes ahead of time. Device-side timeouts of sync = 0 calls are reported by the
+ * next of these calls made with sync = 1 on that device, as J1_ERR_DEVICE_TIMEOUT. Operands whose
+ * rows all start on 16-byte boundaries are read in place and nothing is allocated; other operands of
+ * a product are copied first, to stream-ordered memory of a pool of the library, which keeps the most
+ * it ever needed at once. */
 typedef enum j1_dtype { J1_DTYPE_BF16 = 0, J1_DTYPE_FP16 = 1 } j1_dtype;
 typedef enum j1_act {
   J1_ACT_NONE = 0,
